@@ -224,8 +224,9 @@ def _quantize(x):
     """f32 [rows, width] -> E4M3 values and scales amax / 448 [rows, blocks]."""
     b = _blocks(x)
     amax = b.abs().amax(-1).clamp_min(AMAX_FLOOR)
-    q = (b * (E4M3_MAX / amax)[..., None]).to(torch.float8_e4m3fn)
-    return q.view(x.shape[0], -1)[:, : x.shape[1]].contiguous(), amax / E4M3_MAX
+    top = torch.full_like(amax, E4M3_MAX)  # a quotient with a plain number would be a product with its reciprocal
+    q = (b * (top / amax)[..., None]).to(torch.float8_e4m3fn)
+    return q.view(x.shape[0], -1)[:, : x.shape[1]].contiguous(), amax / top
 
 
 def _dequantize(q, scale):
