@@ -343,6 +343,74 @@ int b200moe_fold_nvfp4_to_mxfp4(void* stream, const uint8_t* codes, const uint8_
                                 const float* global_scale, int rows, int k, uint8_t* out_codes,
                                 uint8_t* out_e8m0, uint32_t* err);
 
+/* ---- Operators of the FP8 expert path (no layer object, no counterpart in
+ * the reference, whose experts are FP4 and GGUF only and are never trained).
+ * They run on the current device, allocate nothing and never wait for the
+ * host.  A row or offset out of range is left out and sets a bit in the current
+ * device's operator error word, read and cleared (after `stream`) by
+ * b200moe_op_errors. */
+int b200moe_op_errors(void* stream, uint32_t* bits);
+
+/* Routes sorted by expert (stable; ids int32 [routes], routes = T * k <= 2^26,
+ * 1 <= num_experts <= 1024): row_of_route[route] = its row in that order, and
+ * offsets int32 [num_experts + 1] = where each expert's rows begin.  A route
+ * whose id is outside [0, num_experts) has no expert: it sorts last and gets
+ * ~row (negative); its row holds zeros and takes no part in sums.  workspace:
+ * b200moe_sort_workspace_bytes (0 up to 2048 routes). */
+size_t b200moe_sort_workspace_bytes(int routes, int num_experts);
+int b200moe_sort_routes(void* stream, const int32_t* ids, int routes, int num_experts, int32_t* row_of_route,
+                        int32_t* offsets, void* workspace, size_t workspace_bytes);
+
+/* rows[row_of_route[t * k + s]] = x[t]: row_bytes bytes of any type per token
+ * (x_stride bytes between tokens; rows [T * k][row_bytes]), and n_scale floats
+ * per token beside them (0: none). */
+int b200moe_permute_rows(void* stream, const void* x, int64_t x_stride, int64_t row_bytes, const float* scale,
+                         int64_t scale_stride, int n_scale, const int32_t* row_of_route, int T, int k, void* rows,
+                         float* row_scale);
+
+/* out[t] = sum over slots, in slot order, of fma(weights[t][s], rows[row], sum)
+ * in f32 (weights NULL: 1), rounded once; out_dtype is dtype or F32.  With
+ * weights NULL it is also the gradient of b200moe_permute_rows. */
+int b200moe_unpermute(void* stream, const void* rows, int dtype, const int32_t* row_of_route, const float* weights,
+                      int T, int k, int H, void* out, int out_dtype);
+
+/* Its gradients: grad_rows[row] = weights[t][s] * grad[t] (zeros in the row of a
+ * route without an expert), grad_weights[t][s] = <grad[t], rows[row]> in f32.
+ * Either may be NULL.  grad: dtype or F32, grad_stride elements between tokens. */
+int b200moe_unpermute_grad(void* stream, const void* grad, int grad_dtype, int64_t grad_stride, const void* rows,
+                           int dtype, const int32_t* row_of_route, const float* weights, int T, int k, int H,
+                           void* grad_rows, float* grad_weights);
+
+/* Rows to E4M3 with a scale per 128 columns: amax = max(max |x|, 1e-30),
+ * scale = amax / 448, q = e4m3(x * (448 / amax)), every step in f32.  x
+ * [rows][width] (swiglu: [rows][2 width], gate then up columns, quantizing
+ * min(g, limit) / (1 + e^-min(g, limit)) * clamp(u, +-limit)); q [rows][width],
+ * scale [rows][ceil(width / 128)].  A NaN or an infinity makes its block NaN. */
+int b200moe_fp8_quantize(void* stream, const void* x, int dtype, int64_t x_stride, int rows, int width, int swiglu,
+                         float limit, void* q, float* scale);
+/* Gradient of that SwiGLU: grad [rows][width] -> grad_h [rows][2 width] (zero where a bound cut the value). */
+int b200moe_swiglu_grad(void* stream, const void* h, int dtype, int64_t h_stride, const void* grad,
+                        int64_t grad_stride, int rows, int width, float limit, void* grad_h);
+/* Weights w [mats][n][k] to E4M3 with a scale per 128 x 128 block
+ * [mats][ceil(n / 128)][ceil(k / 128)], and the transpose of packed weights. */
+int b200moe_fp8_quantize_weight(void* stream, const void* w, int dtype, int mats, int n, int k, void* q, float* scale);
+int b200moe_fp8_transpose_weight(void* stream, const void* w, const float* scale, int mats, int n, int k, void* out,
+                                 float* out_scale);
+
+/* out [S][N] = a . w^T with the blocks' scales, f32 sums: a [S][K] E4M3 with
+ * a_scale [S][ceil(K / 128)] (a_scale_stride floats between rows), w [E][N][K]
+ * E4M3 with w_scale [E][ceil(N / 128)][ceil(K / 128)].  offsets (device, int32
+ * [E + 1]): rows offsets[e] .. offsets[e + 1] use w[e], rows from offsets[E] on
+ * become zeros; NULL: E is 1.  K a multiple of 16, a and w on 16-byte
+ * addresses, E <= 1024. */
+int b200moe_fp8_matmul(void* stream, const void* a, const float* a_scale, int64_t a_scale_stride, const void* w,
+                       const float* w_scale, const int32_t* offsets, int S, int N, int K, int E, void* out,
+                       int out_dtype);
+/* The same for one matrix and S <= 8 rows of f16 or bf16 (ldx elements between
+ * them, a multiple of 8; x on a 16-byte address), quantized inside the kernel. */
+int b200moe_fp8_linear(void* stream, const void* x, int x_dtype, int64_t ldx, const void* w, const float* w_scale,
+                       int S, int N, int K, void* out, int out_dtype);
+
 #ifdef __cplusplus
 }
 #endif

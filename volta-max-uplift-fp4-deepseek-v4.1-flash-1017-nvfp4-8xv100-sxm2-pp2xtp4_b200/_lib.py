@@ -21,6 +21,8 @@ PIN_PATH = HERE / "libb200moe.so.sha256"
 
 P = ctypes.c_void_p
 I32 = ctypes.c_int
+I64 = ctypes.c_int64
+SIZE = ctypes.c_size_t
 F32 = ctypes.c_float
 
 STATUS = {
@@ -92,6 +94,18 @@ SIGNATURES = {
     "b200moe_ep_received": ([P, P, P, P, I32], I32),
     "b200moe_forward_rows": ([P, P, P, P, P, P, I32, P], I32),
     "b200moe_f32_to_f16": ([P, P, ctypes.c_int64, P], I32),
+    "b200moe_op_errors": ([P, ctypes.POINTER(ctypes.c_uint32)], I32),
+    "b200moe_sort_workspace_bytes": ([I32, I32], SIZE),
+    "b200moe_sort_routes": ([P, P, I32, I32, P, P, P, SIZE], I32),
+    "b200moe_permute_rows": ([P, P, I64, I64, P, I64, I32, P, I32, I32, P, P], I32),
+    "b200moe_unpermute": ([P, P, I32, P, P, I32, I32, I32, P, I32], I32),
+    "b200moe_unpermute_grad": ([P, P, I32, I64, P, I32, P, P, I32, I32, I32, P, P], I32),
+    "b200moe_fp8_quantize": ([P, P, I32, I64, I32, I32, I32, F32, P, P], I32),
+    "b200moe_swiglu_grad": ([P, P, I32, I64, P, I64, I32, I32, F32, P], I32),
+    "b200moe_fp8_quantize_weight": ([P, P, I32, I32, I32, I32, P, P], I32),
+    "b200moe_fp8_transpose_weight": ([P, P, P, I32, I32, I32, P, P], I32),
+    "b200moe_fp8_matmul": ([P, P, P, I64, P, P, P, I32, I32, I32, I32, P, I32], I32),
+    "b200moe_fp8_linear": ([P, P, I32, I64, P, P, I32, I32, I32, P, I32], I32),
     "b200moe_mma_peak": ([I32, I32, I32, ctypes.POINTER(F32), ctypes.POINTER(F32)], I32),
 }
 

@@ -292,4 +292,8 @@ struct TcArgs {
 };
 int launch_tc_gemm(cudaStream_t s, int fmt, int epi, const TcArgs& a, const void* map, int grid);
 
+// ---- stateless operators (ops.cu): the current device's error word and SM count
+uint32_t* op_error_word();
+int sm_count();
+
 }  // namespace b200moe
