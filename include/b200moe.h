@@ -361,16 +361,17 @@ size_t b200moe_sort_workspace_bytes(int routes, int num_experts);
 int b200moe_sort_routes(void* stream, const int32_t* ids, int routes, int num_experts, int32_t* row_of_route,
                         int32_t* offsets, void* workspace, size_t workspace_bytes);
 
-/* rows[row_of_route[t * k + s]] = x[t]: row_bytes bytes of any type per token
- * (x_stride bytes between tokens; rows [T * k][row_bytes]), and n_scale floats
- * per token beside them (0: none). */
-int b200moe_permute_rows(void* stream, const void* x, int64_t x_stride, int64_t row_bytes, const float* scale,
-                         int64_t scale_stride, int n_scale, const int32_t* row_of_route, int T, int k, void* rows,
-                         float* row_scale);
+/* The sort (T * k routes) and the copies rows[row_of_route[t * k + s]] = x[t]:
+ * row_bytes bytes of any type per token (x_stride bytes between tokens; rows
+ * [T * k][row_bytes]), and n_scale floats per token beside them (0: none). */
+int b200moe_permute(void* stream, const int32_t* ids, int num_experts, const void* x, int64_t x_stride,
+                    int64_t row_bytes, const float* scale, int64_t scale_stride, int n_scale, int T, int k,
+                    int32_t* row_of_route, int32_t* offsets, void* rows, float* row_scale, void* workspace,
+                    size_t workspace_bytes);
 
 /* out[t] = sum over slots, in slot order, of fma(weights[t][s], rows[row], sum)
  * in f32 (weights NULL: 1), rounded once; out_dtype is dtype or F32.  With
- * weights NULL it is also the gradient of b200moe_permute_rows. */
+ * weights NULL it is also the gradient of b200moe_permute. */
 int b200moe_unpermute(void* stream, const void* rows, int dtype, const int32_t* row_of_route, const float* weights,
                       int T, int k, int H, void* out, int out_dtype);
 
@@ -406,10 +407,14 @@ int b200moe_fp8_transpose_weight(void* stream, const void* w, const float* scale
 int b200moe_fp8_matmul(void* stream, const void* a, const float* a_scale, int64_t a_scale_stride, const void* w,
                        const float* w_scale, const int32_t* offsets, int S, int N, int K, int E, void* out,
                        int out_dtype);
-/* The same for one matrix and S <= 8 rows of f16 or bf16 (ldx elements between
- * them, a multiple of 8; x on a 16-byte address), quantized inside the kernel. */
+/* The same for one matrix and rows x of f16, bf16 or f32 (ldx elements between
+ * them), quantized in the call: inside the product's kernel for up to 8 rows of
+ * 16 bits on 16-byte addresses, else into the workspace
+ * (b200moe_fp8_linear_workspace_bytes, on a 16-byte address; the 0 it gives for
+ * few rows holds for such x only, S * (K + 4 ceil(K / 128)) + 16 always suffices). */
+size_t b200moe_fp8_linear_workspace_bytes(int S, int N, int K);
 int b200moe_fp8_linear(void* stream, const void* x, int x_dtype, int64_t ldx, const void* w, const float* w_scale,
-                       int S, int N, int K, void* out, int out_dtype);
+                       int S, int N, int K, void* out, int out_dtype, void* workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

@@ -97,7 +97,7 @@ SIGNATURES = {
     "b200moe_op_errors": ([P, ctypes.POINTER(ctypes.c_uint32)], I32),
     "b200moe_sort_workspace_bytes": ([I32, I32], SIZE),
     "b200moe_sort_routes": ([P, P, I32, I32, P, P, P, SIZE], I32),
-    "b200moe_permute_rows": ([P, P, I64, I64, P, I64, I32, P, I32, I32, P, P], I32),
+    "b200moe_permute": ([P, P, I32, P, I64, I64, P, I64, I32, I32, I32, P, P, P, P, P, SIZE], I32),
     "b200moe_unpermute": ([P, P, I32, P, P, I32, I32, I32, P, I32], I32),
     "b200moe_unpermute_grad": ([P, P, I32, I64, P, I32, P, P, I32, I32, I32, P, P], I32),
     "b200moe_fp8_quantize": ([P, P, I32, I64, I32, I32, I32, F32, P, P], I32),
@@ -105,7 +105,8 @@ SIGNATURES = {
     "b200moe_fp8_quantize_weight": ([P, P, I32, I32, I32, I32, P, P], I32),
     "b200moe_fp8_transpose_weight": ([P, P, P, I32, I32, I32, P, P], I32),
     "b200moe_fp8_matmul": ([P, P, P, I64, P, P, P, I32, I32, I32, I32, P, I32], I32),
-    "b200moe_fp8_linear": ([P, P, I32, I64, P, P, I32, I32, I32, P, I32], I32),
+    "b200moe_fp8_linear_workspace_bytes": ([I32, I32, I32], SIZE),
+    "b200moe_fp8_linear": ([P, P, I32, I64, P, P, I32, I32, I32, P, I32, P, SIZE], I32),
     "b200moe_mma_peak": ([I32, I32, I32, ctypes.POINTER(F32), ctypes.POINTER(F32)], I32),
 }
 

@@ -47,7 +47,16 @@ __device__ __forceinline__ uint32_t e4m3x4(float v0, float v1, float v2, float v
 __device__ __forceinline__ void build_tile_table(const int32_t* __restrict__ offsets, int E, int n_rows,
                                                  int rows_per_tile, int per_row_tile, int* off, int* start,
                                                  uint32_t* err) {
-  for (int e = threadIdx.x; e <= E; e += blockDim.x) off[e] = offsets ? offsets[e] : (e ? n_rows : 0);
+  if (!offsets) {  // one matrix, all rows
+    if (threadIdx.x == 0) {
+      off[0] = start[0] = 0;
+      off[1] = n_rows;
+      start[1] = (n_rows + rows_per_tile - 1) / rows_per_tile * per_row_tile;
+    }
+    __syncthreads();
+    return;
+  }
+  for (int e = threadIdx.x; e <= E; e += blockDim.x) off[e] = offsets[e];
   __syncthreads();
   if (threadIdx.x < 32) {
     int carry = 0;

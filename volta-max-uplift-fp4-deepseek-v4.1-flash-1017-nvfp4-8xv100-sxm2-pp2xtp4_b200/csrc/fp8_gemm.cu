@@ -9,7 +9,7 @@
 //     128-byte swizzle) into a ring of stages;
 //   warp 1 (MMA): one thread issues 4 x tcgen05.mma.kind::f8f6f4 (M 128, N BN,
 //     K 32) into one of the TMEM buffers of BN columns and commits;
-//   warps 2-9 (sums): read the block's product (a thread holds one row and half
+//   warps 4-11 (sums): read the block's product (a thread holds one row and half
 //     the columns, so both scales are one factor per thread and block) and add
 //     factor * product to f32 sums in registers, two columns per instruction,
 //     while the tensor core fills the next buffer.
@@ -26,6 +26,7 @@
 
 #include "fp8_device.cuh"
 #include "fp8_ops.h"
+#include "fp8_tc.cuh"
 #include "internal.h"
 
 namespace b200moe {
@@ -33,10 +34,14 @@ namespace {
 
 constexpr int kBM = 128;
 constexpr int kSumWarps = 8;
-constexpr int kThreads = (2 + kSumWarps) * 32;
+constexpr int kSumWarp0 = 4;  // warps 0-3: producer, MMA, two without work (a register share is a group of four)
+constexpr int kThreads = (kSumWarp0 + kSumWarps) * 32;
+// registers per thread: the launch's 384 x 168 split as 128 x 40 + 256 x 232
+constexpr int kFewRegs = 40, kSumRegs = 232;
 constexpr int kMaxExperts = 1024;
 constexpr int kABytes = kBM * kFp8Block;
 constexpr int kOutBytes = 32 * 64;  // per sum warp: 32 rows in pieces of 64 bytes
+constexpr int kAhead = 4;           // K blocks whose scales are loaded ahead of their sums
 
 template <int BN>
 struct Cfg {
@@ -48,58 +53,6 @@ struct Cfg {
   static constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
   static_assert(kSmem + 8 * (kMaxExperts + 1) + 64 <= 227 * 1024, "shared memory, with the tile table");
 };
-
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
-  // K-major, 128-byte swizzle: rows of 128 bytes, 8-row atoms 1024 bytes apart
-  return uint64_t((addr >> 4) & 0x3FFF) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
-         (uint64_t(2) << 61);
-}
-
-__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p; }" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
-}
-
-__device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-
-// 16 columns of this thread's TMEM lane; the values are there after tmem_wait on the same array.
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr));
-}
-// The registers pass through the wait, so no use of them can move above it.
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
-}
-
-// acc += s * p for two columns at once (each an f32 fma)
-__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t p0, uint32_t p1, uint64_t s2) {
-  uint64_t p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "r"(p0), "r"(p1));
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(p), "l"(s2));
-}
 
 struct GemmArgs {
   const float* a_scale;  // [S][KB], row stride lda_s
@@ -132,7 +85,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* acc_empty = acc_full + NBUF;
   volatile int* abort_ptr = &abort_flag;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(&full[s], 1);
@@ -159,65 +112,69 @@ __global__ void __launch_bounds__(kThreads, 1)
   build_tile_table(a.offsets, a.E, a.S, kBM, n_nt, off, start, a.err);
   const int n_items = start[a.E];
 
-  if (warp == 0) {
-    if (lane == 0) {
-      uint32_t g = 0, issued = 0, par = 0;
-      for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+  if (warp < kSumWarp0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+    // whole warps run these loops (values stay uniform); one elected lane issues
+    if (warp == 0) {
+      int st = 0;
+      uint32_t ph = 0, issued = 0, par = 0;
+      bool ok = true;
+      for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x) {
         const int e = tile_expert(start, a.E, item), local = item - start[e];
         const int row = off[e] + local / n_nt * kBM, wrow = e * a.N + local % n_nt * BN;
-        for (int kb = 0; kb < a.KB; ++kb, ++g) {
-          const int s = g % ST;
-          const uint32_t ph = (g / ST) & 1u;
-          if (*abort_ptr || !mbar_wait(&empty[s], ph ^ 1u, a.err)) {
-            *abort_ptr = 1;
-            break;
+        for (int kb = 0; kb < a.KB; ++kb) {
+          ok = __all_sync(0xffffffffu, !*abort_ptr && mbar_wait(&empty[st], ph ^ 1u, a.err));
+          if (!ok) break;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&full[st], uint32_t(kABytes + C::kWBytes));
+            tma_2d(at + st * kABytes, &map_a, kb * kFp8Block, row, &full[st]);
+            tma_2d(wt + st * C::kWBytes, &map_w, kb * kFp8Block, wrow, &full[st]);
           }
-          mbar_arrive_expect_tx(&full[s], uint32_t(kABytes + C::kWBytes));
-          tma_2d(at + s * kABytes, &map_a, kb * kFp8Block, row, &full[s]);
-          tma_2d(wt + s * C::kWBytes, &map_w, kb * kFp8Block, wrow, &full[s]);
-          issued |= 1u << s;
-          par = (par & ~(1u << s)) | (ph << s);
+          issued |= 1u << st;
+          par = (par & ~(1u << st)) | (ph << st);
+          if (++st == ST) st = 0, ph ^= 1u;
         }
-        if (*abort_ptr) break;
       }
+      if (!ok) *abort_ptr = 1;
       // no copy may be in flight when the CTA exits
       for (int s = 0; s < ST; ++s)
         if (issued & (1u << s)) mbar_wait(&full[s], (par >> s) & 1u, a.err);
     }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      uint32_t g = 0;
+    if (warp == 1) {
+      int st = 0, b = 0, last = 0;
+      uint32_t ph = 0, bph = 0, last_ph = 0;
       bool ok = true, committed = false;
-      int last_b = 0;
-      uint32_t last_ph = 0;
+      const uint64_t da0 = desc_sw128(smem_u32(at)), dw0 = desc_sw128(smem_u32(wt));
       for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x) {
-        for (int kb = 0; kb < a.KB; ++kb, ++g) {
-          const int s = g % ST, b = g % NBUF;
-          const uint32_t ph = (g / ST) & 1u, bph = (g / NBUF) & 1u;
-          if (*abort_ptr || !mbar_wait(&acc_empty[b], bph ^ 1u, a.err) || !mbar_wait(&full[s], ph, a.err)) {
-            *abort_ptr = 1;
-            ok = false;
-            break;
-          }
+        for (int kb = 0; kb < a.KB; ++kb) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[b], bph ^ 1u, a.err) && mbar_wait(&full[st], ph, a.err));
+          if (!ok) break;
           fence_after();
-          const uint64_t da = desc_sw128(smem_u32(at + s * kABytes)), dw = desc_sw128(smem_u32(wt + s * C::kWBytes));
-#pragma unroll
-          for (int k = 0; k < 4; ++k)  // 32 columns = 32 bytes of the swizzled row each
-            mma_f8(tmem + b * BN, da + 2 * k, dw + 2 * k, C::kIdesc, k != 0);
-          commit(&empty[s]);
-          commit(&acc_full[b]);
+          const uint64_t da = da0 + st * (kABytes >> 4), dw = dw0 + st * (C::kWBytes >> 4);
+          if (elect_one()) {
+            mma_block(tmem + b * BN, da, dw, C::kIdesc);
+            commit(&empty[st]);
+            commit(&acc_full[b]);
+          }
+          __syncwarp();
           committed = true;
-          last_b = b;
+          last = b;
           last_ph = bph;
+          if (++st == ST) st = 0, ph ^= 1u;
+          if (++b == NBUF) b = 0, bph ^= 1u;
         }
       }
-      if (committed) mbar_wait(&acc_full[last_b], last_ph, a.err);
+      if (!ok) *abort_ptr = 1;
+      if (committed) mbar_wait(&acc_full[last], last_ph, a.err);
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
     // a warp may read the TMEM lanes 32 (warp % 4) ..; the two warps of a quarter split the columns
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* mine = stage_out + (warp - 2) * kOutBytes;
-    uint32_t g = 0;
+    const int quarter = warp & 3, half = (warp - kSumWarp0) >> 2;
+    uint8_t* mine = stage_out + (warp - kSumWarp0) * kOutBytes;
+    const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16) + half * COLS;
+    int b = 0;
+    uint32_t bph = 0;
     bool ok = true;
     for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x) {
       const int e = tile_expert(start, a.E, item), local = item - start[e];
@@ -226,36 +183,41 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int nb = min(col0 / kFp8Block, a.NB - 1);
       const float* sa = a.a_scale + int64_t(min(row0 + lane, a.S - 1)) * a.lda_s;
       const float* sb = a.w_scale + (int64_t(e) * a.NB + nb) * a.KB;
-      uint64_t acc[COLS / 2];
+      float acc[COLS];
 #pragma unroll
-      for (int i = 0; i < COLS / 2; ++i) acc[i] = 0;
-      float sa_next = __ldg(sa), sb_next = __ldg(sb);
-      for (int kb = 0; kb < a.KB; ++kb, ++g) {
-        const float f = sa_next * sb_next;
-        if (kb + 1 < a.KB) {
-          sa_next = __ldg(sa + kb + 1);
-          sb_next = __ldg(sb + kb + 1);
+      for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
+      float fa[kAhead], fb[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        fa[j] = __ldg(sa + min(j, a.KB - 1));
+        fb[j] = __ldg(sb + min(j, a.KB - 1));
+      }
+      for (int kb0 = 0; ok && kb0 < a.KB; kb0 += kAhead) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const int kb = kb0 + j;
+          if (kb >= a.KB) break;
+          const float f = fa[j] * fb[j];
+          const int ahead = min(kb + kAhead, a.KB - 1);
+          fa[j] = __ldg(sa + ahead);
+          fb[j] = __ldg(sb + ahead);
+          ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[b], bph, a.err));
+          if (!ok) break;
+          fence_after();
+          const uint32_t addr = lanes + b * BN;
+          uint32_t p[32];
+#pragma unroll
+          for (int c = 0; c < COLS / 32; ++c) {
+            tmem_ld32(addr + c * 32, p);
+            tmem_wait(p);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(p[i]), f, acc[c * 32 + i]);
+          }
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[b]);
+          if (++b == NBUF) b = 0, bph ^= 1u;
         }
-        uint64_t f2;
-        asm("mov.b64 %0, {%1, %1};" : "=l"(f2) : "r"(__float_as_uint(f)));
-        const int b = g % NBUF;
-        ok = !*abort_ptr && mbar_wait(&acc_full[b], (g / NBUF) & 1u, a.err);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        fence_after();
-        const uint32_t addr = tmem + (uint32_t(quarter * 32) << 16) + b * BN + half * COLS;
-        uint32_t p[2][16];
-        tmem_ld16(addr, p[0]);
-#pragma unroll
-        for (int c = 0; c < COLS / 16; ++c) {
-          tmem_wait(p[c & 1]);
-          if (c + 1 < COLS / 16) tmem_ld16(addr + (c + 1) * 16, p[(c + 1) & 1]);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) fma2(acc[c * 8 + i], p[c & 1][2 * i], p[c & 1][2 * i + 1], f2);
-        }
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[b]);
       }
       if (!ok) {
         *abort_ptr = 1;
@@ -272,11 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int ch = 0; ch < 4; ++ch) {
           float v[CW];
 #pragma unroll
-          for (int i = 0; i < CW / 2; ++i) {
-            const uint64_t u = acc[(pc * PW + ch * CW) / 2 + i];
-            v[2 * i] = __uint_as_float(uint32_t(u));
-            v[2 * i + 1] = __uint_as_float(uint32_t(u >> 32));
-          }
+          for (int i = 0; i < CW; ++i) v[i] = acc[pc * PW + ch * CW + i];
           store_vec<TO, CW>(reinterpret_cast<TO*>(mine + lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4)), v);
         }
         __syncwarp();
@@ -298,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
     }
-    if (a.offsets) zero_rows(static_cast<TO*>(a.out), a.N, off[a.E], a.S, threadIdx.x - 64, kSumWarps * 32);
+    if (a.offsets) zero_rows(static_cast<TO*>(a.out), a.N, off[a.E], a.S, threadIdx.x - kSumWarp0 * 32, kSumWarps * 32);
   }
   fence_before();
   __syncthreads();
@@ -373,6 +331,25 @@ int product_status(const Fp8Product& p, int out_dtype) {
   return B200MOE_OK;
 }
 
+// The kernel by rows per matrix, as measured on B200 (us; kernels of 8, 16, 32 and 128 rows per tile):
+//   one matrix 4096 x 4096: 6.8 / 11.5 / 12.4 / 14.2 at 1 row, - / 11.9 / 13.0 / 14.5 at 32, - / 12.1 / 13.1 / 14.5
+//   at 64, - / 20.9 / 13.2 / 14.6 at 96, - / 29.7 / 23.1 / 15.4 at 192: a tile of fewer rows gives more CTAs, so the
+//   smallest whose tiles still run in one wave;
+//   64 matrices 2816 x 2048: - / 67 / 64 / 71 at 8 rows each, - / 104 / 66 / 73 at 24, - / 112 / 91 / 74 at 32, where
+//   experts above 32 rows read their weights twice.
+// Returns 8, 16, 32 or 128.
+int choose(const Fp8Product& p) {
+  if (!p.offsets) {
+    const int64_t n_tiles = (p.N + 127) / 128;
+    if (fp8_skinny_fits(p) && int64_t(p.N) * p.K <= (48 << 20)) return 8;
+    for (int t = 16; t <= 32; t *= 2)
+      if ((p.S + t - 1) / t * n_tiles <= sm_count() && fp8_stream_fits(p.K, t)) return t;
+    // more columns than one wave holds, bound by their bytes as long as one tile has all rows
+    return p.S <= 32 && fp8_stream_fits(p.K, 32) ? 32 : 128;
+  }
+  return p.S <= 24 * int64_t(p.E) && fp8_stream_fits(p.K, 32) ? 32 : 128;
+}
+
 int launch_status(int rc) {
   if (rc == 0) return B200MOE_OK;
   cudaGetLastError();
@@ -380,6 +357,13 @@ int launch_status(int rc) {
 }
 
 }  // namespace
+
+static int run_product(cudaStream_t s, const Fp8Product& p, int out_dtype) {
+  const int kind = choose(p);
+  return launch_status(kind == 8     ? launch_fp8_skinny(s, p, out_dtype)
+                       : kind == 128 ? launch_fp8_gemm(s, p, out_dtype)
+                                     : launch_fp8_stream(s, p, kind, out_dtype));
+}
 
 extern "C" int b200moe_fp8_matmul(void* stream, const void* a, const float* a_scale, int64_t a_scale_stride,
                                   const void* w, const float* w_scale, const int32_t* offsets, int S, int N, int K,
@@ -389,20 +373,36 @@ extern "C" int b200moe_fp8_matmul(void* stream, const void* a, const float* a_sc
   if (st) return st;
   if (!a || !a_scale || a_scale_stride < 0) return B200MOE_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(a) % 16) return B200MOE_ERR_ALIGN;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (S <= 8 * int64_t(E)) return launch_status(launch_fp8_skinny(s, p, 8, out_dtype));
-  if (S <= 16 * int64_t(E)) return launch_status(launch_fp8_skinny(s, p, 16, out_dtype));
-  return launch_status(launch_fp8_gemm(s, p, out_dtype));
+  return run_product(static_cast<cudaStream_t>(stream), p, out_dtype);
+}
+
+extern "C" size_t b200moe_fp8_linear_workspace_bytes(int S, int N, int K) {
+  const Fp8Product p{nullptr, nullptr, 0, nullptr, nullptr, nullptr, nullptr, S, N, K, 1};
+  if (S < 1 || N < 1 || K < 1 || choose(p) == 8) return 0;
+  const size_t q = (size_t(S) * K + 15) / 16 * 16;
+  return q + size_t(S) * ((K + kFp8Block - 1) / kFp8Block) * sizeof(float);
 }
 
 extern "C" int b200moe_fp8_linear(void* stream, const void* x, int x_dtype, int64_t ldx, const void* w,
-                                  const float* w_scale, int S, int N, int K, void* out, int out_dtype) {
-  const Fp8Product p{nullptr, nullptr, 0, w, w_scale, nullptr, out, S, N, K, 1};
+                                  const float* w_scale, int S, int N, int K, void* out, int out_dtype, void* workspace,
+                                  size_t workspace_bytes) {
+  Fp8Product p{nullptr, nullptr, 0, w, w_scale, nullptr, out, S, N, K, 1};
   const int st = product_status(p, out_dtype);
   if (st) return st;
-  if (!x || ldx < 0 || S > 8) return B200MOE_ERR_INVALID_ARG;
-  if (x_dtype != B200MOE_F16 && x_dtype != B200MOE_BF16) return B200MOE_ERR_DTYPE;
-  if (reinterpret_cast<uintptr_t>(x) % 16 || ldx % 8) return B200MOE_ERR_ALIGN;
-  return launch_status(
-      launch_fp8_skinny_x(static_cast<cudaStream_t>(stream), p, x, x_dtype, ldx, out_dtype));
+  if (!x || ldx < 0) return B200MOE_ERR_INVALID_ARG;
+  if (x_dtype < 0 || x_dtype > B200MOE_F32) return B200MOE_ERR_DTYPE;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t ld_bytes = ldx * (x_dtype == B200MOE_F32 ? 4 : 2);
+  if (choose(p) == 8 && x_dtype != B200MOE_F32 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_bytes % 16 == 0)
+    return launch_status(launch_fp8_skinny_x(s, p, x, x_dtype, ldx, out_dtype));
+  const size_t q_bytes = (size_t(S) * K + 15) / 16 * 16, kb = (K + kFp8Block - 1) / kFp8Block;
+  if (!workspace || workspace_bytes < q_bytes + size_t(S) * kb * sizeof(float)) return B200MOE_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return B200MOE_ERR_ALIGN;
+  float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + q_bytes);
+  const int qs = b200moe_fp8_quantize(stream, x, x_dtype, ldx, S, K, 0, 1.f, workspace, scale);
+  if (qs) return qs;
+  p.a = workspace;
+  p.a_scale = scale;
+  p.a_scale_stride = int64_t(kb);
+  return run_product(s, p, out_dtype);
 }

@@ -22,9 +22,14 @@ struct Fp8Product {
 
 // tcgen05 kernel (fp8_gemm.cu): tiles of 128 rows
 int launch_fp8_gemm(cudaStream_t s, const Fp8Product& p, int out_dtype);
-// streaming kernel for few rows per matrix (fp8_skinny.cu): tiles of 8, 16 or 32 rows
-int launch_fp8_skinny(cudaStream_t s, const Fp8Product& p, int rows_per_tile, int out_dtype);
-// the same for one matrix and S <= 8 rows of f16 or bf16 (x [S][K], row stride ldx), quantized in the kernel
+// tcgen05 kernel for few rows per matrix, the weights as the MMA's M (fp8_stream.cu): tiles of 16 or 32 rows
+int launch_fp8_stream(cudaStream_t s, const Fp8Product& p, int rows_per_tile, int out_dtype);
+// whether a tile's row scales fit in its shared memory
+bool fp8_stream_fits(int K, int rows_per_tile);
+// kernel for one matrix and at most eight rows (fp8_skinny.cu)
+int launch_fp8_skinny(cudaStream_t s, const Fp8Product& p, int out_dtype);
+// the same on rows of f16 or bf16 (x [S][K], row stride ldx), quantized in the kernel
 int launch_fp8_skinny_x(cudaStream_t s, const Fp8Product& p, const void* x, int x_dtype, int64_t ldx, int out_dtype);
+bool fp8_skinny_fits(const Fp8Product& p);
 
 }  // namespace b200moe

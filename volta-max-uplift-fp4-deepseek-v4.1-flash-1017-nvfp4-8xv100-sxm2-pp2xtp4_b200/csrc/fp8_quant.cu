@@ -17,13 +17,56 @@ namespace {
 
 constexpr int kQuantThreads = 256;
 
+// Minimum / maximum that keep a NaN.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float o;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(o) : "f"(a), "f"(b));
+  return o;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float o;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(o) : "f"(a), "f"(b));
+  return o;
+}
+
+// 1 + e^-g, at most 1e38 so that the quotients below stay finite (g / y is below E4M3's reach of the amax floor there).
+__device__ __forceinline__ float one_plus_exp_neg(float g) { return min_nan(1.f + expf(-g), 1e38f); }
+
+// x / y for y in [1, 1e38]: the hardware reciprocal and one Newton step on the quotient's remainder. Within an ulp or
+// two of the quotient, for five instructions: an IEEE division's dozen, with its branch, bounded these kernels.
+__device__ __forceinline__ float quotient(float x, float y) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(y));
+  const float q = x * r;
+  return fmaf(fmaf(-q, y, x), r, q);
+}
+
 // Limited SwiGLU (the framework's): g = min(gate, limit), u = clamp(up, +-limit), g / (1 + e^-g) * u.
 __device__ __forceinline__ float swiglu(float g, float u, float limit) {
-  g = g > limit ? limit : g;
-  u = u > limit ? limit : u;
-  u = u < -limit ? -limit : u;
-  return __fmul_rn(__fdiv_rn(g, __fadd_rn(1.f, expf(-g))), u);
+  g = min_nan(g, limit);
+  u = max_nan(min_nan(u, limit), -limit);
+  return quotient(g, one_plus_exp_neg(g)) * u;
 }
+
+// Position (row, block) of a walk over rows x blocks in steps, without a division per step.
+struct Walk {
+  int64_t row, d_row;
+  int b, d_b, n_b;
+  __device__ __forceinline__ Walk(int64_t first, int64_t step, int blocks) : n_b(blocks) {
+    row = first / blocks;
+    b = int(first - row * blocks);
+    d_row = step / blocks;
+    d_b = int(step - d_row * blocks);
+  }
+  __device__ __forceinline__ void next() {
+    row += d_row;
+    b += d_b;
+    if (b >= n_b) {
+      b -= n_b;
+      ++row;
+    }
+  }
+};
 
 // Eight values from p, those at or past `left` zero.
 template <typename T, bool WIDE>
@@ -41,49 +84,58 @@ __device__ __forceinline__ void load8(const T* p, int64_t left, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] = !WIDE && i < left ? to_f32(p[i]) : 0.f;
 }
 
+// Half a warp per block; two blocks (SwiGLU) or four in flight before the first is worked on.
 template <typename T, bool SWIGLU, bool WIDE>
 __global__ void __launch_bounds__(kQuantThreads) fp8_rows_kernel(const T* __restrict__ x, int64_t x_stride, int rows,
                                                                  int width, float limit, uint8_t* __restrict__ q,
                                                                  float* __restrict__ scale) {
+  constexpr int U = (SWIGLU ? 2 : 4) / (sizeof(T) == 4 ? 2 : 1);
   const int nb = (width + kFp8Block - 1) / kFp8Block, l = threadIdx.x & 15;
-  const int64_t groups = int64_t(rows) * nb, step = int64_t(gridDim.x) * (kQuantThreads / 16);
+  const int64_t step = int64_t(gridDim.x) * (kQuantThreads / 16);
   pdl_wait();
   pdl_trigger();
-  // both halves of a warp take the same number of turns: the shuffles want every lane
-  const int64_t turns = (groups + step - 1) / step;
-  int64_t gi = int64_t(blockIdx.x) * (kQuantThreads / 16) + threadIdx.x / 16;
-  for (int64_t t = 0; t < turns; ++t, gi += step) {
-    const bool live = gi < groups;
-    const int64_t row = live ? gi / nb : 0;
-    const int b = live ? int(gi - row * nb) : 0;
-    const int c = b * kFp8Block + l * 8;
-    const int64_t left = live ? width - c : 0;
-    const T* src = x + row * x_stride + c;
-    float v[8];
-    load8<T, WIDE>(src, left, v);
-    if constexpr (SWIGLU) {
-      float u[8];
-      load8<T, WIDE>(src + width, left, u);
+  // the warp's first lane decides: both halves take the same turns, as the shuffles want every lane
+  const int64_t first = int64_t(blockIdx.x) * (kQuantThreads / 16) + threadIdx.x / 16;
+  const int64_t groups = int64_t(rows) * nb;
+  Walk at(first, step, nb);
+  for (int64_t base = first & ~int64_t(1); base < groups; base += U * step) {
+    float v[U][8], w[SWIGLU ? U : 1][8];
+    int64_t row[U];
+    int c[U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = swiglu(v[i], u[i], limit);
+    for (int u = 0; u < U; ++u) {
+      row[u] = at.row;
+      c[u] = at.b * kFp8Block + l * 8;
+      at.next();
+      const int64_t left = row[u] < rows ? width - c[u] : 0;
+      const T* src = x + row[u] * x_stride + c[u];
+      load8<T, WIDE>(src, left, v[u]);
+      if constexpr (SWIGLU) load8<T, WIDE>(src + width, left, w[u]);
     }
-    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
+    for (int u = 0; u < U; ++u) {
+      float m = 0.f;
 #pragma unroll
-    for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const Fp8Scale s = fp8_scale(m);
-    const uint32_t lo = e4m3x4(v[0] * s.inv, v[1] * s.inv, v[2] * s.inv, v[3] * s.inv);
-    const uint32_t hi = e4m3x4(v[4] * s.inv, v[5] * s.inv, v[6] * s.inv, v[7] * s.inv);
-    uint8_t* dst = q + row * width + c;
-    if (WIDE) {
-      if (left > 0) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-    } else {
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (SWIGLU) v[u][i] = swiglu(v[u][i], w[u][i], limit);
+        m = max_nan(m, fabsf(v[u][i]));
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < left) dst[i] = uint8_t((i < 4 ? lo : hi) >> (8 * (i & 3)));
+      for (int d = 8; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+      const Fp8Scale s = fp8_scale(abs_bits(m));
+      if (row[u] >= rows) continue;
+      const uint32_t lo = e4m3x4(v[u][0] * s.inv, v[u][1] * s.inv, v[u][2] * s.inv, v[u][3] * s.inv);
+      const uint32_t hi = e4m3x4(v[u][4] * s.inv, v[u][5] * s.inv, v[u][6] * s.inv, v[u][7] * s.inv);
+      uint8_t* dst = q + row[u] * width + c[u];
+      if (WIDE) {
+        if (c[u] < width) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c[u] + i < width) dst[i] = uint8_t((i < 4 ? lo : hi) >> (8 * (i & 3)));
+      }
+      if (l == 0) scale[row[u] * nb + c[u] / kFp8Block] = s.scale;
     }
-    if (live && l == 0) scale[gi] = s.scale;
   }
 }
 
@@ -94,26 +146,25 @@ __global__ void __launch_bounds__(kQuantThreads) swiglu_grad_kernel(const T* __r
                                                                     int rows, int width, float limit,
                                                                     T* __restrict__ grad_h) {
   const int per_row = (width + 7) / 8;
-  const int64_t n = int64_t(rows) * per_row, step = int64_t(gridDim.x) * kQuantThreads;
   pdl_wait();
   pdl_trigger();
-  for (int64_t i0 = int64_t(blockIdx.x) * kQuantThreads + threadIdx.x; i0 < n; i0 += step) {
-    const int64_t row = i0 / per_row;
-    const int c = int(i0 - row * per_row) * 8;
+  for (Walk at(int64_t(blockIdx.x) * kQuantThreads + threadIdx.x, int64_t(gridDim.x) * kQuantThreads, per_row);
+       at.row < rows; at.next()) {
+    const int c = at.b * 8;
     const int left = width - c;
     float gate[8], up[8], d[8], dg[8], du[8];
-    load8<T, WIDE>(h + row * h_stride + c, left, gate);
-    load8<T, WIDE>(h + row * h_stride + width + c, left, up);
-    load8<T, WIDE>(grad + row * grad_stride + c, left, d);
+    load8<T, WIDE>(h + at.row * h_stride + c, left, gate);
+    load8<T, WIDE>(h + at.row * h_stride + width + c, left, up);
+    load8<T, WIDE>(grad + at.row * grad_stride + c, left, d);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float g = gate[i] > limit ? limit : gate[i];
-      const float u0 = up[i] > limit ? limit : up[i], u = u0 < -limit ? -limit : u0;
-      const float s = __fdiv_rn(1.f, 1.f + expf(-g));
-      dg[i] = gate[i] > limit ? 0.f : d[i] * u * (s * (1.f + g * (1.f - s)));
-      du[i] = fabsf(up[i]) > limit ? 0.f : d[i] * (g * s);
+      const float g = min_nan(gate[i], limit), u = max_nan(min_nan(up[i], limit), -limit);
+      const float s = quotient(1.f, one_plus_exp_neg(g));
+      const float gs = g * s;
+      dg[i] = gate[i] > limit ? 0.f : d[i] * u * fmaf(gs, 1.f - s, s);
+      du[i] = fabsf(up[i]) > limit ? 0.f : d[i] * gs;
     }
-    T* dst = grad_h + row * 2 * width + c;
+    T* dst = grad_h + at.row * 2 * width + c;
     if (WIDE) {
       store_vec<T, 8>(dst, dg);
       store_vec<T, 8>(dst + width, du);

@@ -15,13 +15,12 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import DTYPE_CODE, check_errors, on, stream, want, want_shape  # noqa: F401
+from .ops import DTYPE_CODE, check_errors, empty, on, stream, want, want_shape  # noqa: F401
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
 FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 MAX_EXPERTS = 1024
-FUSED_ROWS = 8  # rows that the product of one matrix quantizes itself
 
 
 def _blocks(n: int) -> int:
@@ -37,8 +36,8 @@ def _check_limit(limit) -> float:
 
 def _quantize(x, width: int, swiglu: int, limit: float):
     rows, dev = x.shape[0], x.device
-    q = torch.empty((rows, width), dtype=E4M3, device=dev)
-    scale = torch.empty((rows, _blocks(width)), dtype=torch.float32, device=dev)
+    q = empty(rows, width, E4M3, dev)
+    scale = empty(rows, _blocks(width), torch.float32, dev)
     if rows:
         with on(dev):
             _lib.check("b200moe_fp8_quantize", _lib.lib().b200moe_fp8_quantize(
@@ -75,7 +74,7 @@ def swiglu_grad(h: torch.Tensor, grad: torch.Tensor, limit: float | None = 10.0)
     want_shape("grad", grad, (rows, width))
     limit = _check_limit(limit)
     dev = h.device
-    out = torch.empty(h.shape, dtype=h.dtype, device=dev)
+    out = empty(rows, 2 * width, h.dtype, dev)
     if rows:
         with on(dev):
             _lib.check("b200moe_swiglu_grad", _lib.lib().b200moe_swiglu_grad(
@@ -138,7 +137,7 @@ def _check_out(out_dtype) -> None:
 def _product(q, scale, offsets, w, w_scale, out_dtype):
     s, k = q.shape
     n, dev = w.shape[-2], q.device
-    out = torch.empty((s, n), dtype=out_dtype, device=dev)
+    out = empty(s, n, out_dtype, dev)
     if s:
         with on(dev):
             _lib.check("b200moe_fp8_matmul", _lib.lib().b200moe_fp8_matmul(
@@ -180,17 +179,19 @@ def grouped_matmul(q: torch.Tensor, scale: torch.Tensor, offsets: torch.Tensor, 
 
 
 def _linear(x, w, w_scale, out_dtype):
-    m, k = x.shape
-    if 0 < m <= FUSED_ROWS and x.dtype != torch.float32 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
-        n, dev = w.shape[0], x.device
-        out = torch.empty((m, n), dtype=out_dtype, device=dev)
+    (m, k), n, dev = x.shape, w.shape[0], x.device
+    out = empty(m, n, out_dtype, dev)
+    if m:
+        # the quantized rows and their scales; few rows are quantized inside the product's kernel
+        nbytes = m * (k + 4 * _blocks(k)) + 16
+        if m <= 8 and x.dtype != torch.float32 and x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0:
+            nbytes = _lib.lib().b200moe_fp8_linear_workspace_bytes(m, n, k)
+        ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=dev) if nbytes else None
         with on(dev):
             _lib.check("b200moe_fp8_linear", _lib.lib().b200moe_fp8_linear(
                 stream(dev), x.data_ptr(), DTYPE_CODE[x.dtype], x.stride(0), w.data_ptr(), w_scale.data_ptr(), m, n,
-                k, out.data_ptr(), DTYPE_CODE[out_dtype]))
-        return out
-    q, scale = _quantize(x, k, 0, 1.0)
-    return _product(q, scale, None, w, w_scale, out_dtype)
+                k, out.data_ptr(), DTYPE_CODE[out_dtype], _lib.ptr(ws), nbytes))
+    return out
 
 
 class _Linear(torch.autograd.Function):

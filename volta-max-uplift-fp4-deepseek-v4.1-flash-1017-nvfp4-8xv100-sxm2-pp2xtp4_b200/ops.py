@@ -24,6 +24,11 @@ def on(device: torch.device):
     return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
+def empty(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """A contiguous matrix (the strided call parses its arguments in two thirds of ``torch.empty``'s time)."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
 def want(name: str, t: torch.Tensor, dtypes, dim: int, device: torch.device | None = None, rows: bool = False) -> None:
     """``t`` is a CUDA tensor of one of ``dtypes`` with ``dim`` axes, contiguous or
     (``rows``) with any distance between rows, on ``device`` when given."""

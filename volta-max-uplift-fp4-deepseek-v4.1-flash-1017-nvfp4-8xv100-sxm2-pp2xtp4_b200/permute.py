@@ -19,11 +19,12 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .ops import DTYPE_CODE, check_errors, on, stream, want, want_shape  # noqa: F401
+from .ops import DTYPE_CODE, check_errors, empty, on, stream, want, want_shape  # noqa: F401
 
 FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 ROWS = FLOATS + (torch.float8_e4m3fn,)
 MAX_EXPERTS, MAX_ROUTES, MAX_TOP_K = 1024, 1 << 26, 1024
+ONE_RUN = 2048  # routes up to which the sort needs no workspace
 
 
 class Permuted(NamedTuple):
@@ -36,54 +37,61 @@ class Permuted(NamedTuple):
     offsets: torch.Tensor
 
 
-def _check_routes(ids, t: int, device) -> int:
+def _check_routes(ids, t: int, num_experts: int, device) -> int:
     want("topk_ids", ids, (torch.int32,), 2, device)
     k = ids.shape[1]
     if ids.shape[0] != t or not 1 <= k <= MAX_TOP_K or t * k > MAX_ROUTES:
         raise ValueError(f"bad routing shape {tuple(ids.shape)} for {t} tokens")
+    if not 1 <= num_experts <= MAX_EXPERTS:
+        raise ValueError(f"num_experts must be 1..{MAX_EXPERTS}, got {num_experts}")
     return k
+
+
+def _tables(ids, num_experts: int):
+    """row_of_route, offsets and the sort's workspace (None where it needs none)."""
+    n, dev = ids.numel(), ids.device
+    nbytes = _lib.lib().b200moe_sort_workspace_bytes(n, num_experts) if n > ONE_RUN else 0
+    return (torch.empty_like(ids), torch.empty_strided((num_experts + 1,), (1,), dtype=torch.int32, device=dev),
+            torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None, nbytes)
 
 
 def sort_routes(topk_ids: torch.Tensor, num_experts: int) -> tuple[torch.Tensor, torch.Tensor]:
     """int32 ids [T, k] -> (row_of_route int32 [T, k], offsets int32 [num_experts + 1])."""
     want("topk_ids", topk_ids, (torch.int32,), 2)
     dev = topk_ids.device
-    _check_routes(topk_ids, topk_ids.shape[0], dev)
-    if not 1 <= num_experts <= MAX_EXPERTS:
-        raise ValueError(f"num_experts must be 1..{MAX_EXPERTS}, got {num_experts}")
+    _check_routes(topk_ids, topk_ids.shape[0], num_experts, dev)
+    row_of_route, offsets, ws, nbytes = _tables(topk_ids, num_experts)
     n = topk_ids.numel()
-    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
-    row_of_route = torch.empty_like(topk_ids)
     if n == 0:
         return row_of_route, offsets.zero_()
-    L = _lib.lib()
-    nbytes = L.b200moe_sort_workspace_bytes(n, num_experts)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with on(dev):
-        _lib.check("b200moe_sort_routes", L.b200moe_sort_routes(
+        _lib.check("b200moe_sort_routes", _lib.lib().b200moe_sort_routes(
             stream(dev), topk_ids.data_ptr(), n, num_experts, row_of_route.data_ptr(), offsets.data_ptr(),
             _lib.ptr(ws), nbytes))
     return row_of_route, offsets
 
 
-def _permute_rows(x, scale, row_of_route):
-    (t, h), k, dev = x.shape, row_of_route.shape[1], x.device
-    rows = torch.empty((t * k, h), dtype=x.dtype, device=dev)
+def _permute(x, ids, num_experts, scale):
+    (t, h), k, dev = x.shape, ids.shape[1], x.device
+    row_of_route, offsets, ws, nbytes = _tables(ids, num_experts)
+    rows = empty(t * k, h, x.dtype, dev)
     n_scale = 0 if scale is None else scale.shape[1]
-    row_scale = None if scale is None else torch.empty((t * k, n_scale), dtype=torch.float32, device=dev)
-    if t:
+    row_scale = None if scale is None else empty(t * k, n_scale, torch.float32, dev)
+    if t == 0:
+        offsets.zero_()
+    else:
         b = x.element_size()
         with on(dev):
-            _lib.check("b200moe_permute_rows", _lib.lib().b200moe_permute_rows(
-                stream(dev), x.data_ptr(), x.stride(0) * b, h * b, _lib.ptr(scale),
-                scale.stride(0) if n_scale else 0, n_scale, row_of_route.data_ptr(), t, k, rows.data_ptr(),
-                _lib.ptr(row_scale)))
-    return rows, row_scale
+            _lib.check("b200moe_permute", _lib.lib().b200moe_permute(
+                stream(dev), ids.data_ptr(), num_experts, x.data_ptr(), x.stride(0) * b, h * b, _lib.ptr(scale),
+                scale.stride(0) if n_scale else 0, n_scale, t, k, row_of_route.data_ptr(), offsets.data_ptr(),
+                rows.data_ptr(), _lib.ptr(row_scale), _lib.ptr(ws), nbytes))
+    return Permuted(rows, row_scale, row_of_route, offsets)
 
 
 def _unpermute(rows, row_of_route, weights, out_dtype):
     (t, k), h, dev = row_of_route.shape, rows.shape[1], rows.device
-    out = torch.empty((t, h), dtype=out_dtype, device=dev)
+    out = empty(t, h, out_dtype, dev)
     if t:
         with on(dev):
             _lib.check("b200moe_unpermute", _lib.lib().b200moe_unpermute(
@@ -126,14 +134,19 @@ def _check_row_of_route(row_of_route, rows, weights):
 
 class _Permute(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, row_of_route):
-        ctx.save_for_backward(row_of_route)
-        return _permute_rows(x, None, row_of_route)[0]
+    def forward(ctx, x, ids, num_experts):
+        p = _permute(x, ids, num_experts, None)
+        ctx.save_for_backward(p.row_of_route)
+        ctx.mark_non_differentiable(p.row_of_route, p.offsets)
+        ctx.set_materialize_grads(False)
+        return p.rows, p.row_of_route, p.offsets
 
     @staticmethod
-    def backward(ctx, grad):
+    def backward(ctx, grad, *_):
+        if grad is None:
+            return None, None, None
         row_of_route, = ctx.saved_tensors
-        return _unpermute(grad.contiguous(), row_of_route, None, grad.dtype), None
+        return _unpermute(grad.contiguous(), row_of_route, None, grad.dtype), None, None
 
 
 class _Unpermute(torch.autograd.Function):
@@ -159,18 +172,17 @@ def permute(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int, scale: to
     t, h = x.shape
     if h < 1:
         raise ValueError(f"x must have columns, got {tuple(x.shape)}")
-    _check_routes(topk_ids, t, x.device)
+    _check_routes(topk_ids, t, num_experts, x.device)
     if scale is not None:
         want("scale", scale, (torch.float32,), 2, x.device, rows=True)
         if scale.shape[0] != t:
             raise ValueError(f"scale must have {t} rows, got {tuple(scale.shape)}")
-    row_of_route, offsets = sort_routes(topk_ids, num_experts)
     if x.requires_grad and torch.is_grad_enabled():
         if scale is not None:
             raise ValueError("rows with scales are quantized: permute them without gradient")
-        return Permuted(_Permute.apply(x, row_of_route), None, row_of_route, offsets)
-    rows, row_scale = _permute_rows(x, scale, row_of_route)
-    return Permuted(rows, row_scale, row_of_route, offsets)
+        rows, row_of_route, offsets = _Permute.apply(x, topk_ids, num_experts)
+        return Permuted(rows, None, row_of_route, offsets)
+    return _permute(x, topk_ids, num_experts, scale)
 
 
 def unpermute(rows: torch.Tensor, row_of_route: torch.Tensor, weights: torch.Tensor | None = None,
