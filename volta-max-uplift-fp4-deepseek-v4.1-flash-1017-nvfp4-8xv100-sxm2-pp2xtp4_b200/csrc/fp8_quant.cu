@@ -16,6 +16,9 @@ namespace b200moe {
 namespace {
 
 constexpr int kQuantThreads = 256;
+// CTAs at most, for walks of several turns: SwiGLU of 49152 x 1408 takes 83 us with 16 per SM and 90 without a cap
+// (92 with 48), its gradient 102 us with 48 per SM, 116 without a cap and 108 with 16
+constexpr int64_t kCtaCap = 148 * 16, kGradCap = 148 * 48;
 
 // Minimum / maximum that keep a NaN.
 __device__ __forceinline__ float min_nan(float a, float b) {
@@ -29,40 +32,59 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return o;
 }
 
-// 1 + e^-g, at most 1e38 so that the quotients below stay finite (g / y is below E4M3's reach of the amax floor there).
-__device__ __forceinline__ float one_plus_exp_neg(float g) { return min_nan(1.f + expf(-g), 1e38f); }
+// 1 + e^-g for g >= -88. e^-g = 2^t 2^d with t the rounded product -g log2(e) and d what that rounding (an error-free
+// product, by fma) and log2(e)'s own last bits left out, 2^d = 1 + d ln 2: the power of two is the hardware's, and its
+// argument's error does not grow with g. expf and an IEEE division instead bounded these kernels: 43 instructions per
+// value, 103 us for 49152 x 1408.
+__device__ __forceinline__ float one_plus_exp_neg(float g) {
+  constexpr float kLog2e = 1.44269502162933349609375f;      // log2(e) rounded to f32
+  constexpr float kLog2eRest = 1.92596299112661746887e-8f;  // log2(e) - kLog2e
+  constexpr float kLn2 = 0.693147180559945309417f;
+  const float t = -g * kLog2e;
+  const float d = fmaf(-g, kLog2eRest, fmaf(-g, kLog2e, -t));
+  float p;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(t));
+  return 1.f + fmaf(p, d * kLn2, p);
+}
 
-// x / y for y in [1, 1e38]: the hardware reciprocal and one Newton step on the quotient's remainder. Within an ulp or
-// two of the quotient, for five instructions: an IEEE division's dozen, with its branch, bounded these kernels.
+// x / y for y in [1, 2e38]: the hardware reciprocal and one Newton step on the quotient's remainder. Past 2^126 the
+// reciprocal is flushed, and the quotient with it, to 0.
 __device__ __forceinline__ float quotient(float x, float y) {
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(y));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
   const float q = x * r;
   return fmaf(fmaf(-q, y, x), r, q);
 }
 
+// The limited gate: min(gate, limit), and -88 for what is below it (the lowest values of a type, -inf): the SwiGLU and
+// its gradient are 0 there, as g / (1 + e^-g) of any such g is in f32.
+__device__ __forceinline__ float limited_gate(float gate, float limit) { return max_nan(min_nan(gate, limit), -88.f); }
+__device__ __forceinline__ float limited_up(float up, float limit) { return max_nan(min_nan(up, limit), -limit); }
+
 // Limited SwiGLU (the framework's): g = min(gate, limit), u = clamp(up, +-limit), g / (1 + e^-g) * u.
-__device__ __forceinline__ float swiglu(float g, float u, float limit) {
-  g = min_nan(g, limit);
-  u = max_nan(min_nan(u, limit), -limit);
-  return quotient(g, one_plus_exp_neg(g)) * u;
+__device__ __forceinline__ float swiglu(float gate, float up, float limit) {
+  const float g = limited_gate(gate, limit);
+  return quotient(g, one_plus_exp_neg(g)) * limited_up(up, limit);
 }
 
-// Position (row, block) of a walk over rows x blocks in steps, without a division per step.
+// Position (row, block) of a walk over rows x blocks in steps of d_row rows and d_b blocks: one division at its start.
 struct Walk {
-  int64_t row, d_row;
-  int b, d_b, n_b;
-  __device__ __forceinline__ Walk(int64_t first, int64_t step, int blocks) : n_b(blocks) {
-    row = first / blocks;
-    b = int(first - row * blocks);
-    d_row = step / blocks;
-    d_b = int(step - d_row * blocks);
+  int64_t row;
+  int b;
+  __device__ __forceinline__ Walk(int64_t first, int blocks) {
+    if (first <= INT32_MAX) {
+      row = unsigned(first) / unsigned(blocks);
+      b = int(unsigned(first) - unsigned(row) * unsigned(blocks));
+    } else {
+      row = first / blocks;
+      b = int(first - row * blocks);
+    }
   }
-  __device__ __forceinline__ void next() {
+  __device__ __forceinline__ void next(int d_row, int d_b, int blocks) {
     row += d_row;
     b += d_b;
-    if (b >= n_b) {
-      b -= n_b;
+    if (b >= blocks) {
+      b -= blocks;
       ++row;
     }
   }
@@ -84,12 +106,17 @@ __device__ __forceinline__ void load8(const T* p, int64_t left, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] = !WIDE && i < left ? to_f32(p[i]) : 0.f;
 }
 
-// Half a warp per block; two blocks (SwiGLU) or four in flight before the first is worked on.
+// Half a warp per block; several blocks in flight before the first is worked on.
+template <typename T, bool SWIGLU>
+__host__ __device__ constexpr int blocks_in_flight() {
+  return (SWIGLU ? 2 : 4) / (sizeof(T) == 4 ? 2 : 1);
+}
+
 template <typename T, bool SWIGLU, bool WIDE>
 __global__ void __launch_bounds__(kQuantThreads) fp8_rows_kernel(const T* __restrict__ x, int64_t x_stride, int rows,
-                                                                 int width, float limit, uint8_t* __restrict__ q,
-                                                                 float* __restrict__ scale) {
-  constexpr int U = (SWIGLU ? 2 : 4) / (sizeof(T) == 4 ? 2 : 1);
+                                                                 int width, float limit, int d_row, int d_b,
+                                                                 uint8_t* __restrict__ q, float* __restrict__ scale) {
+  constexpr int U = blocks_in_flight<T, SWIGLU>();
   const int nb = (width + kFp8Block - 1) / kFp8Block, l = threadIdx.x & 15;
   const int64_t step = int64_t(gridDim.x) * (kQuantThreads / 16);
   pdl_wait();
@@ -97,7 +124,7 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_rows_kernel(const T* __rest
   // the warp's first lane decides: both halves take the same turns, as the shuffles want every lane
   const int64_t first = int64_t(blockIdx.x) * (kQuantThreads / 16) + threadIdx.x / 16;
   const int64_t groups = int64_t(rows) * nb;
-  Walk at(first, step, nb);
+  Walk at(first, nb);
   for (int64_t base = first & ~int64_t(1); base < groups; base += U * step) {
     float v[U][8], w[SWIGLU ? U : 1][8];
     int64_t row[U];
@@ -106,7 +133,7 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_rows_kernel(const T* __rest
     for (int u = 0; u < U; ++u) {
       row[u] = at.row;
       c[u] = at.b * kFp8Block + l * 8;
-      at.next();
+      at.next(d_row, d_b, nb);
       const int64_t left = row[u] < rows ? width - c[u] : 0;
       const T* src = x + row[u] * x_stride + c[u];
       load8<T, WIDE>(src, left, v[u]);
@@ -122,10 +149,13 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_rows_kernel(const T* __rest
       }
 #pragma unroll
       for (int d = 8; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
-      const Fp8Scale s = fp8_scale(abs_bits(m));
+      // both quotients of fp8_scale in one division: even lanes 448 / amax, odd lanes amax / 448
+      const float amax = max_nan(m, kAmaxFloor);
+      const float ratio = __fdiv_rn(l & 1 ? amax : kE4m3Max, l & 1 ? kE4m3Max : amax);
+      const float inv = __shfl_sync(0xffffffffu, ratio, 0, 16);
       if (row[u] >= rows) continue;
-      const uint32_t lo = e4m3x4(v[u][0] * s.inv, v[u][1] * s.inv, v[u][2] * s.inv, v[u][3] * s.inv);
-      const uint32_t hi = e4m3x4(v[u][4] * s.inv, v[u][5] * s.inv, v[u][6] * s.inv, v[u][7] * s.inv);
+      const uint32_t lo = e4m3x4(v[u][0] * inv, v[u][1] * inv, v[u][2] * inv, v[u][3] * inv);
+      const uint32_t hi = e4m3x4(v[u][4] * inv, v[u][5] * inv, v[u][6] * inv, v[u][7] * inv);
       uint8_t* dst = q + row[u] * width + c[u];
       if (WIDE) {
         if (c[u] < width) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
@@ -134,7 +164,7 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_rows_kernel(const T* __rest
         for (int i = 0; i < 8; ++i)
           if (c[u] + i < width) dst[i] = uint8_t((i < 4 ? lo : hi) >> (8 * (i & 3)));
       }
-      if (l == 0) scale[row[u] * nb + c[u] / kFp8Block] = s.scale;
+      if (l == 1) scale[row[u] * nb + c[u] / kFp8Block] = ratio;
     }
   }
 }
@@ -143,13 +173,13 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_rows_kernel(const T* __rest
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kQuantThreads) swiglu_grad_kernel(const T* __restrict__ h, int64_t h_stride,
                                                                     const T* __restrict__ grad, int64_t grad_stride,
-                                                                    int rows, int width, float limit,
-                                                                    T* __restrict__ grad_h) {
+                                                                    int rows, int width, float limit, int d_row,
+                                                                    int d_b, T* __restrict__ grad_h) {
   const int per_row = (width + 7) / 8;
   pdl_wait();
   pdl_trigger();
-  for (Walk at(int64_t(blockIdx.x) * kQuantThreads + threadIdx.x, int64_t(gridDim.x) * kQuantThreads, per_row);
-       at.row < rows; at.next()) {
+  for (Walk at(int64_t(blockIdx.x) * kQuantThreads + threadIdx.x, per_row); at.row < rows;
+       at.next(d_row, d_b, per_row)) {
     const int c = at.b * 8;
     const int left = width - c;
     float gate[8], up[8], d[8], dg[8], du[8];
@@ -158,7 +188,7 @@ __global__ void __launch_bounds__(kQuantThreads) swiglu_grad_kernel(const T* __r
     load8<T, WIDE>(grad + at.row * grad_stride + c, left, d);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float g = min_nan(gate[i], limit), u = max_nan(min_nan(up[i], limit), -limit);
+      const float g = limited_gate(gate[i], limit), u = limited_up(up[i], limit);
       const float s = quotient(1.f, one_plus_exp_neg(g));
       const float gs = g * s;
       dg[i] = gate[i] > limit ? 0.f : d[i] * u * fmaf(gs, 1.f - s, s);
@@ -277,11 +307,14 @@ cudaError_t run_rows(cudaStream_t s, const void* x, int64_t x_stride, int rows, 
                      float* scale) {
   const bool w = width % 8 == 0 && wide(x, x_stride * int64_t(sizeof(T)), 16) &&
                  (!SWIGLU || (width * int64_t(sizeof(T))) % 16 == 0) && wide(q, 8, 8);
-  const int64_t groups = int64_t(rows) * ((width + kFp8Block - 1) / kFp8Block);
-  const int64_t blocks = std::min<int64_t>((groups + kQuantThreads / 16 - 1) / (kQuantThreads / 16), 148 * 16);
+  const int nb = (width + kFp8Block - 1) / kFp8Block;
+  constexpr int per_cta = kQuantThreads / 16;
+  const int64_t turn = per_cta * blocks_in_flight<T, SWIGLU>();
+  const int64_t blocks = std::min<int64_t>((int64_t(rows) * nb + turn - 1) / turn, kCtaCap);
+  const int64_t step = blocks * per_cta;
   auto kernel = w ? fp8_rows_kernel<T, SWIGLU, true> : fp8_rows_kernel<T, SWIGLU, false>;
   return launch_chain(kernel, dim3(unsigned(blocks)), dim3(kQuantThreads), 0, s, static_cast<const T*>(x), x_stride,
-                      rows, width, limit, q, scale);
+                      rows, width, limit, int(step / nb), int(step % nb), q, scale);
 }
 
 template <typename T>
@@ -289,11 +322,13 @@ cudaError_t run_swiglu_grad(cudaStream_t s, const void* h, int64_t h_stride, con
                             int rows, int width, float limit, void* grad_h) {
   const int64_t b = sizeof(T);
   const bool w = width % 8 == 0 && wide(h, h_stride * b, 16) && wide(grad, grad_stride * b, 16) && wide(grad_h, 16, 16);
-  const int64_t n = int64_t(rows) * ((width + 7) / 8);
-  const int64_t blocks = std::min<int64_t>((n + kQuantThreads - 1) / kQuantThreads, 148 * 16);
+  const int per_row = (width + 7) / 8;
+  const int64_t blocks = std::min<int64_t>((int64_t(rows) * per_row + kQuantThreads - 1) / kQuantThreads, kGradCap);
+  const int64_t step = blocks * kQuantThreads;
   auto kernel = w ? swiglu_grad_kernel<T, true> : swiglu_grad_kernel<T, false>;
   return launch_chain(kernel, dim3(unsigned(blocks)), dim3(kQuantThreads), 0, s, static_cast<const T*>(h), h_stride,
-                      static_cast<const T*>(grad), grad_stride, rows, width, limit, static_cast<T*>(grad_h));
+                      static_cast<const T*>(grad), grad_stride, rows, width, limit, int(step / per_row),
+                      int(step % per_row), static_cast<T*>(grad_h));
 }
 
 template <typename T>
