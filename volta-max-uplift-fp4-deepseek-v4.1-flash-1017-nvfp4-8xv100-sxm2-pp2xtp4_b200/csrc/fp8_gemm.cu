@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int e = tile_expert(start, a.E, item), local = item - start[e];
         const int row = off[e] + local / n_nt * kBM, wrow = e * a.N + local % n_nt * BN;
         for (int kb = 0; kb < a.KB; ++kb) {
-          ok = __all_sync(0xffffffffu, !*abort_ptr && mbar_wait(&empty[st], ph ^ 1u, a.err));
+          ok = __all_sync(0xffffffffu, !*abort_ptr && mbar_poll(&empty[st], ph ^ 1u, a.err));
           if (!ok) break;
           if (elect_one()) {
             mbar_arrive_expect_tx(&full[st], uint32_t(kABytes + C::kWBytes));
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) *abort_ptr = 1;
       // no copy may be in flight when the CTA exits
       for (int s = 0; s < ST; ++s)
-        if (issued & (1u << s)) mbar_wait(&full[s], (par >> s) & 1u, a.err);
+        if (issued & (1u << s)) mbar_poll(&full[s], (par >> s) & 1u, a.err);
     }
     if (warp == 1) {
       int st = 0, b = 0, last = 0;
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t da0 = desc_sw128(smem_u32(at)), dw0 = desc_sw128(smem_u32(wt));
       for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x) {
         for (int kb = 0; kb < a.KB; ++kb) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[b], bph ^ 1u, a.err) && mbar_wait(&full[st], ph, a.err));
+          ok = __all_sync(0xffffffffu, mbar_poll(&acc_empty[b], bph ^ 1u, a.err) && mbar_poll(&full[st], ph, a.err));
           if (!ok) break;
           fence_after();
           const uint64_t da = da0 + st * (kABytes >> 4), dw = dw0 + st * (C::kWBytes >> 4);
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!ok) *abort_ptr = 1;
-      if (committed) mbar_wait(&acc_full[last], last_ph, a.err);
+      if (committed) mbar_poll(&acc_full[last], last_ph, a.err);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int ahead = min(kb + kAhead, a.KB - 1);
           fa[j] = __ldg(sa + ahead);
           fb[j] = __ldg(sb + ahead);
-          ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[b], bph, a.err));
+          ok = __all_sync(0xffffffffu, mbar_poll(&acc_full[b], bph, a.err));
           if (!ok) break;
           fence_after();
           const uint32_t addr = lanes + b * BN;
@@ -210,12 +210,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = 0; c < COLS / 32; ++c) {
             tmem_ld32(addr + c * 32, p);
             tmem_wait(p);
+            if (c + 1 == COLS / 32) {  // all of the block's columns are in registers: the buffer is free
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&acc_empty[b]);
+            }
 #pragma unroll
             for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(p[i]), f, acc[c * 32 + i]);
           }
-          fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[b]);
           if (++b == NBUF) b = 0, bph ^= 1u;
         }
       }

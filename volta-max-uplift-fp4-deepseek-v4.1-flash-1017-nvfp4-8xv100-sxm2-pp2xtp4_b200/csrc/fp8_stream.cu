@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int e = tile_expert(start, a.E, item), local = item - start[e];
       const int row = off[e] + local / n_wt * NTOK, wrow = e * a.N + local % n_wt * kRows;
       for (int kb = 0; kb < a.KB; ++kb) {
-        ok = __all_sync(0xffffffffu, !*abort_ptr && mbar_wait(&empty[st], ph ^ 1u, a.err));
+        ok = __all_sync(0xffffffffu, !*abort_ptr && mbar_poll(&empty[st], ph ^ 1u, a.err));
         if (!ok) break;
         if (elect_one()) {
           uint8_t* dst = stages + st * C::kStage;
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok) *abort_ptr = 1;
     // no copy may be in flight when the CTA exits
     for (int s = 0; s < ST; ++s)
-      if (issued & (1u << s)) mbar_wait(&full[s], (par >> s) & 1u, a.err);
+      if (issued & (1u << s)) mbar_poll(&full[s], (par >> s) & 1u, a.err);
   } else if (warp == 1) {
     int st = 0, b = 0, last = 0;
     uint32_t ph = 0, bph = 0, last_ph = 0;
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t d0 = desc_sw128(smem_u32(stages));
     for (int item = first; ok && item < stop; ++item) {
       for (int kb = 0; kb < a.KB; ++kb) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[b], bph ^ 1u, a.err) && mbar_wait(&full[st], ph, a.err));
+        ok = __all_sync(0xffffffffu, mbar_poll(&acc_empty[b], bph ^ 1u, a.err) && mbar_poll(&full[st], ph, a.err));
         if (!ok) break;
         fence_after();
         const uint64_t d = d0 + st * (C::kStage >> 4);
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (!ok) *abort_ptr = 1;
-    if (committed) mbar_wait(&acc_full[last], last_ph, a.err);
+    if (committed) mbar_poll(&acc_full[last], last_ph, a.err);
   } else {
     const int quarter = warp & 3, tid = threadIdx.x - 64;
     const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (kb >= a.KB) break;
           const float f = fb[j];
           fb[j] = __ldg(sb + min(kb + kAhead, a.KB - 1));
-          ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[b], bph, a.err));
+          ok = __all_sync(0xffffffffu, mbar_poll(&acc_full[b], bph, a.err));
           if (!ok) break;
           fence_after();
           const float4* s4 = reinterpret_cast<const float4*>(ss + kb * NTOK);
