@@ -34,10 +34,10 @@ namespace {
 
 constexpr int kBM = 128;
 constexpr int kSumWarps = 8;
-constexpr int kSumWarp0 = 4;  // warps 0-3: producer, MMA, two without work (a register share is a group of four)
+constexpr int kSumWarp0 = 4;  // warps 0-3: producer, MMA, two for the scales (a register share is a group of four)
 constexpr int kThreads = (kSumWarp0 + kSumWarps) * 32;
-// registers per thread: the launch's 384 x 168 split as 128 x 40 + 256 x 232
-constexpr int kFewRegs = 40, kSumRegs = 232;
+// registers per thread: the launch's 384 x 168 split as 128 x 56 + 256 x 224
+constexpr int kFewRegs = 56, kSumRegs = 224;
 constexpr int kMaxExperts = 1024;
 constexpr int kABytes = kBM * kFp8Block;
 constexpr int kOutBytes = 32 * 64;  // per sum warp: 32 rows in pieces of 64 bytes
@@ -49,7 +49,8 @@ struct Cfg {
   static constexpr int kStages = BN == 256 ? 4 : 6;
   static constexpr int kBufs = 512 / BN > 4 ? 4 : 512 / BN;  // TMEM buffers
   static constexpr int kCols = BN / 2;                        // columns per sum thread
-  static constexpr size_t kSmem = 1024 + size_t(kStages) * (kABytes + kWBytes) + kSumWarps * kOutBytes + 256;
+  static constexpr size_t kSmem = 1024 + size_t(kStages) * (kABytes + kWBytes) + kSumWarps * kOutBytes +
+                                  size_t(kBufs) * 2 * kBM * sizeof(float) + 256;
   static constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
   static_assert(kSmem + 8 * (kMaxExperts + 1) + 64 <= 227 * 1024, "shared memory, with the tile table");
 };
@@ -74,12 +75,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int off[kMaxExperts + 1], start[kMaxExperts + 1];
   __shared__ uint32_t tmem_base_sh;
   __shared__ int abort_flag;
+  __shared__ __align__(8) uint64_t mma_done;
   const uint32_t base_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* base = smem_raw + (base_u32 - smem_u32(smem_raw));
   uint8_t* at = base;                       // [ST][16 KB]
   uint8_t* wt = at + ST * kABytes;          // [ST][BN x 128]
   uint8_t* stage_out = wt + ST * C::kWBytes;  // [8][2 KB]
-  uint64_t* full = reinterpret_cast<uint64_t*>(stage_out + kSumWarps * kOutBytes);
+  float* factor = reinterpret_cast<float*>(stage_out + kSumWarps * kOutBytes);  // [NBUF][column half][row]
+  uint64_t* full = reinterpret_cast<uint64_t*>(factor + NBUF * 2 * kBM);
   uint64_t* empty = full + ST;
   uint64_t* acc_full = empty + ST;
   uint64_t* acc_empty = acc_full + NBUF;
@@ -92,9 +95,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < NBUF; ++b) {
-      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_full[b], 3);  // the MMA's commit and the two warps with its factors
       mbar_init(&acc_empty[b], kSumWarps);
     }
+    mbar_init(&mma_done, 1);
     fence_barrier_init();
     abort_flag = 0;
   }
@@ -141,8 +145,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (issued & (1u << s)) mbar_poll(&full[s], (par >> s) & 1u, a.err);
     }
     if (warp == 1) {
-      int st = 0, b = 0, last = 0;
-      uint32_t ph = 0, bph = 0, last_ph = 0;
+      int st = 0, b = 0;
+      uint32_t ph = 0, bph = 0;
       bool ok = true, committed = false;
       const uint64_t da0 = desc_sw128(smem_u32(at)), dw0 = desc_sw128(smem_u32(wt));
       for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x) {
@@ -158,14 +162,65 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
           committed = true;
-          last = b;
-          last_ph = bph;
           if (++st == ST) st = 0, ph ^= 1u;
           if (++b == NBUF) b = 0, bph ^= 1u;
         }
       }
       if (!ok) *abort_ptr = 1;
-      if (committed) mbar_poll(&acc_full[last], last_ph, a.err);
+      if (committed) {  // TMEM may be freed only after the last MMA, also after an abort
+        if (elect_one()) commit(&mma_done);
+        mbar_poll(&mma_done, 0, a.err);
+      }
+    }
+    if (warp >= 2) {
+      // both scales of each row and column half as one factor, beside the TMEM buffer that it belongs to
+      const int r0 = (warp - 2) * 64 + lane;
+      int b = 0;
+      uint32_t bph = 0;
+      bool ok = true;
+      for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x) {
+        const int e = tile_expert(start, a.E, item), local = item - start[e];
+        const int row = off[e] + local / n_nt * kBM + r0, col = local % n_nt * BN;
+        const float* sa[2] = {a.a_scale + int64_t(min(row, a.S - 1)) * a.lda_s,
+                              a.a_scale + int64_t(min(row + 32, a.S - 1)) * a.lda_s};
+        const float* sb[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          sb[h] = a.w_scale + (int64_t(e) * a.NB + min((col + h * COLS) / kFp8Block, a.NB - 1)) * a.KB;
+        float va[kAhead][2], vb[kAhead][2];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            va[j][h] = __ldg(sa[h] + min(j, a.KB - 1));
+            vb[j][h] = __ldg(sb[h] + min(j, a.KB - 1));
+          }
+        for (int kb0 = 0; ok && kb0 < a.KB; kb0 += kAhead) {
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j) {
+            const int kb = kb0 + j;
+            if (kb >= a.KB) break;
+            ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[b], bph ^ 1u, a.err));
+            if (!ok) break;
+            float* f = factor + b * 2 * kBM + r0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              f[h * kBM] = va[j][0] * vb[j][h];
+              f[h * kBM + 32] = va[j][1] * vb[j][h];
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_full[b]);
+            const int ahead = min(kb + kAhead, a.KB - 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              va[j][h] = __ldg(sa[h] + ahead);
+              vb[j][h] = __ldg(sb[h] + ahead);
+            }
+            if (++b == NBUF) b = 0, bph ^= 1u;
+          }
+        }
+      }
+      if (!ok) *abort_ptr = 1;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
@@ -180,45 +235,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int e = tile_expert(start, a.E, item), local = item - start[e];
       const int row0 = off[e] + local / n_nt * kBM + quarter * 32, end = off[e + 1];
       const int col0 = local % n_nt * BN + half * COLS;
-      const int nb = min(col0 / kFp8Block, a.NB - 1);
-      const float* sa = a.a_scale + int64_t(min(row0 + lane, a.S - 1)) * a.lda_s;
-      const float* sb = a.w_scale + (int64_t(e) * a.NB + nb) * a.KB;
       float acc[COLS];
 #pragma unroll
       for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
-      float fa[kAhead], fb[kAhead];
+      for (int kb = 0; kb < a.KB; ++kb) {
+        ok = __all_sync(0xffffffffu, mbar_poll(&acc_full[b], bph, a.err));
+        if (!ok) break;
+        fence_after();
+        const float f = factor[(b * 2 + half) * kBM + quarter * 32 + lane];
+        const uint32_t addr = lanes + b * BN;
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        fa[j] = __ldg(sa + min(j, a.KB - 1));
-        fb[j] = __ldg(sb + min(j, a.KB - 1));
-      }
-      for (int kb0 = 0; ok && kb0 < a.KB; kb0 += kAhead) {
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          const int kb = kb0 + j;
-          if (kb >= a.KB) break;
-          const float f = fa[j] * fb[j];
-          const int ahead = min(kb + kAhead, a.KB - 1);
-          fa[j] = __ldg(sa + ahead);
-          fb[j] = __ldg(sb + ahead);
-          ok = __all_sync(0xffffffffu, mbar_poll(&acc_full[b], bph, a.err));
-          if (!ok) break;
-          fence_after();
-          const uint32_t addr = lanes + b * BN;
+        for (int c = 0; c < COLS / 32; ++c) {
           uint32_t p[32];
-#pragma unroll
-          for (int c = 0; c < COLS / 32; ++c) {
-            tmem_ld32(addr + c * 32, p);
-            tmem_wait(p);
-            if (c + 1 == COLS / 32) {  // all of the block's columns are in registers: the buffer is free
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&acc_empty[b]);
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(p[i]), f, acc[c * 32 + i]);
+          tmem_ld32(addr + c * 32, p);
+          tmem_wait(p);
+          if (c + 1 == COLS / 32) {  // all of the block's columns are in registers: the buffer is free
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[b]);
           }
-          if (++b == NBUF) b = 0, bph ^= 1u;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(p[i]), f, acc[c * 32 + i]);
         }
+        if (++b == NBUF) b = 0, bph ^= 1u;
       }
       if (!ok) {
         *abort_ptr = 1;
@@ -228,6 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr int PW = 64 / int(sizeof(TO));  // columns per piece
       constexpr int CW = 16 / int(sizeof(TO));  // columns per chunk
       TO* out = static_cast<TO*>(a.out);
+      TO* dst = out + int64_t(row0 + (lane >> 2)) * a.N + col0 + (lane & 3) * CW;
       const bool vec = (int64_t(a.N) * sizeof(TO)) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
 #pragma unroll
       for (int pc = 0; pc < COLS / PW; ++pc) {
@@ -239,19 +278,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           store_vec<TO, CW>(reinterpret_cast<TO*>(mine + lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4)), v);
         }
         __syncwarp();
+        if (vec && col0 + (pc + 1) * PW <= a.N) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = j * 8 + (lane >> 2), ch = lane & 3;
-          const TO* src = reinterpret_cast<const TO*>(mine + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4));
-          const int col = col0 + pc * PW + ch * CW;
-          if (row0 + r < end) {
-            TO* dst = out + int64_t(row0 + r) * a.N + col;
-            if (vec && col + CW <= a.N) {
-              *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-            } else {
+          for (int j = 0; j < 4; ++j) {
+            const int r = j * 8 + (lane >> 2);
+            if (row0 + r < end)
+              *reinterpret_cast<uint4*>(dst + j * 8 * int64_t(a.N) + pc * PW) =
+                  *reinterpret_cast<const uint4*>(mine + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = j * 8 + (lane >> 2), col = col0 + pc * PW + (lane & 3) * CW;
+            const TO* src = reinterpret_cast<const TO*>(mine + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+            if (row0 + r < end)
               for (int i = 0; i < CW; ++i)
-                if (col + i < a.N) dst[i] = src[i];
-            }
+                if (col + i < a.N) dst[j * 8 * int64_t(a.N) + pc * PW + i] = src[i];
           }
         }
         __syncwarp();
