@@ -148,6 +148,26 @@ def test_unpermute_and_gradients(ops, dtype, t, k, e, h, drop):
 
 
 @pytest.mark.gpu
+def test_unpermute_gradients_one_at_a_time(ops):
+    """Rows without weights, weights alone, and an expanded gradient (no row of its own in memory)."""
+    g = rng(21)
+    t, k, e, h = 23, 3, 7, 96
+    row, _ = ops.permute.sort_routes(routes(g, t, k, e, 0.2), e)
+    rows, w = randn(g, t * k, h), torch.rand(t, k, generator=g, device="cuda")
+    r = rows.clone().requires_grad_()
+    gr, = torch.autograd.grad(ops.permute.unpermute(r, row).sum(), r)
+    want = torch.zeros(t * k, h, device="cuda")
+    want[row[row >= 0].long()] = 1.0
+    assert torch.equal(gr, want)
+    wr = w.clone().requires_grad_()
+    gw, = torch.autograd.grad(ops.permute.unpermute(rows, row, wr).sum(), wr)
+    y = torch.where((row >= 0)[..., None], rows.double()[row.long().clamp_min(0)], 0.0)
+    within(gw, y.sum(-1), (h + 2) * 2.0**-23 * y.abs().sum(-1))
+    gr, gw = ops.permute.unpermute_grad(torch.ones(t, h, device="cuda"), rows, row, None)
+    assert gw is None and torch.equal(gr, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("t,k,e,h,drop", SHAPES)
 def test_permute_gradient(ops, dtype, t, k, e, h, drop):

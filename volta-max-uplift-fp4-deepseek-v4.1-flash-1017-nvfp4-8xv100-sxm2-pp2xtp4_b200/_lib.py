@@ -12,12 +12,14 @@ from __future__ import annotations
 
 import ctypes
 import hashlib
+import importlib.util
 import os
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 LIB_PATH = HERE / "libb200moe.so"
 PIN_PATH = HERE / "libb200moe.so.sha256"
+OPS_PATH = HERE / "b200moe_ops.so"  # torch binding of the stateless operators (csrc/bind.cpp)
 
 P = ctypes.c_void_p
 I32 = ctypes.c_int
@@ -141,6 +143,31 @@ def lib() -> ctypes.CDLL:
             fn.restype = res
         _LIB = dll
     return _LIB
+
+
+_OPS = None
+
+
+def ops():
+    """The torch binding of the stateless operators (``permute``, ``fp8``), which calls
+    the library; built and pinned with it (raises when missing: no fallback exists)."""
+    global _OPS
+    if _OPS is None:
+        lib()
+        if not OPS_PATH.exists():
+            raise RuntimeError(f"{OPS_PATH} is missing: build it with __graft_entry__.build()")
+        pin = OPS_PATH.with_suffix(".so.sha256")
+        want = pin.read_text().strip() if pin.exists() else ""
+        if want and hashlib.sha256(OPS_PATH.read_bytes()).hexdigest() != want:
+            raise RuntimeError(f"{OPS_PATH} differs from its pin: rebuild with __graft_entry__.build()")
+        import torch  # noqa: F401  (its libraries are what the binding links to)
+
+        spec = importlib.util.spec_from_file_location("b200moe_ops", OPS_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.set_error_class(B200MoeError)
+        _OPS = mod
+    return _OPS
 
 
 def check(where: str, status: int) -> None:

@@ -1,4 +1,5 @@
-"""Build the sm_100a CUDA library ``libb200moe.so`` in place (next to this file).
+"""Build the sm_100a CUDA library ``libb200moe.so`` and the torch binding of its stateless
+operators, ``b200moe_ops.so``, in place (next to this file).
 
 Each ``csrc/*.cu`` is compiled with nvcc for ``-gencode arch=compute_100a,code=sm_100a``
 into an object, then linked into one shared library that the ctypes front end
@@ -11,6 +12,7 @@ import hashlib
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -18,7 +20,7 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OBJ = HERE / "_build"
 LIB = HERE / "libb200moe.so"
-PIN = HERE / "libb200moe.so.sha256"
+OPS = HERE / "b200moe_ops.so"
 INCLUDE = HERE.parent / "include"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -45,6 +47,31 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
+def _pin(lib: Path) -> None:
+    """The digest the loader checks a library against (a different file is refused)."""
+    lib.with_suffix(".so.sha256").write_text(hashlib.sha256(lib.read_bytes()).hexdigest() + "\n")
+
+
+def _build_ops() -> None:
+    """``csrc/bind.cpp``: the torch binding of the stateless operators, linked to the library beside it."""
+    import torch
+
+    src = CSRC / "bind.cpp"
+    newest = max(src.stat().st_mtime, *(h.stat().st_mtime for h in INCLUDE.glob("*.h")))
+    if not OPS.exists() or OPS.stat().st_mtime < newest:
+        t = Path(torch.__file__).parent
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               "-I", str(t / "include"), "-I", str(t / "include/torch/csrc/api/include"),
+               "-I", str(Path(NVCC).parent.parent / "include"), "-I", sysconfig.get_paths()["include"], str(src),
+               "-o", str(OPS), "-L", str(HERE), "-l:" + LIB.name, "-L", str(t / "lib"), "-lc10", "-lc10_cuda",
+               "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN",
+               f"-Wl,-rpath,{t / 'lib'}"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"g++ failed on {src.name}:\n{r.stdout}\n{r.stderr}")
+    _pin(OPS)
+
+
 def build(verbose: bool = False) -> Path:
     OBJ.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.cu"))
@@ -55,8 +82,8 @@ def build(verbose: bool = False) -> Path:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
-    # the digest the loader checks the library against (a different file is refused)
-    PIN.write_text(hashlib.sha256(LIB.read_bytes()).hexdigest() + "\n")
+    _pin(LIB)
+    _build_ops()
     return LIB
 
 

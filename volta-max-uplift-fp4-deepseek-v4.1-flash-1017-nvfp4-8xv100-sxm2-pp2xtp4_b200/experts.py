@@ -11,9 +11,8 @@ from __future__ import annotations
 
 import torch
 
-from . import fp8
-from .ops import want, want_shape
-from .permute import _unpermute, permute, unpermute, unpermute_grad
+from . import _lib, fp8
+from .permute import permute, unpermute, unpermute_grad
 
 SWIGLU_LIMIT = 10.0
 
@@ -25,13 +24,12 @@ class Fp8Experts:
 
     def __init__(self, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor, w2_scale: torch.Tensor, *,
                  swiglu_limit: float | None = SWIGLU_LIMIT, trainable: bool = False):
-        fp8._check_weight(w13, w13_scale, 3, None)
-        fp8._check_weight(w2, w2_scale, 3, w13.device)
+        _lib.ops().check_weight("w13", w13, w13_scale)
+        _lib.ops().check_weight("w2", w2, w2_scale)
         e, i2, h = w13.shape
-        want_shape("w2", w2, (e, h, i2 // 2))
-        if i2 % 32 or h % 16 or e > fp8.MAX_EXPERTS:
-            raise ValueError(f"hidden and inter must be multiples of 16 and experts at most {fp8.MAX_EXPERTS}, "
-                             f"got w13 {tuple(w13.shape)}")
+        if w2.shape != (e, h, i2 // 2) or i2 % 32 or h % 16 or e > 1024 or w2.device != w13.device:
+            raise ValueError("w13 [E, 2 I, H] and w2 [E, H, I] need H and I multiples of 16, E at most 1024 and one "
+                             f"device, got {tuple(w13.shape)} and {tuple(w2.shape)}")
         self.num_experts, self.hidden, self.inter = e, h, i2 // 2
         self.w13, self.w13_scale, self.w2, self.w2_scale = w13, w13_scale, w2, w2_scale
         self.swiglu_limit = swiglu_limit
@@ -57,10 +55,12 @@ class Fp8Experts:
     def forward(self, x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor) -> torch.Tensor:
         """x [T, H] (bf16 or f16), int32 ids and fp32 weights [T, k] -> [T, H] in x's dtype.
         An id outside [0, E) contributes nothing."""
-        want("x", x, (torch.bfloat16, torch.float16), 2, self.w13.device, rows=True)
-        want_shape("x", x, (x.shape[0], self.hidden))
-        want("topk_weights", topk_weights, (torch.float32,), 2, x.device)
-        want_shape("topk_weights", topk_weights, topk_ids.shape)
+        if x.dtype not in (torch.bfloat16, torch.float16) or x.dim() != 2 or x.shape[1] != self.hidden or \
+                x.device != self.w13.device:
+            raise ValueError(f"x must be fp16 or bf16 [T, {self.hidden}] on {self.w13.device}, got {x.dtype} "
+                             f"{tuple(x.shape)} on {x.device}")
+        if topk_weights.shape != topk_ids.shape:
+            raise ValueError(f"bad routing shape {tuple(topk_ids.shape)} with weights {tuple(topk_weights.shape)}")
         if torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad):
             if self.w13_t is None:
                 raise ValueError("gradients need trainable=True (the transposed weights)")
@@ -94,4 +94,4 @@ class _Experts(torch.autograd.Function):
         ga = fp8.grouped_matmul(q, scale, offsets, m.w2_t, m.w2_t_scale, h.dtype)
         q, scale = fp8.quantize(fp8.swiglu_grad(h, ga, m.swiglu_limit))
         gx = fp8.grouped_matmul(q, scale, offsets, m.w13_t, m.w13_t_scale, h.dtype)
-        return _unpermute(gx, row_of_route, None, h.dtype), gw, None, None
+        return unpermute(gx, row_of_route), gw, None, None
