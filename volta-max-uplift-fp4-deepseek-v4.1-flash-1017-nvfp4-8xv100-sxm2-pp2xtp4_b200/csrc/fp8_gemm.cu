@@ -7,18 +7,29 @@
 // of 128 rows x BN columns; per K block
 //   warp 0 (producer): two TMA boxes (128 rows of a, BN rows of w; 128 columns,
 //     128-byte swizzle) into a ring of stages;
-//   warp 1 (MMA): one thread issues 4 x tcgen05.mma.kind::f8f6f4 (M 128, N BN,
-//     K 32) into one of the TMEM buffers of BN columns and commits;
+//   warp 1 (MMA): one lane issues 4 x tcgen05.mma.kind::f8f6f4 (M 128, N BN,
+//     K 32) into one of the TMEM buffers of BN columns and commits; the whole
+//     warp runs the loop, so that its operands stay in uniform registers (issued
+//     by a lone lane of a diverged warp the four MMAs take 345 clocks);
 //   warps 4-11 (sums): read the block's product (a thread holds one row and half
 //     the columns, so both scales are one factor per thread and block) and add
-//     factor * product to f32 sums in registers, two columns per instruction,
-//     while the tensor core fills the next buffer.
-// At BN = 256 the block's MMAs take 512 clocks and its sums about 300 of each
-// scheduler's issue slots, so the tensor pipe stays the bound.  The finished
-// tile goes through shared memory so that rows are stored in 64-byte pieces.
-// Rows of a tile that belong to the next expert are computed and not stored.
-// Every wait is bounded; after an abort the roles drain in-flight copies and
-// MMAs before TMEM is freed.
+//     factor * product to f32 sums in registers while the tensor core fills the
+//     next buffer.
+// The finished tile goes through shared memory so that rows are stored in 64-byte
+// pieces.  Rows of a tile that belong to the next expert are computed and not
+// stored.  Every wait is bounded; after an abort the roles drain in-flight copies
+// and MMAs before TMEM is freed.
+//
+// Bound: at BN = 256 a block's MMAs take 516 clocks by themselves, beside
+// copies, TMEM reads and sums too, and it advances every 780: its sums take 470
+// (256 fused multiply-adds and 256 columns of TMEM reads per scheduler), and with
+// two buffers the wait for them, for the commit's arrival (230 clocks after the
+// last MMA) and for the MMA warp's turn among the sums' instructions is not
+// hidden.  8192 x 4096 x 4096: 132 us, 2.08 PFLOP/s.  Measured and not kept: sums
+// by packed f32x2 (157 us: half the rate of the scalar ones beside the copies),
+// by sixteen warps (151 us), from 16 columns at a time (167 us), blocks in halves
+// of 128 columns with barriers of their own (138 us), the factors computed by two
+// more warps (134 us), BN = 128 with four buffers (163 us).
 #include <cuda.h>
 
 #include <algorithm>
@@ -34,10 +45,10 @@ namespace {
 
 constexpr int kBM = 128;
 constexpr int kSumWarps = 8;
-constexpr int kSumWarp0 = 4;  // warps 0-3: producer, MMA, two for the scales (a register share is a group of four)
+constexpr int kSumWarp0 = 4;  // warps 0-3: producer, MMA, two without work (a register share is a group of four)
 constexpr int kThreads = (kSumWarp0 + kSumWarps) * 32;
-// registers per thread: the launch's 384 x 168 split as 128 x 56 + 256 x 224
-constexpr int kFewRegs = 56, kSumRegs = 224;
+// registers per thread: the launch's 384 x 168 split as 128 x 40 + 256 x 232
+constexpr int kFewRegs = 40, kSumRegs = 232;
 constexpr int kMaxExperts = 1024;
 constexpr int kABytes = kBM * kFp8Block;
 constexpr int kOutBytes = 32 * 64;  // per sum warp: 32 rows in pieces of 64 bytes
@@ -49,8 +60,7 @@ struct Cfg {
   static constexpr int kStages = BN == 256 ? 4 : 6;
   static constexpr int kBufs = 512 / BN > 4 ? 4 : 512 / BN;  // TMEM buffers
   static constexpr int kCols = BN / 2;                        // columns per sum thread
-  static constexpr size_t kSmem = 1024 + size_t(kStages) * (kABytes + kWBytes) + kSumWarps * kOutBytes +
-                                  size_t(kBufs) * 2 * kBM * sizeof(float) + 256;
+  static constexpr size_t kSmem = 1024 + size_t(kStages) * (kABytes + kWBytes) + kSumWarps * kOutBytes + 256;
   static constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
   static_assert(kSmem + 8 * (kMaxExperts + 1) + 64 <= 227 * 1024, "shared memory, with the tile table");
 };
@@ -75,14 +85,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int off[kMaxExperts + 1], start[kMaxExperts + 1];
   __shared__ uint32_t tmem_base_sh;
   __shared__ int abort_flag;
-  __shared__ __align__(8) uint64_t mma_done;
   const uint32_t base_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* base = smem_raw + (base_u32 - smem_u32(smem_raw));
   uint8_t* at = base;                       // [ST][16 KB]
   uint8_t* wt = at + ST * kABytes;          // [ST][BN x 128]
   uint8_t* stage_out = wt + ST * C::kWBytes;  // [8][2 KB]
-  float* factor = reinterpret_cast<float*>(stage_out + kSumWarps * kOutBytes);  // [NBUF][column half][row]
-  uint64_t* full = reinterpret_cast<uint64_t*>(factor + NBUF * 2 * kBM);
+  uint64_t* full = reinterpret_cast<uint64_t*>(stage_out + kSumWarps * kOutBytes);
   uint64_t* empty = full + ST;
   uint64_t* acc_full = empty + ST;
   uint64_t* acc_empty = acc_full + NBUF;
@@ -95,10 +103,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < NBUF; ++b) {
-      mbar_init(&acc_full[b], 3);  // the MMA's commit and the two warps with its factors
+      mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], kSumWarps);
     }
-    mbar_init(&mma_done, 1);
     fence_barrier_init();
     abort_flag = 0;
   }
@@ -145,13 +152,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (issued & (1u << s)) mbar_poll(&full[s], (par >> s) & 1u, a.err);
     }
     if (warp == 1) {
-      int st = 0, b = 0;
-      uint32_t ph = 0, bph = 0;
+      int st = 0, b = 0, last = 0;
+      uint32_t ph = 0, bph = 0, last_ph = 0;
       bool ok = true, committed = false;
       const uint64_t da0 = desc_sw128(smem_u32(at)), dw0 = desc_sw128(smem_u32(wt));
       for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x) {
         for (int kb = 0; kb < a.KB; ++kb) {
-          ok = __all_sync(0xffffffffu, mbar_poll(&acc_empty[b], bph ^ 1u, a.err) && mbar_poll(&full[st], ph, a.err));
+          ok = __all_sync(0xffffffffu, mbar_poll(&full[st], ph, a.err) && mbar_poll(&acc_empty[b], bph ^ 1u, a.err));
           if (!ok) break;
           fence_after();
           const uint64_t da = da0 + st * (kABytes >> 4), dw = dw0 + st * (C::kWBytes >> 4);
@@ -162,65 +169,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
           committed = true;
+          last = b;
+          last_ph = bph;
           if (++st == ST) st = 0, ph ^= 1u;
           if (++b == NBUF) b = 0, bph ^= 1u;
         }
       }
       if (!ok) *abort_ptr = 1;
-      if (committed) {  // TMEM may be freed only after the last MMA, also after an abort
-        if (elect_one()) commit(&mma_done);
-        mbar_poll(&mma_done, 0, a.err);
-      }
-    }
-    if (warp >= 2) {
-      // both scales of each row and column half as one factor, beside the TMEM buffer that it belongs to
-      const int r0 = (warp - 2) * 64 + lane;
-      int b = 0;
-      uint32_t bph = 0;
-      bool ok = true;
-      for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x) {
-        const int e = tile_expert(start, a.E, item), local = item - start[e];
-        const int row = off[e] + local / n_nt * kBM + r0, col = local % n_nt * BN;
-        const float* sa[2] = {a.a_scale + int64_t(min(row, a.S - 1)) * a.lda_s,
-                              a.a_scale + int64_t(min(row + 32, a.S - 1)) * a.lda_s};
-        const float* sb[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          sb[h] = a.w_scale + (int64_t(e) * a.NB + min((col + h * COLS) / kFp8Block, a.NB - 1)) * a.KB;
-        float va[kAhead][2], vb[kAhead][2];
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            va[j][h] = __ldg(sa[h] + min(j, a.KB - 1));
-            vb[j][h] = __ldg(sb[h] + min(j, a.KB - 1));
-          }
-        for (int kb0 = 0; ok && kb0 < a.KB; kb0 += kAhead) {
-#pragma unroll
-          for (int j = 0; j < kAhead; ++j) {
-            const int kb = kb0 + j;
-            if (kb >= a.KB) break;
-            ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[b], bph ^ 1u, a.err));
-            if (!ok) break;
-            float* f = factor + b * 2 * kBM + r0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              f[h * kBM] = va[j][0] * vb[j][h];
-              f[h * kBM + 32] = va[j][1] * vb[j][h];
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_full[b]);
-            const int ahead = min(kb + kAhead, a.KB - 1);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              va[j][h] = __ldg(sa[h] + ahead);
-              vb[j][h] = __ldg(sb[h] + ahead);
-            }
-            if (++b == NBUF) b = 0, bph ^= 1u;
-          }
-        }
-      }
-      if (!ok) *abort_ptr = 1;
+      if (committed) mbar_poll(&acc_full[last], last_ph, a.err);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
@@ -235,28 +191,45 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int e = tile_expert(start, a.E, item), local = item - start[e];
       const int row0 = off[e] + local / n_nt * kBM + quarter * 32, end = off[e + 1];
       const int col0 = local % n_nt * BN + half * COLS;
+      const int nb = min(col0 / kFp8Block, a.NB - 1);
+      const float* sa = a.a_scale + int64_t(min(row0 + lane, a.S - 1)) * a.lda_s;
+      const float* sb = a.w_scale + (int64_t(e) * a.NB + nb) * a.KB;
       float acc[COLS];
 #pragma unroll
       for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
-      for (int kb = 0; kb < a.KB; ++kb) {
-        ok = __all_sync(0xffffffffu, mbar_poll(&acc_full[b], bph, a.err));
-        if (!ok) break;
-        fence_after();
-        const float f = factor[(b * 2 + half) * kBM + quarter * 32 + lane];
-        const uint32_t addr = lanes + b * BN;
+      float fa[kAhead], fb[kAhead];
 #pragma unroll
-        for (int c = 0; c < COLS / 32; ++c) {
+      for (int j = 0; j < kAhead; ++j) {
+        fa[j] = __ldg(sa + min(j, a.KB - 1));
+        fb[j] = __ldg(sb + min(j, a.KB - 1));
+      }
+      for (int kb0 = 0; ok && kb0 < a.KB; kb0 += kAhead) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const int kb = kb0 + j;
+          if (kb >= a.KB) break;
+          const float f = fa[j] * fb[j];
+          const int ahead = min(kb + kAhead, a.KB - 1);
+          fa[j] = __ldg(sa + ahead);
+          fb[j] = __ldg(sb + ahead);
+          ok = __all_sync(0xffffffffu, mbar_poll(&acc_full[b], bph, a.err));
+          if (!ok) break;
+          fence_after();
+          const uint32_t addr = lanes + b * BN;
           uint32_t p[32];
-          tmem_ld32(addr + c * 32, p);
-          tmem_wait(p);
-          if (c + 1 == COLS / 32) {  // all of the block's columns are in registers: the buffer is free
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[b]);
-          }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(p[i]), f, acc[c * 32 + i]);
+          for (int c = 0; c < COLS / 32; ++c) {
+            tmem_ld32(addr + c * 32, p);
+            tmem_wait(p);
+            if (c + 1 == COLS / 32) {  // all of the block's columns are in registers: the buffer is free
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&acc_empty[b]);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(p[i]), f, acc[c * 32 + i]);
+          }
+          if (++b == NBUF) b = 0, bph ^= 1u;
         }
-        if (++b == NBUF) b = 0, bph ^= 1u;
       }
       if (!ok) {
         *abort_ptr = 1;
@@ -384,7 +357,7 @@ int product_status(const Fp8Product& p, int out_dtype) {
 int choose(const Fp8Product& p) {
   if (!p.offsets) {
     const int64_t n_tiles = (p.N + 127) / 128;
-    if (fp8_skinny_fits(p) && int64_t(p.N) * p.K <= (48 << 20)) return 8;
+    if (fp8_skinny_fits(p) && int64_t(p.N) * p.K <= (32 << 20)) return 8;
     for (int t = 16; t <= 32; t *= 2)
       if ((p.S + t - 1) / t * n_tiles <= sm_count() && fp8_stream_fits(p.K, t)) return t;
     // more columns than one wave holds, bound by their bytes as long as one tile has all rows
