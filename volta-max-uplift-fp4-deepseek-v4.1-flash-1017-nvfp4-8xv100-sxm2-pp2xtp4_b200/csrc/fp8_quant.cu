@@ -3,8 +3,8 @@
 // packed weights (the gradient of a product's rows contracts over the weights'
 // other axis).
 //
-// Row blocks are 1 x 128: sixteen lanes hold a block, eight columns each (one
-// 16-byte load of 16-bit values), so the maximum is four shuffles and a block
+// Row blocks are 1 x 128: eight lanes hold a block, sixteen columns each (two
+// 16-byte loads of 16-bit values), so the maximum is three shuffles and a block
 // is read once.  Weight blocks are 128 x 128: a CTA holds one in registers.
 // Bound: HBM (f32 or 16-bit columns in, one byte out).
 #include <algorithm>
@@ -16,6 +16,7 @@ namespace b200moe {
 namespace {
 
 constexpr int kQuantThreads = 256;
+constexpr int kQuantBlocks = kQuantThreads / 8;  // row blocks of a CTA's turn
 // CTAs at most, for walks of several turns: SwiGLU of 49152 x 1408 takes 83 us with 16 per SM and 90 without a cap
 // (92 with 48), its gradient 102 us with 48 per SM, 116 without a cap and 108 with 16
 constexpr int64_t kCtaCap = 148 * 16, kGradCap = 148 * 48;
@@ -106,10 +107,12 @@ __device__ __forceinline__ void load8(const T* p, int64_t left, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] = !WIDE && i < left ? to_f32(p[i]) : 0.f;
 }
 
-// Half a warp per block; several blocks in flight before the first is worked on.
+// Eight lanes per block, sixteen columns each: what a block costs beside its values (its place, the maximum's
+// shuffles, the division) is shared by sixteen values per lane. Several blocks are in flight before the first is
+// worked on.
 template <typename T, bool SWIGLU>
 __host__ __device__ constexpr int blocks_in_flight() {
-  return (SWIGLU ? 2 : 4) / (sizeof(T) == 4 ? 2 : 1);
+  return SWIGLU || sizeof(T) == 4 ? 1 : 2;
 }
 
 template <typename T, bool SWIGLU, bool WIDE>
@@ -117,52 +120,61 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_rows_kernel(const T* __rest
                                                                  int width, float limit, int d_row, int d_b,
                                                                  uint8_t* __restrict__ q, float* __restrict__ scale) {
   constexpr int U = blocks_in_flight<T, SWIGLU>();
-  const int nb = (width + kFp8Block - 1) / kFp8Block, l = threadIdx.x & 15;
-  const int64_t step = int64_t(gridDim.x) * (kQuantThreads / 16);
+  const int nb = (width + kFp8Block - 1) / kFp8Block, l = threadIdx.x & 7;
+  const int64_t step = int64_t(gridDim.x) * kQuantBlocks;
   pdl_wait();
   pdl_trigger();
-  // the warp's first lane decides: both halves take the same turns, as the shuffles want every lane
-  const int64_t first = int64_t(blockIdx.x) * (kQuantThreads / 16) + threadIdx.x / 16;
+  // the warp's first block decides: its four take the same turns, as the shuffles want every lane
+  const int64_t first = int64_t(blockIdx.x) * kQuantBlocks + threadIdx.x / 8;
   const int64_t groups = int64_t(rows) * nb;
   Walk at(first, nb);
-  for (int64_t base = first & ~int64_t(1); base < groups; base += U * step) {
-    float v[U][8], w[SWIGLU ? U : 1][8];
+  for (int64_t base = first & ~int64_t(3); base < groups; base += U * step) {
+    float v[U][2][8], w[SWIGLU ? U : 1][2][8];
     int64_t row[U];
     int c[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       row[u] = at.row;
-      c[u] = at.b * kFp8Block + l * 8;
+      c[u] = at.b * kFp8Block + l * 16;
       at.next(d_row, d_b, nb);
       const int64_t left = row[u] < rows ? width - c[u] : 0;
       const T* src = x + row[u] * x_stride + c[u];
-      load8<T, WIDE>(src, left, v[u]);
-      if constexpr (SWIGLU) load8<T, WIDE>(src + width, left, w[u]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        load8<T, WIDE>(src + 8 * h, left - 8 * h, v[u][h]);
+        if constexpr (SWIGLU) load8<T, WIDE>(src + width + 8 * h, left - 8 * h, w[u][h]);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (SWIGLU) v[u][i] = swiglu(v[u][i], w[u][i], limit);
-        m = max_nan(m, fabsf(v[u][i]));
-      }
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int d = 8; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (SWIGLU) v[u][h][i] = swiglu(v[u][h][i], w[u][h][i], limit);
+          m = max_nan(m, fabsf(v[u][h][i]));
+        }
+#pragma unroll
+      for (int d = 4; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
       // both quotients of fp8_scale in one division: even lanes 448 / amax, odd lanes amax / 448
       const float amax = max_nan(m, kAmaxFloor);
       const float ratio = __fdiv_rn(l & 1 ? amax : kE4m3Max, l & 1 ? kE4m3Max : amax);
-      const float inv = __shfl_sync(0xffffffffu, ratio, 0, 16);
+      const float inv = __shfl_sync(0xffffffffu, ratio, 0, 8);
       if (row[u] >= rows) continue;
-      const uint32_t lo = e4m3x4(v[u][0] * inv, v[u][1] * inv, v[u][2] * inv, v[u][3] * inv);
-      const uint32_t hi = e4m3x4(v[u][4] * inv, v[u][5] * inv, v[u][6] * inv, v[u][7] * inv);
       uint8_t* dst = q + row[u] * width + c[u];
-      if (WIDE) {
-        if (c[u] < width) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-      } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c[u] + i < width) dst[i] = uint8_t((i < 4 ? lo : hi) >> (8 * (i & 3)));
+      for (int h = 0; h < 2; ++h) {
+        const float(&y)[8] = v[u][h];
+        const uint32_t lo = e4m3x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+        const uint32_t hi = e4m3x4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv);
+        if (WIDE) {
+          if (c[u] + 8 * h < width) *reinterpret_cast<uint2*>(dst + 8 * h) = make_uint2(lo, hi);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c[u] + 8 * h + i < width) dst[8 * h + i] = uint8_t((i < 4 ? lo : hi) >> (8 * (i & 3)));
+        }
       }
       if (l == 1) scale[row[u] * nb + c[u] / kFp8Block] = ratio;
     }
@@ -308,10 +320,9 @@ cudaError_t run_rows(cudaStream_t s, const void* x, int64_t x_stride, int rows, 
   const bool w = width % 8 == 0 && wide(x, x_stride * int64_t(sizeof(T)), 16) &&
                  (!SWIGLU || (width * int64_t(sizeof(T))) % 16 == 0) && wide(q, 8, 8);
   const int nb = (width + kFp8Block - 1) / kFp8Block;
-  constexpr int per_cta = kQuantThreads / 16;
-  const int64_t turn = per_cta * blocks_in_flight<T, SWIGLU>();
+  const int64_t turn = kQuantBlocks * blocks_in_flight<T, SWIGLU>();
   const int64_t blocks = std::min<int64_t>((int64_t(rows) * nb + turn - 1) / turn, kCtaCap);
-  const int64_t step = blocks * per_cta;
+  const int64_t step = blocks * kQuantBlocks;
   auto kernel = w ? fp8_rows_kernel<T, SWIGLU, true> : fp8_rows_kernel<T, SWIGLU, false>;
   return launch_chain(kernel, dim3(unsigned(blocks)), dim3(kQuantThreads), 0, s, static_cast<const T*>(x), x_stride,
                       rows, width, limit, int(step / nb), int(step % nb), q, scale);
