@@ -17,8 +17,8 @@ namespace {
 
 constexpr int kQuantThreads = 256;
 constexpr int kQuantBlocks = kQuantThreads / 8;  // row blocks of a CTA's turn
-// CTAs at most, for walks of several turns: SwiGLU of 49152 x 1408 takes 83 us with 16 per SM and 90 without a cap
-// (92 with 48), its gradient 102 us with 48 per SM, 116 without a cap and 108 with 16
+// CTAs at most, for walks of several turns: SwiGLU of 49152 x 1408 takes 70 us with 16 per SM, 72 with 8 and 77
+// without a cap, its gradient 102 us with 48 per SM, 116 without a cap and 108 with 16
 constexpr int64_t kCtaCap = 148 * 16, kGradCap = 148 * 48;
 
 // Minimum / maximum that keep a NaN.
@@ -48,13 +48,13 @@ __device__ __forceinline__ float one_plus_exp_neg(float g) {
   return 1.f + fmaf(p, d * kLn2, p);
 }
 
-// x / y for y in [1, 2e38]: the hardware reciprocal and one Newton step on the quotient's remainder. Past 2^126 the
-// reciprocal is flushed, and the quotient with it, to 0.
+// x / y for y in [1, 2e38], by the hardware reciprocal: with the exponential above within 5.1 units of 2^-24 of the
+// value over gates in [-70, 12] (f32's own exponential and division: 3.6; a Newton step on the remainder: 5.2). Past
+// 2^126 the reciprocal is flushed, and the quotient with it, to 0.
 __device__ __forceinline__ float quotient(float x, float y) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
-  const float q = x * r;
-  return fmaf(fmaf(-q, y, x), r, q);
+  return x * r;
 }
 
 // The limited gate: min(gate, limit), and -88 for what is below it (the lowest values of a type, -inf): the SwiGLU and

@@ -323,8 +323,9 @@ __device__ __forceinline__ float warp_sum8(const float (&v)[8], int lane) {
 
 // A CTA per token: g[t] is read once for up to eight slots; each slot's row is
 // read for the dot product and its gradient row written in the same pass.
+// Three CTAs per SM where the registers allow it: 95 us at 4096 tokens of 8 x 4096, 99 with two.
 template <typename TG, typename TI, int V>
-__global__ void __launch_bounds__(256) unpermute_grad_kernel(const TG* __restrict__ grad, int64_t grad_stride,
+__global__ void __launch_bounds__(256, V > 1 && sizeof(TI) == 2 ? 3 : 2) unpermute_grad_kernel(const TG* __restrict__ grad, int64_t grad_stride,
                                                              const TI* __restrict__ rows,
                                                              const int32_t* __restrict__ row_of_route,
                                                              const float* __restrict__ weights, int T, int k, int H,
