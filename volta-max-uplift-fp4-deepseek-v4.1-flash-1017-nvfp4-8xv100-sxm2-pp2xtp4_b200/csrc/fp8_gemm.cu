@@ -350,7 +350,9 @@ int product_status(const Fp8Product& p, int out_dtype) {
 // The kernel by rows per matrix, as measured on B200 (us; kernels of 8, 16, 32 and 128 rows per tile):
 //   one matrix 4096 x 4096: 6.8 / 11.5 / 12.4 / 14.2 at 1 row, - / 11.9 / 13.0 / 14.5 at 32, - / 12.1 / 13.1 / 14.5
 //   at 64, - / 20.9 / 13.2 / 14.6 at 96, - / 29.7 / 23.1 / 15.4 at 192: a tile of fewer rows gives more CTAs, so the
-//   smallest whose tiles still run in one wave;
+//   smallest whose tiles still run in one wave (the kernels' order, as each has become faster since: 5.6 at 1 row, 9.0
+//   at 32, 10.9 at 96, 13.6 at 192). The first is left where its bandwidth costs more than its latency saves: 8192 x
+//   4096 takes 11.3 / 11.6 with one row, 11264 x 4096 15.2 / 12.3;
 //   64 matrices 2816 x 2048: - / 67 / 64 / 71 at 8 rows each, - / 104 / 66 / 73 at 24, - / 112 / 91 / 74 at 32, where
 //   experts above 32 rows read their weights twice.
 // Returns 8, 16, 32 or 128.

@@ -7,15 +7,18 @@
 // rows), a contiguous range of them, so that it streams an expert's weights in
 // order. Per K block of 128
 //   warp 0 (producer): TMA boxes of 128 weight rows and NTOK token rows into a
-//     ring of stages that keeps about 180 KB in flight;
-//   warp 1 (MMA): 4 x tcgen05.mma.kind::f8f6f4 (M 128, N NTOK, K 32) into one of
-//     eight TMEM buffers;
+//     ring of eight stages, 144 or 160 KB in flight;
+//   warps 1 and 6 (MMA), a block each in turn: 4 x tcgen05.mma.kind::f8f6f4 (M 128,
+//     N NTOK, K 32) into one of eight TMEM buffers;
 //   warps 2-5 (sums): a thread holds one weight row; product times the weight
 //     block's scale and each token's (in shared memory, four per load) joins the
 //     f32 sums of its NTOK columns.
-// Streaming the weights through registers into mma.sync instead reached 4.9 of
-// the copy's 6.55 TB/s at best: a warp's loads in flight share its six
-// scoreboards, and the conversions to f16 take issue slots.
+// 190 experts of 4096 x 4096 for 256 rows: 461 us, 6.95 TB/s, the rate of a plain
+// copy and a little more (it reads only). Streaming the weights through registers
+// into mma.sync instead reached 4.9 TB/s at best: a warp's loads in flight share
+// its few scoreboards, and the conversions to f16 take issue slots. One matrix of
+// 4096 x 4096 for 64 rows has 32 x 4 items and takes 9.2 us, 4.2 of them the
+// launch and the first bytes; with one MMA warp 10.7.
 #include <cuda.h>
 
 #include <algorithm>
@@ -31,7 +34,7 @@ namespace {
 
 constexpr int kMaxExperts = 1024;
 constexpr int kRows = 128;  // weight rows per item
-constexpr int kThreads = 192;
+constexpr int kThreads = 224;  // producer, four warps of sums, two of MMAs
 constexpr int kWBytes = kRows * kFp8Block;
 constexpr int kScaleBytes = 16 * 1024;  // the token tile's scales
 constexpr int kBufs = 8;
@@ -40,7 +43,11 @@ constexpr int kAhead = 4;  // K blocks whose weight scales are loaded ahead
 template <int NTOK>
 struct Cfg {
   static constexpr int kStage = kWBytes + NTOK * kFp8Block;
-  static constexpr int kStages = (195 * 1024) / kStage;
+  // even, as the TMEM buffers: a stage then stays with one of the two MMA warps. Were it shared, one warp could wait
+  // for its second filling before the first has landed, and a parity wait would take the phase before for it. Eight
+  // measure better than ten: 461 and 482 us for 190 experts of 4096 x 4096.
+  static constexpr int kStages = 8;
+  static_assert(kStages % 2 == 0 && kBufs % 2 == 0, "stages and buffers by MMA warp");
   static constexpr size_t kSmem = 1024 + size_t(kStages) * kStage + kScaleBytes + 512;
   static constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(NTOK >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
   static_assert(kSmem + 8 * (kMaxExperts + 1) + 64 <= 227 * 1024, "shared memory, with the tile table");
@@ -130,29 +137,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     // no copy may be in flight when the CTA exits
     for (int s = 0; s < ST; ++s)
       if (issued & (1u << s)) mbar_poll(&full[s], (par >> s) & 1u, a.err);
-  } else if (warp == 1) {
-    int st = 0, b = 0, last = 0;
+  } else if (warp == 1 || warp == 6) {
+    // two warps take the K blocks in turn, whatever their items: one block's four MMAs and two commits take 250 clocks
+    // to issue, where its bytes arrive in 180
+    const int64_t total = int64_t(stop - first) * a.KB;
+    int st = warp == 6, b = st, last = 0;
     uint32_t ph = 0, bph = 0, last_ph = 0;
     bool ok = true, committed = false;
     const uint64_t d0 = desc_sw128(smem_u32(stages));
-    for (int item = first; ok && item < stop; ++item) {
-      for (int kb = 0; kb < a.KB; ++kb) {
-        ok = __all_sync(0xffffffffu, mbar_poll(&acc_empty[b], bph ^ 1u, a.err) && mbar_poll(&full[st], ph, a.err));
-        if (!ok) break;
-        fence_after();
-        const uint64_t d = d0 + st * (C::kStage >> 4);
-        if (elect_one()) {
-          mma_block(tmem + b * NTOK, d, d + (kWBytes >> 4), C::kIdesc);
-          commit(&empty[st]);
-          commit(&acc_full[b]);
-        }
-        __syncwarp();
-        committed = true;
-        last = b;
-        last_ph = bph;
-        if (++st == ST) st = 0, ph ^= 1u;
-        if (++b == kBufs) b = 0, bph ^= 1u;
+    for (int64_t g = st; ok && g < total; g += 2) {
+      ok = __all_sync(0xffffffffu, mbar_poll(&full[st], ph, a.err) && mbar_poll(&acc_empty[b], bph ^ 1u, a.err));
+      if (!ok) break;
+      fence_after();
+      const uint64_t d = d0 + st * (C::kStage >> 4);
+      if (elect_one()) {
+        mma_block(tmem + b * NTOK, d, d + (kWBytes >> 4), C::kIdesc);
+        commit(&empty[st]);
+        commit(&acc_full[b]);
       }
+      __syncwarp();
+      committed = true;
+      last = b;
+      last_ph = bph;
+      if ((st += 2) >= ST) st -= ST, ph ^= 1u;
+      if ((b += 2) >= kBufs) b -= kBufs, bph ^= 1u;
     }
     if (!ok) *abort_ptr = 1;
     if (committed) mbar_poll(&acc_full[last], last_ph, a.err);
