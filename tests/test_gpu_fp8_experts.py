@@ -665,3 +665,19 @@ def test_refusals(ops):
     flat = torch.zeros(12 * 64 + 16, dtype=torch.uint8, device=dev).view(E4M3)
     with pytest.raises(B200MoeError):
         F.matmul(flat[8: 8 + 6 * 64].view(6, 64), s, w, ws)
+
+
+@pytest.mark.gpu
+def test_example_learns_and_serves():
+    """The example's loss falls, and single tokens give the batch's rows up to the last rounding (both differ from the
+    exact sum by half a bf16 step, 2^-9 in the rms at most)."""
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "fp8_experts.py"
+    spec = importlib.util.spec_from_file_location("fp8_experts_example", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    got = mod.main(["--tokens", "96", "--hidden", "256", "--inter", "128", "--experts", "8", "--steps", "20"])
+    assert got["last"] < 0.9 * got["first"]
+    assert got["single"] <= 2 * 2.0**-8
