@@ -71,6 +71,7 @@ struct GemmArgs {
   const float* w_scale;  // [E][NB][KB]
   const int32_t* offsets;  // [E + 1], null: one matrix, all S rows
   void* out;             // [S][N]
+  int copy_out;          // its rows lie on 16 bytes
   int S, N, K, E, KB, NB;
   uint32_t* err;
 };
@@ -78,7 +79,7 @@ struct GemmArgs {
 template <int BN, typename TO>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_gemm_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap map_a,
-                    const __grid_constant__ CUtensorMap map_w) {
+                    const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out) {
   using C = Cfg<BN>;
   constexpr int ST = C::kStages, NBUF = C::kBufs, COLS = C::kCols;
   extern __shared__ uint8_t smem_raw[];
@@ -238,11 +239,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       // through shared memory in pieces of 64 bytes per row, 16-byte chunks swizzled by pairs of rows
       constexpr int PW = 64 / int(sizeof(TO));  // columns per piece
       constexpr int CW = 16 / int(sizeof(TO));  // columns per chunk
-      TO* out = static_cast<TO*>(a.out);
-      TO* dst = out + int64_t(row0 + (lane >> 2)) * a.N + col0 + (lane & 3) * CW;
-      const bool vec = (int64_t(a.N) * sizeof(TO)) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+      TO* dst = static_cast<TO*>(a.out) + int64_t(row0 + (lane >> 2)) * a.N + col0 + (lane & 3) * CW;
+      // whole rows of one expert leave by a copy of their own (the warp's 32 rows, 64 bytes each, swizzled as the map
+      // says); a tile that ends inside, or rows off 16 bytes, by the threads
+      const bool copies = a.copy_out && row0 + 32 <= end;
 #pragma unroll
       for (int pc = 0; pc < COLS / PW; ++pc) {
+        if (lane == 0) tma_stores_read();  // the piece before has left
+        __syncwarp();
 #pragma unroll
         for (int ch = 0; ch < 4; ++ch) {
           float v[CW];
@@ -250,28 +254,31 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < CW; ++i) v[i] = acc[pc * PW + ch * CW + i];
           store_vec<TO, CW>(reinterpret_cast<TO*>(mine + lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4)), v);
         }
-        __syncwarp();
-        if (vec && col0 + (pc + 1) * PW <= a.N) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = j * 8 + (lane >> 2);
-            if (row0 + r < end)
-              *reinterpret_cast<uint4*>(dst + j * 8 * int64_t(a.N) + pc * PW) =
-                  *reinterpret_cast<const uint4*>(mine + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
-          }
+        const int col = col0 + pc * PW;
+        if (copies) {
+          fence_async();
+          __syncwarp();
+          if (lane == 0 && col < a.N) tma_store_2d(&map_out, col * int(sizeof(TO)), row0, mine);
         } else {
+          __syncwarp();
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int r = j * 8 + (lane >> 2), col = col0 + pc * PW + (lane & 3) * CW;
+            const int r = j * 8 + (lane >> 2), c = col + (lane & 3) * CW;
             const TO* src = reinterpret_cast<const TO*>(mine + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
-            if (row0 + r < end)
+            TO* d = dst + j * 8 * int64_t(a.N) + pc * PW;
+            if (row0 + r >= end) continue;
+            if (a.copy_out && c + CW <= a.N) {
+              *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(src);
+            } else {
               for (int i = 0; i < CW; ++i)
-                if (col + i < a.N) dst[j * 8 * int64_t(a.N) + pc * PW + i] = src[i];
+                if (c + i < a.N) d[i] = src[i];
+            }
           }
+          __syncwarp();
         }
-        __syncwarp();
       }
     }
+    if (lane == 0) tma_stores_done();
     if (a.offsets) zero_rows(static_cast<TO*>(a.out), a.N, off[a.E], a.S, threadIdx.x - kSumWarp0 * 32, kSumWarps * 32);
   }
   fence_before();
@@ -284,7 +291,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int BN, typename TO>
-int launch_one(cudaStream_t s, const GemmArgs& a, const CUtensorMap& ma, const CUtensorMap& mw, int grid) {
+int launch_one(cudaStream_t s, const GemmArgs& a, const CUtensorMap& ma, const CUtensorMap& mw, const CUtensorMap& mo,
+               int grid) {
   static std::atomic<uint64_t> attr_set{0};  // devices whose attribute is set
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -1;
@@ -294,7 +302,8 @@ int launch_one(cudaStream_t s, const GemmArgs& a, const CUtensorMap& ma, const C
       return -1;
     attr_set.fetch_or(uint64_t(1) << dev);
   }
-  return launch_chain(fp8_gemm_kernel<BN, TO>, dim3(grid), dim3(kThreads), Cfg<BN>::kSmem, s, a, ma, mw) == cudaSuccess
+  return launch_chain(fp8_gemm_kernel<BN, TO>, dim3(grid), dim3(kThreads), Cfg<BN>::kSmem, s, a, ma, mw, mo) ==
+                 cudaSuccess
              ? 0
              : -1;
 }
@@ -321,12 +330,15 @@ int launch_fp8_gemm(cudaStream_t s, const Fp8Product& p, int out_dtype) {
   const int64_t wide_tiles = m_tiles * ((p.N + 255) / 256);
   const bool wide = wide_tiles >= sms;
   const int bn = wide ? 256 : 128;
-  CUtensorMap ma, mw;
+  const int64_t out_bytes = int64_t(p.N) * (out_dtype == B200MOE_F32 ? 4 : 2);
+  a.copy_out = out_bytes % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+  CUtensorMap ma, mw, mo{};
   if (make_u8_tile_map(&ma, p.a, p.S, p.K, kFp8Block, kBM) ||
       make_u8_tile_map(&mw, p.w, int64_t(p.E) * p.N, p.K, kFp8Block, bn))
     return -1;
+  if (a.copy_out && make_u8_store_map(&mo, p.out, p.S, out_bytes, 32)) return -1;
   const int grid = int(std::min<int64_t>(sms, m_tiles * ((p.N + bn - 1) / bn)));
-  auto run = [&](auto one) { return one(s, a, ma, mw, grid); };
+  auto run = [&](auto one) { return one(s, a, ma, mw, mo, grid); };
   if (out_dtype == B200MOE_F16) return run(wide ? launch_one<256, __half> : launch_one<128, __half>);
   if (out_dtype == B200MOE_BF16) return run(wide ? launch_one<256, __nv_bfloat16> : launch_one<128, __nv_bfloat16>);
   return run(wide ? launch_one<256, float> : launch_one<128, float>);

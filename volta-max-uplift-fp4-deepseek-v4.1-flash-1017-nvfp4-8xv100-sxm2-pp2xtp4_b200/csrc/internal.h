@@ -204,6 +204,8 @@ int launch_fp4_tile(cudaStream_t s, bool mx, const uint8_t* codes, const uint8_t
                     int rows_per_slot, int K, bool gate_up, const float* globals, uint32_t* err, uint8_t* out);
 // 2D uint8 TMA map with 128-byte swizzle: rows x row_bytes, box box_bytes x box_rows, zero fill out of range
 int make_u8_tile_map(void* map_out, const void* base, int64_t rows, int64_t row_bytes, int box_bytes, int box_rows);
+// the same for stores of 64-byte wide boxes with 64-byte swizzle; what lies out of range is not written
+int make_u8_store_map(void* map_out, void* base, int64_t rows, int64_t row_bytes, int box_rows);
 
 size_t plan_smem_bytes(int n_keys);
 // the receive of this rank's expert-parallel exchange object (the C ABI's b200moe_ep)
