@@ -514,6 +514,43 @@ def test_empty_batches(ops):
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits(ops):
+    """2.4 million rows of 1024: elements past 2^31 in every operator; the last rows are looked at."""
+    g = rng(31)
+    t, k, e, h = 300_000, 8, 16, 1024
+    ids = torch.randint(0, e, (t, k), generator=g, device="cuda", dtype=torch.int32)
+    x = randn(g, t, h, dtype=torch.bfloat16)
+    p = ops.permute.permute(x, ids, e)
+    assert p.rows.numel() > 2**31
+    tail = p.row_of_route[-500:].long()
+    assert torch.equal(p.rows[tail], x[-500:, None].expand(-1, k, -1))
+    w = torch.rand(t, k, generator=g, device="cuda")
+    out = ops.permute.unpermute(p.rows, p.row_of_route, w)[-500:]
+    want, mag = plain_unpermute(p.rows[tail].reshape(-1, h), torch.arange(500 * k, device="cuda").view(500, k), w[-500:])
+    within(out, want, (k + 1) * 2.0**-23 * mag + U[torch.bfloat16] * want.abs() + TINY[torch.bfloat16])
+    grad_rows, _ = ops.permute.unpermute_grad(x, p.rows, p.row_of_route, w, need_weights=False)
+    back = w[-500:, :, None].double() * x[-500:, None].double()
+    within(grad_rows[tail], back, 2 * U[torch.bfloat16] * back.abs() + TINY[torch.bfloat16])
+    del grad_rows
+    q, scale = ops.fp8.quantize(p.rows)
+    want_q, want_scale = plain_quantize(p.rows[-300:])
+    assert torch.equal(scale[-300:], want_scale)
+    same_bits(q[-300:], want_q)
+    wq, ws = weights(g, e, h, h)
+    y = ops.fp8.grouped_matmul(q, scale, p.offsets, wq, ws)[-300:]  # the last expert's
+    want, mag = plain_product(q[-300:], scale[-300:], wq[-1], ws[-1])
+    within(y, want, sum_bound(mag, h) + U[torch.bfloat16] * want.abs() + TINY[torch.bfloat16])
+    del y, q, scale
+    half = p.rows.view(t * k // 2, 2 * h)
+    a, a_scale = ops.fp8.swiglu_quantize(half)
+    a0, s0 = ops.fp8.swiglu_quantize(half[-100:])
+    same_bits(a[-100:], a0)
+    assert torch.equal(a_scale[-100:], s0)
+    d = ops.fp8.swiglu_grad(half, half[:, :h])
+    assert torch.equal(d[-100:], ops.fp8.swiglu_grad(half[-100:], half[-100:, :h]))
+
+
+@pytest.mark.gpu
 def test_same_bits_and_another_stream(ops):
     g = rng(9)
     t, k, e, h, i = 50, 4, 16, 256, 128

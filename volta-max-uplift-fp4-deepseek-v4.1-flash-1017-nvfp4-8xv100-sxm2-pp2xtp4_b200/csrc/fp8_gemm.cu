@@ -15,21 +15,22 @@
 //     the columns, so both scales are one factor per thread and block) and add
 //     factor * product to f32 sums in registers while the tensor core fills the
 //     next buffer.
-// The finished tile goes through shared memory so that rows are stored in 64-byte
-// pieces.  Rows of a tile that belong to the next expert are computed and not
+// The finished tile leaves through shared memory by TMA stores of 32 rows x 64
+// bytes.  Rows of a tile that belong to the next expert are computed and not
 // stored.  Every wait is bounded; after an abort the roles drain in-flight copies
 // and MMAs before TMEM is freed.
 //
-// Bound: at BN = 256 a block's MMAs take 516 clocks by themselves, beside
-// copies, TMEM reads and sums too, and it advances every 780: its sums take 470
-// (256 fused multiply-adds and 256 columns of TMEM reads per scheduler), and with
-// two buffers the wait for them, for the commit's arrival (230 clocks after the
-// last MMA) and for the MMA warp's turn among the sums' instructions is not
-// hidden.  8192 x 4096 x 4096: 132 us, 2.08 PFLOP/s.  Measured and not kept: sums
-// by packed f32x2 (157 us: half the rate of the scalar ones beside the copies),
-// by sixteen warps (151 us), from 16 columns at a time (167 us), blocks in halves
-// of 128 columns with barriers of their own (138 us), the factors computed by two
-// more warps (134 us), BN = 128 with four buffers (163 us).
+// Bound: at BN = 256 a block's MMAs take 516 clocks by themselves, beside copies,
+// TMEM reads and sums too (each measured apart), and the kernel takes about 800 a
+// block: the sums 470 (256 fused multiply-adds and 256 columns of TMEM reads per
+// scheduler), and with two buffers their waits, the issue and the commit's arrival
+// (290 together) and the MMA warp's turns among the sums' instructions are not
+// hidden. 8192 x 4096 x 4096: 129 us, 2.12 PFLOP/s, the tensor pipe 55 % busy.
+// Measured and not kept: sums by packed f32x2 (157 us: half the rate of the scalar
+// ones), by sixteen warps (151 us), from 16 columns at a time (167 us), blocks in
+// halves of 128 columns with barriers of their own (138 us), the factors computed by
+// two more warps (134 us), BN = 128 with four buffers (163 us), L2 prefetch of the
+// next blocks (138 us).
 #include <cuda.h>
 
 #include <algorithm>
@@ -72,7 +73,7 @@ struct GemmArgs {
   const int32_t* offsets;  // [E + 1], null: one matrix, all S rows
   void* out;             // [S][N]
   int copy_out;          // its rows lie on 16 bytes
-  int S, N, K, E, KB, NB;
+  int S, N, E, KB, NB;
   uint32_t* err;
 };
 
@@ -319,7 +320,6 @@ int launch_fp8_gemm(cudaStream_t s, const Fp8Product& p, int out_dtype) {
   a.out = p.out;
   a.S = p.S;
   a.N = p.N;
-  a.K = p.K;
   a.E = p.E;
   a.KB = (p.K + kFp8Block - 1) / kFp8Block;
   a.NB = (p.N + kFp8Block - 1) / kFp8Block;

@@ -19,7 +19,6 @@
 // a value is stored in fewer bits.
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
 #include "common.cuh"
 #include "internal.h"
