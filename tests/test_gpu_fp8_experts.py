@@ -514,6 +514,19 @@ def test_empty_batches(ops):
 
 
 @pytest.mark.gpu
+def test_gradients_refuse_a_second_differentiation(ops):
+    """A gradient of a gradient is refused, not left out."""
+    g = rng(2)
+    ids = routes(g, 5, 2, 4)
+    x = randn(g, 5, 32).requires_grad_()
+    w, ws = weights(g, 48, 32)
+    p = ops.permute.permute(x, ids, 4)
+    for y in (p.rows, ops.permute.unpermute(p.rows, p.row_of_route), ops.fp8.linear(x, w, ws)):
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(y.sum(), x, create_graph=True, retain_graph=True)
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits(ops):
     """2.4 million rows of 1024: elements past 2^31 in every operator; the last rows are looked at."""
     g = rng(31)

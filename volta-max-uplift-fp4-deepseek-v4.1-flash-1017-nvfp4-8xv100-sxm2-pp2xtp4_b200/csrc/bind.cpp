@@ -74,6 +74,8 @@ void want(const char* name, const Tensor& t, Kind kind, int64_t dim, const Tenso
                     " axes, got ", t.scalar_type(), " ", t.sizes());
   TORCH_CHECK_VALUE(t.is_contiguous() || (rows && t.stride(-1) == 1 && t.stride(0) >= t.size(1)), name, " must ",
                     rows ? "have contiguous rows" : "be contiguous", ", got strides ", t.strides());
+  TORCH_CHECK_VALUE(t.size(0) <= INT32_MAX && (dim < 2 || t.size(-1) <= INT32_MAX), name, " is too large: ",
+                    t.sizes());
   TORCH_CHECK_VALUE(!like || t.device() == like->device(), name, " is on ", t.device(), ", the other arguments on ",
                     like ? like->device().str() : "");
 }
@@ -175,6 +177,11 @@ std::tuple<Tensor, Tensor> run_unpermute_grad(const Tensor& grad, const Tensor& 
   return {grad_rows, grad_weights};
 }
 
+// The gradients have no graph of their own: asked for one (create_graph), they refuse instead of leaving it out.
+void once_differentiable() {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), "this operator's gradient cannot be differentiated again");
+}
+
 // A gradient as the kernels read it: contiguous columns, rows at any distance.
 Tensor as_rows(const Tensor& grad) {
   return grad.stride(-1) == 1 && grad.stride(0) >= grad.size(1) ? grad : grad.contiguous();
@@ -189,6 +196,7 @@ struct PermuteFn : torch::autograd::Function<PermuteFn> {
     return {rows, row_of_route, offsets};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_differentiable();
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
     return {run_unpermute(grads[0].contiguous(), ctx->get_saved_variables()[0], Tensor(), grads[0].scalar_type()),
             Tensor(), Tensor()};
@@ -202,6 +210,7 @@ struct UnpermuteFn : torch::autograd::Function<UnpermuteFn> {
     return run_unpermute(rows, row_of_route, weights.value_or(Tensor()), out_dtype);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_differentiable();
     const auto saved = ctx->get_saved_variables();
     const bool need_weights = saved[2].defined() && ctx->needs_input_grad(2);
     const auto [grad_rows, grad_weights] = run_unpermute_grad(as_rows(grads[0]), saved[0], saved[1], saved[2],
@@ -436,6 +445,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     return run_linear(x, w, w_scale, out_dtype);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_differentiable();
     const auto saved = ctx->get_saved_variables();
     Tensor wt = saved[0], wt_scale = saved[1];
     if (!ctx->saved_data["transposed"].toBool()) std::tie(wt, wt_scale) = run_transpose(wt, wt_scale);

@@ -171,7 +171,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int b = 0, staged = -1;
     uint32_t bph = 0;
     bool ok = true;
-    for (int item = first; ok && item < stop; ++item) {
+    // after a wait that ran out the items still pass, without waits and stores: the four warps meet at the same barriers
+    for (int item = first; item < stop; ++item) {
       const int e = tile_expert(start, a.E, item), local = item - start[e];
       const int row0 = off[e] + local / n_wt * NTOK, end = off[e + 1], n0 = local % n_wt * kRows;
       if (row0 != staged) {  // a new token tile: its scales, by K block
@@ -221,12 +222,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (++b == kBufs) b = 0, bph ^= 1u;
         }
       }
-      if (!ok) {
-        *abort_ptr = 1;
-        break;
-      }
+      if (!ok) *abort_ptr = 1;
       const int col = n0 + quarter * 32 + lane;
-      if (col < a.N) {
+      if (ok && col < a.N) {
 #pragma unroll
         for (int i = 0; i < NTOK; ++i)
           if (row0 + i < end) out[int64_t(row0 + i) * a.N + col] = from_f32<TO>(acc[i]);

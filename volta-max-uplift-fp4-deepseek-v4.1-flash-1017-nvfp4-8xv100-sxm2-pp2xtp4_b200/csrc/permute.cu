@@ -541,7 +541,7 @@ extern "C" int b200moe_permute(void* stream, const int32_t* ids, int num_experts
 
 extern "C" int b200moe_unpermute(void* stream, const void* rows, int dtype, const int32_t* row_of_route,
                                  const float* weights, int T, int k, int H, void* out, int out_dtype) {
-  if (!rows || !row_of_route || !out || !sizes_ok(T, k) || H < 1) return B200MOE_ERR_INVALID_ARG;
+  if (!rows || !row_of_route || !out || !sizes_ok(T, k) || H < 1 || H > (1 << 28)) return B200MOE_ERR_INVALID_ARG;
   if (dtype < 0 || dtype > B200MOE_F32 || (out_dtype != dtype && out_dtype != B200MOE_F32)) return B200MOE_ERR_DTYPE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint32_t* err = op_error_word();
@@ -556,7 +556,7 @@ extern "C" int b200moe_unpermute(void* stream, const void* rows, int dtype, cons
 extern "C" int b200moe_unpermute_grad(void* stream, const void* grad, int grad_dtype, int64_t grad_stride,
                                       const void* rows, int dtype, const int32_t* row_of_route, const float* weights,
                                       int T, int k, int H, void* grad_rows, float* grad_weights) {
-  if (!grad || !row_of_route || !sizes_ok(T, k) || H < 1 || grad_stride < 0 || (!grad_rows && !grad_weights) ||
+  if (!grad || !row_of_route || !sizes_ok(T, k) || H < 1 || H > (1 << 28) || grad_stride < 0 || (!grad_rows && !grad_weights) ||
       (grad_weights && !rows))
     return B200MOE_ERR_INVALID_ARG;
   if (dtype < 0 || dtype > B200MOE_F32 || (grad_dtype != dtype && grad_dtype != B200MOE_F32)) return B200MOE_ERR_DTYPE;

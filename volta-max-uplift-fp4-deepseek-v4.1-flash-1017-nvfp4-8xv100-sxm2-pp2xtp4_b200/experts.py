@@ -83,6 +83,7 @@ class _Experts(torch.autograd.Function):
         return unpermute(y, row_of_route, topk_weights)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         h, y, row_of_route, offsets, w = ctx.saved_tensors
         m = ctx.experts
