@@ -19,7 +19,7 @@ constexpr int kQuantThreads = 256;
 constexpr int kQuantBlocks = kQuantThreads / 8;  // row blocks of a CTA's turn
 // CTAs at most, for walks of several turns: SwiGLU of 49152 x 1408 takes 70 us with 16 per SM, 72 with 8 and 77
 // without a cap, its gradient 102 us with 48 per SM, 116 without a cap and 108 with 16
-constexpr int64_t kCtaCap = 148 * 16, kGradCap = 148 * 48;
+constexpr int64_t kCtaCap = 148 * 16, kGradCap = 148 * 48, kAnyCap = 148 * 32;
 
 // Minimum / maximum that keep a NaN.
 __device__ __forceinline__ float min_nan(float a, float b) {
@@ -107,7 +107,7 @@ __device__ __forceinline__ void load8(const T* p, int64_t left, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] = !WIDE && i < left ? to_f32(p[i]) : 0.f;
 }
 
-// Eight lanes per block, sixteen columns each: what a block costs beside its values (its place, the maximum's
+// Rows of whole aligned vectors: eight lanes per block, sixteen columns each: what a block costs beside its values (its place, the maximum's
 // shuffles, the division) is shared by sixteen values per lane. Several blocks are in flight before the first is
 // worked on.
 template <typename T, bool SWIGLU>
@@ -115,7 +115,7 @@ __host__ __device__ constexpr int blocks_in_flight() {
   return SWIGLU || sizeof(T) == 4 ? 1 : 2;
 }
 
-template <typename T, bool SWIGLU, bool WIDE>
+template <typename T, bool SWIGLU>
 __global__ void __launch_bounds__(kQuantThreads) fp8_rows_kernel(const T* __restrict__ x, int64_t x_stride, int rows,
                                                                  int width, float limit, int d_row, int d_b,
                                                                  uint8_t* __restrict__ q, float* __restrict__ scale) {
@@ -141,8 +141,8 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_rows_kernel(const T* __rest
       const T* src = x + row[u] * x_stride + c[u];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        load8<T, WIDE>(src + 8 * h, left - 8 * h, v[u][h]);
-        if constexpr (SWIGLU) load8<T, WIDE>(src + width + 8 * h, left - 8 * h, w[u][h]);
+        load8<T, true>(src + 8 * h, left - 8 * h, v[u][h]);
+        if constexpr (SWIGLU) load8<T, true>(src + width + 8 * h, left - 8 * h, w[u][h]);
       }
     }
 #pragma unroll
@@ -168,15 +168,59 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_rows_kernel(const T* __rest
         const float(&y)[8] = v[u][h];
         const uint32_t lo = e4m3x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
         const uint32_t hi = e4m3x4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv);
-        if (WIDE) {
-          if (c[u] + 8 * h < width) *reinterpret_cast<uint2*>(dst + 8 * h) = make_uint2(lo, hi);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c[u] + 8 * h + i < width) dst[8 * h + i] = uint8_t((i < 4 ? lo : hi) >> (8 * (i & 3)));
-        }
+        if (c[u] + 8 * h < width) *reinterpret_cast<uint2*>(dst + 8 * h) = make_uint2(lo, hi);
       }
       if (l == 1) scale[row[u] * nb + c[u] / kFp8Block] = ratio;
+    }
+  }
+}
+
+// Rows of any width and alignment: a warp per block, single columns 32 apart, so that a warp's access is one run of
+// bytes; several blocks in flight.
+template <typename T, bool SWIGLU>
+__global__ void __launch_bounds__(kQuantThreads) fp8_rows_any_kernel(const T* __restrict__ x, int64_t x_stride, int rows,
+                                                                     int width, float limit, int d_row, int d_b,
+                                                                     uint8_t* __restrict__ q,
+                                                                     float* __restrict__ scale) {
+  constexpr int U = SWIGLU ? 2 : 4;
+  const int nb = (width + kFp8Block - 1) / kFp8Block, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
+  Walk at(int64_t(blockIdx.x) * (kQuantThreads / 32) + threadIdx.x / 32, nb);
+  while (at.row < rows) {
+    Vec<T, 4> v[U], w[SWIGLU ? U : 1];
+    int64_t row[U];
+    int c[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      row[u] = at.row;
+      c[u] = at.b * kFp8Block + lane;
+      at.next(d_row, d_b, nb);
+      const int n = row[u] < rows ? width : 0;
+      const T* src = x + row[u] * x_stride;
+      load_columns<false>(v[u], src, c[u], 32, n);
+      if constexpr (SWIGLU) load_columns<false>(w[u], src + width, c[u], 32, n);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (row[u] >= rows) break;  // the same for the whole warp
+      float y[4], m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[i] = v[u].get(i);
+        if constexpr (SWIGLU) y[i] = swiglu(y[i], w[u].get(i), limit);
+        m = max_nan(m, fabsf(y[i]));
+      }
+      const uint32_t amax_bits = __reduce_max_sync(0xffffffffu, abs_bits(m));  // a NaN is above every value
+      const float amax = max_nan(__uint_as_float(amax_bits), kAmaxFloor);
+      const float ratio = __fdiv_rn(lane & 1 ? amax : kE4m3Max, lane & 1 ? kE4m3Max : amax);
+      const float inv = __shfl_sync(0xffffffffu, ratio, 0);
+      const uint32_t o = e4m3x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+      uint8_t* dst = q + row[u] * width;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c[u] + 32 * i < width) dst[c[u] + 32 * i] = uint8_t(o >> (8 * i));
+      if (lane == 1) scale[row[u] * nb + c[u] / kFp8Block] = ratio;
     }
   }
 }
@@ -187,37 +231,31 @@ __global__ void __launch_bounds__(kQuantThreads) swiglu_grad_kernel(const T* __r
                                                                     const T* __restrict__ grad, int64_t grad_stride,
                                                                     int rows, int width, float limit, int d_row,
                                                                     int d_b, T* __restrict__ grad_h) {
-  const int per_row = (width + 7) / 8;
+  // WIDE: a thread's eight consecutive columns; else a warp's 256, eight single ones per thread, 32 apart
+  const int per_row = WIDE ? (width + 7) / 8 : (width + 255) / 256, step = WIDE ? 0 : 32;
+  const int64_t first = int64_t(blockIdx.x) * kQuantThreads + threadIdx.x;
   pdl_wait();
   pdl_trigger();
-  for (Walk at(int64_t(blockIdx.x) * kQuantThreads + threadIdx.x, per_row); at.row < rows;
-       at.next(d_row, d_b, per_row)) {
-    const int c = at.b * 8;
-    const int left = width - c;
-    float gate[8], up[8], d[8], dg[8], du[8];
-    load8<T, WIDE>(h + at.row * h_stride + c, left, gate);
-    load8<T, WIDE>(h + at.row * h_stride + width + c, left, up);
-    load8<T, WIDE>(grad + at.row * grad_stride + c, left, d);
+  for (Walk at(WIDE ? first : first / 32, per_row); at.row < rows; at.next(d_row, d_b, per_row)) {
+    const int c = WIDE ? at.b * 8 : at.b * 256 + (threadIdx.x & 31);
+    if (c >= width) continue;
+    Vec<T, 8> gate, up, d;
+    load_columns<WIDE>(gate, h + at.row * h_stride, c, step, width);
+    load_columns<WIDE>(up, h + at.row * h_stride + width, c, step, width);
+    load_columns<WIDE>(d, grad + at.row * grad_stride, c, step, width);
+    float dg[8], du[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float g = limited_gate(gate[i], limit), u = limited_up(up[i], limit);
+      const float g0 = gate.get(i), u0 = up.get(i), di = d.get(i);
+      const float g = limited_gate(g0, limit), u = limited_up(u0, limit);
       const float s = quotient(1.f, one_plus_exp_neg(g));
       const float gs = g * s;
-      dg[i] = gate[i] > limit ? 0.f : d[i] * u * fmaf(gs, 1.f - s, s);
-      du[i] = fabsf(up[i]) > limit ? 0.f : d[i] * gs;
+      dg[i] = g0 > limit ? 0.f : di * u * fmaf(gs, 1.f - s, s);
+      du[i] = fabsf(u0) > limit ? 0.f : di * gs;
     }
-    T* dst = grad_h + at.row * 2 * width + c;
-    if (WIDE) {
-      store_vec<T, 8>(dst, dg);
-      store_vec<T, 8>(dst + width, du);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < left) {
-          dst[i] = from_f32<T>(dg[i]);
-          dst[width + i] = from_f32<T>(du[i]);
-        }
-    }
+    T* dst = grad_h + at.row * 2 * width;
+    store_columns<WIDE>(dst, c, step, width, dg);
+    store_columns<WIDE>(dst + width, c, step, width, du);
   }
 }
 
@@ -320,10 +358,11 @@ cudaError_t run_rows(cudaStream_t s, const void* x, int64_t x_stride, int rows, 
   const bool w = width % 8 == 0 && wide(x, x_stride * int64_t(sizeof(T)), 16) &&
                  (!SWIGLU || (width * int64_t(sizeof(T))) % 16 == 0) && wide(q, 8, 8);
   const int nb = (width + kFp8Block - 1) / kFp8Block;
-  const int64_t turn = kQuantBlocks * blocks_in_flight<T, SWIGLU>();
-  const int64_t blocks = std::min<int64_t>((int64_t(rows) * nb + turn - 1) / turn, kCtaCap);
-  const int64_t step = blocks * kQuantBlocks;
-  auto kernel = w ? fp8_rows_kernel<T, SWIGLU, true> : fp8_rows_kernel<T, SWIGLU, false>;
+  const int per_cta = w ? kQuantBlocks : kQuantThreads / 32;
+  const int64_t turn = per_cta * (w ? blocks_in_flight<T, SWIGLU>() : SWIGLU ? 2 : 4);
+  const int64_t blocks = std::min<int64_t>((int64_t(rows) * nb + turn - 1) / turn, w ? kCtaCap : kAnyCap);
+  const int64_t step = blocks * per_cta;
+  auto kernel = w ? fp8_rows_kernel<T, SWIGLU> : fp8_rows_any_kernel<T, SWIGLU>;
   return launch_chain(kernel, dim3(unsigned(blocks)), dim3(kQuantThreads), 0, s, static_cast<const T*>(x), x_stride,
                       rows, width, limit, int(step / nb), int(step % nb), q, scale);
 }
@@ -333,9 +372,9 @@ cudaError_t run_swiglu_grad(cudaStream_t s, const void* h, int64_t h_stride, con
                             int rows, int width, float limit, void* grad_h) {
   const int64_t b = sizeof(T);
   const bool w = width % 8 == 0 && wide(h, h_stride * b, 16) && wide(grad, grad_stride * b, 16) && wide(grad_h, 16, 16);
-  const int per_row = (width + 7) / 8;
-  const int64_t blocks = std::min<int64_t>((int64_t(rows) * per_row + kQuantThreads - 1) / kQuantThreads, kGradCap);
-  const int64_t step = blocks * kQuantThreads;
+  const int per_row = w ? (width + 7) / 8 : (width + 255) / 256, units = w ? kQuantThreads : kQuantThreads / 32;
+  const int64_t blocks = std::min<int64_t>((int64_t(rows) * per_row + units - 1) / units, kGradCap);
+  const int64_t step = blocks * units;
   auto kernel = w ? swiglu_grad_kernel<T, true> : swiglu_grad_kernel<T, false>;
   return launch_chain(kernel, dim3(unsigned(blocks)), dim3(kQuantThreads), 0, s, static_cast<const T*>(h), h_stride,
                       static_cast<const T*>(grad), grad_stride, rows, width, limit, int(step / per_row),

@@ -31,6 +31,7 @@ constexpr int kRunRoutes = 2048;  // routes that one CTA ranks: 64 per warp
 constexpr int kSortMaxExperts = 1024;
 constexpr int kUnpermuteCtas = 12;  // per SM: several waves even out the rows' latencies
 constexpr int kGradCtas = 12;
+constexpr int kColumns = 4;  // single columns per thread where rows are not whole aligned vectors
 constexpr int kSortMaxRoutes = 1 << 26;
 
 // ------------------------------------------------------------------ sort
@@ -181,7 +182,7 @@ __device__ __forceinline__ void copy_token(const CopyArgs& a, int t, const int32
   const int64_t row_bytes = int64_t(a.pieces) * sizeof(V);
   const int S = a.T * a.k;
   const V* src = reinterpret_cast<const V*>(a.x + t * a.x_stride);
-  constexpr int U = 2;
+  constexpr int U = sizeof(V) == 16 ? 2 : 8;  // pieces in flight
   for (int c0 = threadIdx.x; c0 < a.pieces; c0 += U * blockDim.x) {
     V v[U];
 #pragma unroll
@@ -241,16 +242,17 @@ __global__ void __launch_bounds__(1024) sort_permute_kernel(const int32_t* __res
 }
 
 // ------------------------------------------------------- weighted return
-// A thread owns V columns of its CTA's tokens; eight slots' rows are in flight
+// A thread owns V columns (of `load_columns`) of its CTA's tokens; eight slots' rows are in flight
 // before the first is added, and the next token's routes are loaded (a lane per
 // slot) while they are.
-template <typename TI, typename TO, int V>
+template <typename TI, typename TO, int V, bool WIDE>
 __global__ void __launch_bounds__(256) unpermute_kernel(const TI* __restrict__ rows, const int32_t* __restrict__ row_of_route,
                                                         const float* __restrict__ weights, int T, int k, int H,
                                                         TO* __restrict__ out, uint32_t* err) {
   constexpr int U = 8;
   const int S = T * k, slot = threadIdx.x & (U - 1);
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
+  const int step = blockDim.x;
+  const int c = blockIdx.y * step * V + (WIDE ? threadIdx.x * V : threadIdx.x);
   pdl_wait();
   pdl_trigger();
   auto routes = [&](int t, int s0, int& r, float& w) {
@@ -281,7 +283,7 @@ __global__ void __launch_bounds__(256) unpermute_kernel(const TI* __restrict__ r
       if (c < H) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (r[u] >= 0) y[u].load(rows + int64_t(r[u]) * H + c);
+          if (r[u] >= 0) load_columns<WIDE>(y[u], rows + int64_t(r[u]) * H, c, step, H);
       }
       const bool more = s0 + U < k;
       routes(more ? t : t + gridDim.x, more ? s0 + U : 0, r_next, w_next);
@@ -294,7 +296,7 @@ __global__ void __launch_bounds__(256) unpermute_kernel(const TI* __restrict__ r
         }
       }
     }
-    if (c < H) store_vec<TO, V>(out + int64_t(t) * H + c, acc);
+    if (c < H) store_columns<WIDE>(out + int64_t(t) * H, c, step, H, acc);
   }
 }
 
@@ -323,8 +325,8 @@ __device__ __forceinline__ float warp_sum8(const float (&v)[8], int lane) {
 // A CTA per token: g[t] is read once for up to eight slots; each slot's row is
 // read for the dot product and its gradient row written in the same pass.
 // Three CTAs per SM where the registers allow it: 95 us at 4096 tokens of 8 x 4096, 99 with two.
-template <typename TG, typename TI, int V>
-__global__ void __launch_bounds__(256, V > 1 && sizeof(TI) == 2 ? 3 : 2) unpermute_grad_kernel(const TG* __restrict__ grad, int64_t grad_stride,
+template <typename TG, typename TI, int V, bool WIDE>
+__global__ void __launch_bounds__(256, WIDE && sizeof(TI) == 2 ? 3 : 2) unpermute_grad_kernel(const TG* __restrict__ grad, int64_t grad_stride,
                                                              const TI* __restrict__ rows,
                                                              const int32_t* __restrict__ row_of_route,
                                                              const float* __restrict__ weights, int T, int k, int H,
@@ -361,14 +363,15 @@ __global__ void __launch_bounds__(256, V > 1 && sizeof(TI) == 2 ? 3 : 2) unpermu
       }
       const bool more = s0 + U < k;
       routes(more ? t : t + gridDim.x, more ? s0 + U : 0, r_next, w_next);
-      for (int c = threadIdx.x * V; c < H; c += blockDim.x * V) {
+      const int step = blockDim.x;
+      for (int c = WIDE ? threadIdx.x * V : threadIdx.x; c < H; c += step * V) {
         Vec<TG, V> g;
         Vec<TI, V> y[U];
-        g.load(grad + t * grad_stride + c);
+        load_columns<WIDE>(g, grad + t * grad_stride, c, step, H);
         if (grad_weights) {
 #pragma unroll
           for (int u = 0; u < U; ++u)
-            if (r[u] >= 0 && r[u] < S) y[u].load(rows + int64_t(r[u]) * H + c);
+            if (r[u] >= 0 && r[u] < S) load_columns<WIDE>(y[u], rows + int64_t(r[u]) * H, c, step, H);
         }
         float gv[V];
 #pragma unroll
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(256, V > 1 && sizeof(TI) == 2 ? 3 : 2) unpermu
             float o[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) o[i] = r[u] >= 0 ? w[u] * gv[i] : 0.f;  // zeros also where g is not finite
-            store_vec<TI, V>(grad_rows + int64_t(r[u] >= 0 ? r[u] : ~r[u]) * H + c, o);
+            store_columns<WIDE>(grad_rows + int64_t(r[u] >= 0 ? r[u] : ~r[u]) * H, c, step, H, o);
           }
         }
       }
@@ -411,12 +414,12 @@ cudaError_t run_unpermute(cudaStream_t s, const void* rows, const int32_t* row_o
                           int k, int H, void* out, uint32_t* err) {
   constexpr int VB = 16 / sizeof(TI);
   const bool wide = H % VB == 0 && aligned(rows, 16, 16) && aligned(out, 16, 16);
-  const int V = wide ? VB : 1;
+  const int V = wide ? VB : kColumns;
   const int cols = (H + V - 1) / V;
   const int threads = std::min(256, (cols + 31) / 32 * 32);
   const int slices = (cols + threads - 1) / threads;
   const dim3 grid(std::min(T, std::max(1, sm_count() * kUnpermuteCtas / slices)), slices);
-  auto kernel = wide ? unpermute_kernel<TI, TO, VB> : unpermute_kernel<TI, TO, 1>;
+  auto kernel = wide ? unpermute_kernel<TI, TO, VB, true> : unpermute_kernel<TI, TO, kColumns, false>;
   return launch_chain(kernel, grid, dim3(threads), 0, s, static_cast<const TI*>(rows), row_of_route, weights, T, k, H,
                       static_cast<TO*>(out), err);
 }
@@ -428,9 +431,9 @@ cudaError_t run_unpermute_grad(cudaStream_t s, const void* grad, int64_t grad_st
   constexpr int VB = 16 / sizeof(TI);
   const bool wide = H % VB == 0 && aligned(rows, 16, 16) && aligned(grad, grad_stride * int64_t(sizeof(TG)), 16) &&
                     aligned(grad_rows, 16, 16);
-  const int V = wide ? VB : 1;
+  const int V = wide ? VB : kColumns;
   const int threads = std::min(256, ((H + V - 1) / V + 31) / 32 * 32);
-  auto kernel = wide ? unpermute_grad_kernel<TG, TI, VB> : unpermute_grad_kernel<TG, TI, 1>;
+  auto kernel = wide ? unpermute_grad_kernel<TG, TI, VB, true> : unpermute_grad_kernel<TG, TI, kColumns, false>;
   return launch_chain(kernel, dim3(std::min(T, sm_count() * kGradCtas)), dim3(threads), 0, s, static_cast<const TG*>(grad),
                       grad_stride, static_cast<const TI*>(rows), row_of_route, weights, T, k, H,
                       static_cast<TI*>(grad_rows), grad_weights, err);

@@ -76,4 +76,28 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[V]) {
   o.store(p);
 }
 
+// V columns of a row per thread: WIDE, consecutive ones from c (whole aligned
+// vectors); else single ones, `step` apart, those below n. The second form serves
+// rows of any width and alignment: neighbouring threads hold neighbouring columns,
+// so a warp's access is one run of bytes, and V of them are in flight per thread.
+template <bool WIDE, typename T, int V>
+__device__ __forceinline__ void load_columns(Vec<T, V>& y, const T* row, int c, int step, int n) {
+  if constexpr (WIDE) {
+    y.load(row + c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) y.v[i] = c + i * step < n ? row[c + i * step] : from_f32<T>(0.f);
+  }
+}
+template <bool WIDE, typename T, int V>
+__device__ __forceinline__ void store_columns(T* row, int c, int step, int n, const float (&x)[V]) {
+  if constexpr (WIDE) {
+    store_vec<T, V>(row + c, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c + i * step < n) row[c + i * step] = from_f32<T>(x[i]);
+  }
+}
+
 }  // namespace b200moe
