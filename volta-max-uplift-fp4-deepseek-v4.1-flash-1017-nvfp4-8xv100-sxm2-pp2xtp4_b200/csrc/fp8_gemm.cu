@@ -7,7 +7,7 @@
 // of 128 rows x BN columns; per K block
 //   warp 0 (producer): two TMA boxes (128 rows of a, BN rows of w; 128 columns,
 //     128-byte swizzle) into a ring of stages;
-//   warp 1 (MMA): one lane issues 4 x tcgen05.mma.kind::f8f6f4 (M 128, N BN,
+//   warp 1 (MMA; at BN = 128 also warp 2, a block each in turn): one lane issues 4 x tcgen05.mma.kind::f8f6f4 (M 128, N BN,
 //     K 32) into one of the TMEM buffers of BN columns and commits; the whole
 //     warp runs the loop, so that its operands stay in uniform registers (issued
 //     by a lone lane of a diverged warp the four MMAs take 345 clocks);
@@ -46,7 +46,7 @@ namespace {
 
 constexpr int kBM = 128;
 constexpr int kSumWarps = 8;
-constexpr int kSumWarp0 = 4;  // warps 0-3: producer, MMA, two without work (a register share is a group of four)
+constexpr int kSumWarp0 = 4;  // warps 0-3: producer, MMA, the rest without work (a register share is a group of four)
 constexpr int kThreads = (kSumWarp0 + kSumWarps) * 32;
 // registers per thread: the launch's 384 x 168 split as 128 x 40 + 256 x 232
 constexpr int kFewRegs = 40, kSumRegs = 232;
@@ -60,6 +60,9 @@ struct Cfg {
   static constexpr int kWBytes = BN * kFp8Block;
   static constexpr int kStages = BN == 256 ? 4 : 6;
   static constexpr int kBufs = 512 / BN > 4 ? 4 : 512 / BN;  // TMEM buffers
+  // at BN = 128 a block's issue takes as long as its MMAs: 333 x 2816 x 2048 in 7.3 us with two warps, 8.5 with one; at
+  // 256 the sums are the longer part either way
+  static constexpr int kMmaWarps = BN == 128 ? 2 : 1;
   static constexpr int kCols = BN / 2;                        // columns per sum thread
   static constexpr size_t kSmem = 1024 + size_t(kStages) * (kABytes + kWBytes) + kSumWarps * kOutBytes + 256;
   static constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
@@ -136,7 +139,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int e = tile_expert(start, a.E, item), local = item - start[e];
         const int row = off[e] + local / n_nt * kBM, wrow = e * a.N + local % n_nt * BN;
         for (int kb = 0; kb < a.KB; ++kb) {
-          ok = __all_sync(0xffffffffu, !*abort_ptr && mbar_poll(&empty[st], ph ^ 1u, a.err));
+          ok = !__any_sync(0xffffffffu, *abort_ptr) && poll_warp(&empty[st], ph ^ 1u, a.err);
           if (!ok) break;
           if (elect_one()) {
             mbar_arrive_expect_tx(&full[st], uint32_t(kABytes + C::kWBytes));
@@ -151,34 +154,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) *abort_ptr = 1;
       // no copy may be in flight when the CTA exits
       for (int s = 0; s < ST; ++s)
-        if (issued & (1u << s)) mbar_poll(&full[s], (par >> s) & 1u, a.err);
+        if (issued & (1u << s)) poll_warp(&full[s], (par >> s) & 1u, a.err);
     }
-    if (warp == 1) {
-      int st = 0, b = 0, last = 0;
+    if (warp >= 1 && warp <= C::kMmaWarps) {
+      // the warps take the K blocks in turn, whatever their tiles: a block's issue by one then runs beside another's
+      // waits. Stages and buffers are multiples of them, so that each stays with one warp: were a stage shared, one warp
+      // could wait for its second filling before the first has landed, and a parity wait would take the phase before
+      // for it.
+      constexpr int MW = C::kMmaWarps;
+      static_assert(ST % MW == 0 && NBUF % MW == 0, "stages and buffers by MMA warp");
+      const int tiles = int(blockIdx.x) < n_items ? (n_items - 1 - int(blockIdx.x)) / int(gridDim.x) + 1 : 0;
+      const int64_t total = int64_t(tiles) * a.KB;
+      int st = warp - 1, b = st, last = 0;
       uint32_t ph = 0, bph = 0, last_ph = 0;
       bool ok = true, committed = false;
       const uint64_t da0 = desc_sw128(smem_u32(at)), dw0 = desc_sw128(smem_u32(wt));
-      for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x) {
-        for (int kb = 0; kb < a.KB; ++kb) {
-          ok = __all_sync(0xffffffffu, mbar_poll(&full[st], ph, a.err) && mbar_poll(&acc_empty[b], bph ^ 1u, a.err));
-          if (!ok) break;
-          fence_after();
-          const uint64_t da = da0 + st * (kABytes >> 4), dw = dw0 + st * (C::kWBytes >> 4);
-          if (elect_one()) {
-            mma_block(tmem + b * BN, da, dw, C::kIdesc);
-            commit(&empty[st]);
-            commit(&acc_full[b]);
-          }
-          __syncwarp();
-          committed = true;
-          last = b;
-          last_ph = bph;
-          if (++st == ST) st = 0, ph ^= 1u;
-          if (++b == NBUF) b = 0, bph ^= 1u;
+      for (int64_t g = st; g < total; g += MW) {
+        ok = poll_warp(&full[st], ph, a.err) && poll_warp(&acc_empty[b], bph ^ 1u, a.err);
+        if (!ok) break;
+        fence_after();
+        const uint64_t da = da0 + st * (kABytes >> 4), dw = dw0 + st * (C::kWBytes >> 4);
+        if (elect_one()) {
+          mma_block(tmem + b * BN, da, dw, C::kIdesc);
+          commit(&empty[st]);
+          commit(&acc_full[b]);
         }
+        __syncwarp();
+        committed = true;
+        last = b;
+        last_ph = bph;
+        if ((st += MW) >= ST) st -= ST, ph ^= 1u;
+        if ((b += MW) >= NBUF) b -= NBUF, bph ^= 1u;
       }
       if (!ok) *abort_ptr = 1;
-      if (committed) mbar_poll(&acc_full[last], last_ph, a.err);
+      if (committed) poll_warp(&acc_full[last], last_ph, a.err);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
@@ -214,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int ahead = min(kb + kAhead, a.KB - 1);
           fa[j] = __ldg(sa + ahead);
           fb[j] = __ldg(sb + ahead);
-          ok = __all_sync(0xffffffffu, mbar_poll(&acc_full[b], bph, a.err));
+          ok = poll_warp(&acc_full[b], bph, a.err);
           if (!ok) break;
           fence_after();
           const uint32_t addr = lanes + b * BN;

@@ -15,10 +15,9 @@
 //     f32 sums of its NTOK columns.
 // 190 experts of 4096 x 4096 for 256 rows: 461 us, 6.95 TB/s, the rate of a plain
 // copy and a little more (it reads only). Streaming the weights through registers
-// into mma.sync instead reached 4.9 TB/s at best: a warp's loads in flight share
-// its few scoreboards, and the conversions to f16 take issue slots. One matrix of
-// 4096 x 4096 for 64 rows has 32 x 4 items and takes 9.2 us: 0.18 per K block, 3 for
-// launch, first bytes and stores; with one MMA warp 10.7.
+// into mma.sync instead reached 4.9 TB/s at best. One matrix of 4096 x 4096 for 64
+// rows has 32 x 4 items and takes 9.2 us: 0.18 per K block, 3 for launch, first
+// bytes and stores; with one MMA warp 10.7.
 #include <cuda.h>
 
 #include <algorithm>
@@ -120,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int e = tile_expert(start, a.E, item), local = item - start[e];
       const int row = off[e] + local / n_wt * NTOK, wrow = e * a.N + local % n_wt * kRows;
       for (int kb = 0; kb < a.KB; ++kb) {
-        ok = __all_sync(0xffffffffu, !*abort_ptr && mbar_poll(&empty[st], ph ^ 1u, a.err));
+        ok = !__any_sync(0xffffffffu, *abort_ptr) && poll_warp(&empty[st], ph ^ 1u, a.err);
         if (!ok) break;
         if (elect_one()) {
           uint8_t* dst = stages + st * C::kStage;
@@ -136,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok) *abort_ptr = 1;
     // no copy may be in flight when the CTA exits
     for (int s = 0; s < ST; ++s)
-      if (issued & (1u << s)) mbar_poll(&full[s], (par >> s) & 1u, a.err);
+      if (issued & (1u << s)) poll_warp(&full[s], (par >> s) & 1u, a.err);
   } else if (warp == 1 || warp == 6) {
     // two warps take the K blocks in turn, whatever their items: one block's four MMAs and two commits take 250 clocks
     // to issue, where its bytes arrive in 180
@@ -146,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true, committed = false;
     const uint64_t d0 = desc_sw128(smem_u32(stages));
     for (int64_t g = st; ok && g < total; g += 2) {
-      ok = __all_sync(0xffffffffu, mbar_poll(&full[st], ph, a.err) && mbar_poll(&acc_empty[b], bph ^ 1u, a.err));
+      ok = poll_warp(&full[st], ph, a.err) && poll_warp(&acc_empty[b], bph ^ 1u, a.err);
       if (!ok) break;
       fence_after();
       const uint64_t d = d0 + st * (C::kStage >> 4);
@@ -163,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if ((b += 2) >= kBufs) b -= kBufs, bph ^= 1u;
     }
     if (!ok) *abort_ptr = 1;
-    if (committed) mbar_poll(&acc_full[last], last_ph, a.err);
+    if (committed) poll_warp(&acc_full[last], last_ph, a.err);
   } else {
     const int quarter = warp & 3, tid = threadIdx.x - 64;
     const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
@@ -197,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (kb >= a.KB) break;
           const float f = fb[j];
           fb[j] = __ldg(sb + min(kb + kAhead, a.KB - 1));
-          ok = __all_sync(0xffffffffu, mbar_poll(&acc_full[b], bph, a.err));
+          ok = poll_warp(&acc_full[b], bph, a.err);
           if (!ok) break;
           fence_after();
           const float4* s4 = reinterpret_cast<const float4*>(ss + kb * NTOK);
