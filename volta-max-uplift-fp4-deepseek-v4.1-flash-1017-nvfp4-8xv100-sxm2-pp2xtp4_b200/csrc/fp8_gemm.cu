@@ -21,11 +21,11 @@
 // and MMAs before TMEM is freed.
 //
 // Bound: at BN = 256 a block's MMAs take 516 clocks by themselves, beside copies,
-// TMEM reads and sums too (each measured apart), and the kernel takes about 800 a
+// TMEM reads and sums too (each measured apart), and the kernel takes about 780 a
 // block: the sums 470 (256 fused multiply-adds and 256 columns of TMEM reads per
 // scheduler), and with two buffers their waits, the issue and the commit's arrival
 // (290 together) and the MMA warp's turns among the sums' instructions are not
-// hidden. 8192 x 4096 x 4096: 129 us, 2.12 PFLOP/s, the tensor pipe 55 % busy.
+// hidden. 8192 x 4096 x 4096: 126 us, 2.18 PFLOP/s, the tensor pipe 59 % busy.
 // Measured and not kept: sums by packed f32x2 (157 us: half the rate of the scalar
 // ones), by sixteen warps (151 us), from 16 columns at a time (167 us), blocks in
 // halves of 128 columns with barriers of their own (138 us), the factors computed by
