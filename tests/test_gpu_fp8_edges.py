@@ -1,0 +1,73 @@
+"""Edges of the FP8 expert path's operators: extreme values, ranges, refusals and the sizes where one kernel gives way
+to the next.  Expected values are plain torch forms in 64 bits, or in f32 step by step where the definition fixes
+every rounding."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+E4M3 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def ops(pkg):
+    from b200moe import experts, fp8, permute
+
+    return type("Ops", (), {"permute": permute, "fp8": fp8, "experts": experts})
+
+
+def randn(seed, *shape, dtype=torch.float32):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+# --------------------------------------------------------------------- SwiGLU
+def swiglu_by_steps(h, limit):
+    """The quantized SwiGLU in f32, one IEEE operation at a time: (E4M3 codes, scales)."""
+    gate, up = h.float().chunk(2, 1)
+    g, u = gate.clamp(max=limit), up.clamp(-limit, limit)
+    a = g / (1 + torch.exp(-g)) * u
+    rows, width = a.shape
+    b = torch.nn.functional.pad(a, (0, -width % 128)).view(rows, -1, 128)
+    amax = b.abs().amax(-1).clamp_min(1e-30)
+    top = torch.full_like(amax, 448.0)
+    q = (b * (top / amax)[..., None]).view(rows, -1)[:, :width].to(E4M3)
+    return q.view(torch.uint8), amax / top
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,width", [(2000, 1408), (1500, 1401), (1, 2048)])
+def test_swiglu_gives_the_bits_of_its_definition(ops, dtype, rows, width):
+    """f32's own exponential and division, as in the layer's SwiGLU: no code and no scale may differ."""
+    h = randn(rows, rows, 2 * width, dtype=dtype) * 3
+    q, scale = ops.fp8.swiglu_quantize(h)
+    want_q, want_scale = swiglu_by_steps(h, 10.0)
+    assert torch.equal(scale, want_scale)
+    assert torch.equal(q.view(torch.uint8), want_q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("limit", [None, 3e38])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("width", [128, 33])
+def test_swiglu_of_the_largest_finite_gates(ops, dtype, width, limit):
+    """exp(-g) is 0 there: the value is g u, finite; its gradients are d u and d g (d u is 0 past the limit)."""
+    top = min(torch.finfo(dtype).max, float("inf") if limit is None else limit)
+    h = torch.zeros(4, 2 * width, device="cuda", dtype=dtype)
+    h[0, 5], h[1, 7], h[2, 9], h[3, 11] = torch.finfo(dtype).max, 2.5e38, 1e30, 200.0
+    h[:, width:] = 0.5
+    q, scale = ops.fp8.swiglu_quantize(h, limit=limit)
+    got = (q.double() * scale.double().repeat_interleave(128, 1)[:, :width]).amax(1)
+    gate = h[:, :width].double().clamp(max=top)
+    want = (gate * 0.5).amax(1)
+    assert bool(((got - want).abs() <= 4 * 2.0**-24 * want).all())  # a block's largest value is exact but for its scale
+    d = torch.ones(4, width, device="cuda", dtype=dtype)
+    grad = ops.fp8.swiglu_grad(h, d, limit=limit).double()
+    for r, c in enumerate((5, 7, 9, 11)):
+        cut = limit is not None and float(h[r, c]) > limit
+        assert float(grad[r, c]) == (0.0 if cut else 0.5)
+        assert abs(float(grad[r, width + c]) - float(gate[r, c])) <= 2.0**-8 * float(gate[r, c])
+    assert not bool(grad.isnan().any())

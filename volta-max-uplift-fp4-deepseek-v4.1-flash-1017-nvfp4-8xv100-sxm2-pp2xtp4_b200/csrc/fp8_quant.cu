@@ -33,30 +33,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return o;
 }
 
-// 1 + e^-g for g >= -88. e^-g = 2^t 2^d with t the rounded product -g log2(e) and d what that rounding (an error-free
-// product, by fma) and log2(e)'s own last bits left out, 2^d = 1 + d ln 2: the power of two is the hardware's, and its
-// argument's error does not grow with g. expf and an IEEE division instead bounded these kernels: 43 instructions per
-// value, 103 us for 49152 x 1408.
-__device__ __forceinline__ float one_plus_exp_neg(float g) {
-  constexpr float kLog2e = 1.44269502162933349609375f;      // log2(e) rounded to f32
-  constexpr float kLog2eRest = 1.92596299112661746887e-8f;  // log2(e) - kLog2e
-  constexpr float kLn2 = 0.693147180559945309417f;
-  const float t = -g * kLog2e;
-  const float d = fmaf(-g, kLog2eRest, fmaf(-g, kLog2e, -t));
-  float p;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(t));
-  return 1.f + fmaf(p, d * kLn2, p);
-}
-
-// x / y for y in [1, 2e38], by the hardware reciprocal: with the exponential above within 5.1 units of 2^-24 of the
-// value over gates in [-70, 12] (f32's own exponential and division: 3.6; a Newton step on the remainder: 5.2). Past
-// 2^126 the reciprocal is flushed, and the quotient with it, to 0.
-__device__ __forceinline__ float quotient(float x, float y) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
-  return x * r;
-}
-
 // The limited gate: min(gate, limit), and -88 for what is below it (the lowest values of a type, -inf): the SwiGLU and
 // its gradient are 0 there, as g / (1 + e^-g) of any such g is in f32.
 __device__ __forceinline__ float limited_gate(float gate, float limit) { return max_nan(min_nan(gate, limit), -88.f); }
@@ -65,7 +41,7 @@ __device__ __forceinline__ float limited_up(float up, float limit) { return max_
 // Limited SwiGLU (the framework's): g = min(gate, limit), u = clamp(up, +-limit), g / (1 + e^-g) * u.
 __device__ __forceinline__ float swiglu(float gate, float up, float limit) {
   const float g = limited_gate(gate, limit);
-  return quotient(g, one_plus_exp_neg(g)) * limited_up(up, limit);
+  return __fdiv_rn(g, 1.f + expf(-g)) * limited_up(up, limit);
 }
 
 // Position (row, block) of a walk over rows x blocks in steps of d_row rows and d_b blocks: one division at its start.
@@ -248,7 +224,7 @@ __global__ void __launch_bounds__(kQuantThreads) swiglu_grad_kernel(const T* __r
     for (int i = 0; i < 8; ++i) {
       const float g0 = gate.get(i), u0 = up.get(i), di = d.get(i);
       const float g = limited_gate(g0, limit), u = limited_up(u0, limit);
-      const float s = quotient(1.f, one_plus_exp_neg(g));
+      const float s = __frcp_rn(1.f + expf(-g));
       const float gs = g * s;
       dg[i] = g0 > limit ? 0.f : di * u * fmaf(gs, 1.f - s, s);
       du[i] = fabsf(u0) > limit ? 0.f : di * gs;
