@@ -71,3 +71,19 @@ def test_swiglu_of_the_largest_finite_gates(ops, dtype, width, limit):
         assert float(grad[r, c]) == (0.0 if cut else 0.5)
         assert abs(float(grad[r, width + c]) - float(gate[r, c])) <= 2.0**-8 * float(gate[r, c])
     assert not bool(grad.isnan().any())
+
+
+# -------------------------------------------------------------------- refusals
+@pytest.mark.gpu
+def test_permute_refuses_gradients_of_quantized_rows(ops):
+    """A float8 tensor may require a gradient in torch; the operators have none for it.  Only the refusal is run."""
+    ids = torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    leaf = randn(0, 3, 64).to(E4M3).requires_grad_()
+    cast = randn(0, 3, 64).requires_grad_().to(E4M3)
+    assert leaf.requires_grad and cast.requires_grad
+    for x in (leaf, cast):
+        for scale in (None, torch.ones(3, 1, device="cuda")):
+            with pytest.raises(ValueError, match="gradient"):
+                ops.permute.permute(x, ids, 4, scale=scale)
+        with torch.no_grad():
+            assert torch.equal(ops.permute.permute(x, ids, 4).rows[0].float(), x[0].float())

@@ -63,6 +63,7 @@ const char* kind_name(Kind k) {
   return names[k];
 }
 int code(ScalarType t) {
+  TORCH_CHECK_VALUE(is_float(t), "must be bfloat16, float16 or float32, got ", t);  // a wrong code is a wrong size
   return t == ScalarType::Half ? B200MOE_F16 : t == ScalarType::BFloat16 ? B200MOE_BF16 : B200MOE_F32;
 }
 
@@ -230,7 +231,8 @@ std::tuple<Tensor, OptTensor, Tensor, Tensor> permute(const Tensor& x, const Ten
     TORCH_CHECK_VALUE(scale.size(0) == x.size(0), "scale must have ", x.size(0), " rows, got ", scale.sizes());
   }
   if (at::GradMode::is_enabled() && x.requires_grad()) {
-    TORCH_CHECK_VALUE(!scale.defined(), "rows with scales are quantized: permute them without gradient");
+    TORCH_CHECK_VALUE(!scale.defined() && is_float(x.scalar_type()),
+                      "quantized rows (E4M3, or with scales) have no gradient: permute them without one");
     const variable_list out = PermuteFn::apply(x, ids, num_experts);
     return {out[0], std::nullopt, out[1], out[2]};
   }

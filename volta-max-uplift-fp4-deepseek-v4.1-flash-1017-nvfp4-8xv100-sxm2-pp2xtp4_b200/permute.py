@@ -42,7 +42,8 @@ def sort_routes(topk_ids: torch.Tensor, num_experts: int) -> tuple[torch.Tensor,
 
 def permute(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int, scale: torch.Tensor | None = None) -> Permuted:
     """Copy each token's row of ``x`` [T, H] (bf16, f16, f32, or E4M3 with its ``scale``
-    f32 [T, B]) to its routes' rows, sorted by expert (``topk_ids`` int32 [T, k])."""
+    f32 [T, B]) to its routes' rows, sorted by expert (``topk_ids`` int32 [T, k]).
+    E4M3 rows and rows with scales have no gradient: where ``x`` requires one they are refused."""
     return Permuted(*_lib.ops().permute(x, topk_ids, num_experts, scale))
 
 
