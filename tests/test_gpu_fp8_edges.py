@@ -87,3 +87,43 @@ def test_permute_refuses_gradients_of_quantized_rows(ops):
                 ops.permute.permute(x, ids, 4, scale=scale)
         with torch.no_grad():
             assert torch.equal(ops.permute.permute(x, ids, 4).rows[0].float(), x[0].float())
+
+
+# -------------------------------------------------------------------- products
+U = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, torch.float32: 2.0**-24}
+TINY = {torch.bfloat16: 2.0**-134, torch.float16: 2.0**-25, torch.float32: 2.0**-150}
+
+
+def packed(seed, *shape):
+    """E4M3 values of any size with a scale per 128 x 128 block."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    q = (60 * torch.randn(*shape, generator=g, device="cuda")).clamp(-448, 448).to(E4M3)
+    n, k = -(-shape[-2] // 128), -(-shape[-1] // 128)
+    return q, torch.rand(*shape[:-2], n, k, generator=g, device="cuda") * 1e-3 + 1e-4
+
+
+def check_product(got, q, scale, w, w_scale):
+    """Against 64 bits: 128 products a block, the scales' two roundings and one addition per block, each losing at
+    most 2^-23 of the sum of magnitudes, and the output's own rounding."""
+    k, n = q.shape[1], w.shape[0]
+    a = q.double() * scale.double().repeat_interleave(128, 1)[:, :k]
+    b = w.double() * w_scale.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+    want, mag = a @ b.T, a.abs() @ b.abs().T
+    bound = (128 + -(-k // 128) + 4) * 2.0**-23 * mag + U[got.dtype] * want.abs() + TINY[got.dtype]
+    assert got.shape == want.shape
+    excess = (got.double() - want).abs() - bound
+    assert bool((excess <= 0).all()), f"worst excess {float(excess.max()):.3e}"
+
+
+@pytest.mark.gpu
+def test_long_product_gives_the_same_bits_every_time(ops):
+    """Tiles of 256 columns hand their two TMEM buffers over 64 times a tile: a sum that met the next block's values
+    would differ from call to call."""
+    q, scale = ops.fp8.quantize(randn(1, 2560, 8192))
+    w, ws = packed(2, 2304, 8192)
+    first = ops.fp8.matmul(q, scale, w, ws, out_dtype=torch.float32)
+    check_product(first, q, scale, w, ws)
+    for _ in range(20):
+        assert torch.equal(ops.fp8.matmul(q, scale, w, ws, out_dtype=torch.float32), first)
+    ops.fp8.check_errors()

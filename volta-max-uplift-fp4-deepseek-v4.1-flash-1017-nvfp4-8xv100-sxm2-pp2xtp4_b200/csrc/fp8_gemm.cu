@@ -233,6 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld32(addr + c * 32, p);
             tmem_wait(p);
             if (c + 1 == COLS / 32) {  // all of the block's columns are in registers: the buffer is free
+              fence_before();  // every lane's reads come before the MMA that overwrites them, across the barrier
               __syncwarp();
               if (lane == 0) mbar_arrive(&acc_empty[b]);
             }
