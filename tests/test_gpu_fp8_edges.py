@@ -89,6 +89,34 @@ def test_permute_refuses_gradients_of_quantized_rows(ops):
             assert torch.equal(ops.permute.permute(x, ids, 4).rows[0].float(), x[0].float())
 
 
+@pytest.mark.gpu
+def test_forward_mode_tangents_are_refused(ops):
+    """A dual tensor has no requires_grad: without the refusal its tangent would read as zero."""
+    from torch.autograd import forward_ad
+
+    ids = torch.zeros(4, 2, dtype=torch.int32, device="cuda")
+    w, ws = packed(0, 48, 64)
+    m = ops.experts.Fp8Experts.from_weights(randn(1, 2, 64, 64), randn(2, 2, 64, 32), trainable=True)
+    weights = torch.rand(4, 2, device="cuda")
+    row, _ = ops.permute.sort_routes(ids, 2)
+    with forward_ad.dual_level():
+        dual = lambda v: forward_ad.make_dual(v, torch.ones_like(v))  # noqa: E731
+        x, rows, half = dual(randn(3, 4, 64)), dual(randn(4, 8, 64)), dual(randn(5, 4, 64, dtype=torch.bfloat16))
+        calls = [lambda: ops.permute.permute(x, ids, 2), lambda: ops.permute.unpermute(rows, row),
+                 lambda: ops.permute.unpermute(randn(4, 8, 64), row, dual(weights)),
+                 lambda: ops.fp8.linear(x, w, ws), lambda: ops.fp8.quantize(x), lambda: ops.fp8.swiglu_quantize(x),
+                 lambda: ops.fp8.swiglu_grad(x, randn(6, 4, 32)), lambda: m(half, ids, weights),
+                 lambda: m(randn(7, 4, 64, dtype=torch.bfloat16), ids, dual(weights))]
+        for call in calls:
+            with pytest.raises(NotImplementedError):
+                call()
+        y = randn(8, 4, 64).requires_grad_()  # a tangent of the incoming gradient
+        for out in (ops.permute.permute(y, ids, 2).rows, ops.fp8.linear(y, w, ws),
+                    ops.permute.unpermute(y, torch.tensor([[0], [1], [2], [3]], dtype=torch.int32, device="cuda"))):
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(out, y, dual(torch.ones_like(out.detach())))
+
+
 # -------------------------------------------------------------------- products
 U = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, torch.float32: 2.0**-24}
 TINY = {torch.bfloat16: 2.0**-134, torch.float16: 2.0**-25, torch.float32: 2.0**-150}

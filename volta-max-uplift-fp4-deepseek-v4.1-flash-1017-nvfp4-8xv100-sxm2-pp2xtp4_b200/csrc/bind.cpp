@@ -67,6 +67,12 @@ int code(ScalarType t) {
   return t == ScalarType::Half ? B200MOE_F16 : t == ScalarType::BFloat16 ? B200MOE_BF16 : B200MOE_F32;
 }
 
+// The operators have no forward-mode derivative: a tangent is refused instead of left out.
+void no_tangent(const char* name, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), name,
+                              " carries a forward-mode tangent, which this operator cannot differentiate");
+}
+
 // A CUDA tensor of the kind with `dim` axes, contiguous or (rows) with any distance between rows, on `like`'s device.
 void want(const char* name, const Tensor& t, Kind kind, int64_t dim, const Tensor* like = nullptr, bool rows = false) {
   TORCH_CHECK_VALUE(t.defined() && t.is_cuda(), name, " must be a CUDA tensor, got ",
@@ -79,6 +85,7 @@ void want(const char* name, const Tensor& t, Kind kind, int64_t dim, const Tenso
                     t.sizes());
   TORCH_CHECK_VALUE(!like || t.device() == like->device(), name, " is on ", t.device(), ", the other arguments on ",
                     like ? like->device().str() : "");
+  no_tangent(name, t);
 }
 void want_shape(const char* name, const Tensor& t, at::IntArrayRef shape) {
   TORCH_CHECK_VALUE(t.sizes() == shape, name, " must have shape ", shape, ", got ", t.sizes());
@@ -179,8 +186,9 @@ std::tuple<Tensor, Tensor> run_unpermute_grad(const Tensor& grad, const Tensor& 
 }
 
 // The gradients have no graph of their own: asked for one (create_graph), they refuse instead of leaving it out.
-void once_differentiable() {
+void once_differentiable(const Tensor& grad) {
   TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), "this operator's gradient cannot be differentiated again");
+  if (grad.defined()) no_tangent("the gradient", grad);
 }
 
 // A gradient as the kernels read it: contiguous columns, rows at any distance.
@@ -197,7 +205,7 @@ struct PermuteFn : torch::autograd::Function<PermuteFn> {
     return {rows, row_of_route, offsets};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once_differentiable();
+    once_differentiable(grads[0]);
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
     return {run_unpermute(grads[0].contiguous(), ctx->get_saved_variables()[0], Tensor(), grads[0].scalar_type()),
             Tensor(), Tensor()};
@@ -211,7 +219,7 @@ struct UnpermuteFn : torch::autograd::Function<UnpermuteFn> {
     return run_unpermute(rows, row_of_route, weights.value_or(Tensor()), out_dtype);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once_differentiable();
+    once_differentiable(grads[0]);
     const auto saved = ctx->get_saved_variables();
     const bool need_weights = saved[2].defined() && ctx->needs_input_grad(2);
     const auto [grad_rows, grad_weights] = run_unpermute_grad(as_rows(grads[0]), saved[0], saved[1], saved[2],
@@ -447,7 +455,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     return run_linear(x, w, w_scale, out_dtype);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once_differentiable();
+    once_differentiable(grads[0]);
     const auto saved = ctx->get_saved_variables();
     Tensor wt = saved[0], wt_scale = saved[1];
     if (!ctx->saved_data["transposed"].toBool()) std::tie(wt, wt_scale) = run_transpose(wt, wt_scale);

@@ -1,5 +1,8 @@
 """What the stateless operators (``permute``, ``fp8``) share: their binding and the
-device's operator error word."""
+device's operator error word.
+
+Gradients are of first order and reverse mode: a second differentiation and a tensor
+with a forward-mode tangent (``torch.autograd.forward_ad``) raise ``NotImplementedError``."""
 
 from __future__ import annotations
 
