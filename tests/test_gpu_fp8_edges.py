@@ -117,6 +117,20 @@ def test_forward_mode_tangents_are_refused(ops):
                 torch.autograd.grad(out, y, dual(torch.ones_like(out.detach())))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 2**32 + 5, 1), (1, 2**31, 1), (2**16, 1, 1), (2**23, 1)])
+def test_weights_past_the_kernels_sizes_are_refused(ops, shape):
+    """Every axis counts, the middle one of three too: 2^32 + 5 cut to 32 bits would be five rows."""
+    w = torch.empty(shape, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="too large"):
+        ops.fp8.quantize_weight(w)
+    del w
+    q = torch.empty(shape, dtype=torch.uint8, device="cuda").view(E4M3)
+    scale = torch.empty(*shape[:-2], -(-shape[-2] // 128), 1, device="cuda")
+    with pytest.raises(ValueError, match="too large"):
+        ops.fp8.transpose_weight(q, scale)
+
+
 # -------------------------------------------------------------------- products
 U = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, torch.float32: 2.0**-24}
 TINY = {torch.bfloat16: 2.0**-134, torch.float16: 2.0**-25, torch.float32: 2.0**-150}

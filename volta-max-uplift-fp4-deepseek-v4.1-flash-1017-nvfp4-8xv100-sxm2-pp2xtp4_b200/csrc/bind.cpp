@@ -29,6 +29,7 @@ using OptDtype = std::optional<ScalarType>;
 
 constexpr ScalarType kE4m3 = ScalarType::Float8_e4m3fn;
 constexpr int64_t kBlock = 128, kMaxExperts = 1024, kMaxRoutes = int64_t(1) << 26, kMaxTopK = 1024;
+constexpr int64_t kMaxAxis = INT32_MAX - 256;
 
 // ------------------------------------------------------------------ errors
 // A non-zero status of the library; becomes b200moe._lib.B200MoeError in Python.
@@ -81,8 +82,8 @@ void want(const char* name, const Tensor& t, Kind kind, int64_t dim, const Tenso
                     " axes, got ", t.scalar_type(), " ", t.sizes());
   TORCH_CHECK_VALUE(t.is_contiguous() || (rows && t.stride(-1) == 1 && t.stride(0) >= t.size(1)), name, " must ",
                     rows ? "have contiguous rows" : "be contiguous", ", got strides ", t.strides());
-  TORCH_CHECK_VALUE(t.size(0) <= INT32_MAX && (dim < 2 || t.size(-1) <= INT32_MAX), name, " is too large: ",
-                    t.sizes());
+  // every axis: the kernels' sizes are 32 bits, and their round-ups to whole tiles stay below 2^31
+  for (const int64_t n : t.sizes()) TORCH_CHECK_VALUE(n <= kMaxAxis, name, " is too large: ", t.sizes());
   TORCH_CHECK_VALUE(!like || t.device() == like->device(), name, " is on ", t.device(), ", the other arguments on ",
                     like ? like->device().str() : "");
   no_tangent(name, t);
@@ -335,10 +336,17 @@ Tensor swiglu_grad(const Tensor& h, const Tensor& grad, const std::optional<doub
   return out;
 }
 
+// The quantizer and the transpose of weights launch a CTA per block: grids of at most 65535 matrices and row blocks.
+void check_launch(const char* name, const Tensor& w) {
+  constexpr int64_t most = 65535;
+  TORCH_CHECK_VALUE((w.dim() == 2 || w.size(0) <= most) && blocks(w.size(-2)) <= most, name, " is too large: ", w.sizes());
+}
+
 std::tuple<Tensor, Tensor> quantize_weight(const Tensor& w) {
   const bool many = w.defined() && w.dim() == 3;
   want("w", w, kFloats, many ? 3 : 2);
   TORCH_CHECK_VALUE(w.numel() > 0, "w must not be empty, got ", w.sizes());
+  check_launch("w", w);
   const c10::cuda::CUDAGuard guard(w.device());
   const int64_t n = w.size(-2), k = w.size(-1), mats = many ? w.size(0) : 1;
   Tensor q = empty(w.sizes(), kE4m3, w);
@@ -364,6 +372,7 @@ void check_weight(const char* name, const char* scale_name, const Tensor& w, con
 }
 
 std::tuple<Tensor, Tensor> run_transpose(const Tensor& w, const Tensor& scale) {
+  check_launch("w", w);
   const c10::cuda::CUDAGuard guard(w.device());
   const bool many = w.dim() == 3;
   const int64_t n = w.size(-2), k = w.size(-1), mats = many ? w.size(0) : 1;

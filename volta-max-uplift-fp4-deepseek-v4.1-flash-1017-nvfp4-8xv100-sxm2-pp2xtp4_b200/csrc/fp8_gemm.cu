@@ -361,7 +361,7 @@ using namespace b200moe;
 namespace {
 
 int product_status(const Fp8Product& p, int out_dtype) {
-  if (!p.w || !p.w_scale || !p.out || p.S < 1 || p.N < 1 || p.K < 16 || p.K % 16 || p.E < 1 || p.E > kMaxExperts ||
+  if (!p.w || !p.w_scale || !p.out || p.S < 1 || p.S > INT32_MAX - 256 || p.N < 1 || p.K < 16 || p.K % 16 || p.E < 1 || p.E > kMaxExperts ||
       (!p.offsets && p.E != 1) || int64_t(p.E) * p.N > INT32_MAX - 256 || p.K > (1 << 24))
     return B200MOE_ERR_INVALID_ARG;
   if (out_dtype < 0 || out_dtype > B200MOE_F32) return B200MOE_ERR_DTYPE;
