@@ -401,8 +401,8 @@ int b200moe_fp8_transpose_weight(void* stream, const void* w, const float* scale
 /* out [S][N] = a . w^T with the blocks' scales, f32 sums: a [S][K] E4M3 with
  * a_scale [S][ceil(K / 128)] (a_scale_stride floats between rows), w [E][N][K]
  * E4M3 with w_scale [E][ceil(N / 128)][ceil(K / 128)].  offsets (device, int32
- * [E + 1]): rows offsets[e] .. offsets[e + 1] use w[e], rows from offsets[E] on
- * become zeros; NULL: E is 1.  K a multiple of 16, a and w on 16-byte
+ * [E + 1]): rows offsets[e] .. offsets[e + 1] use w[e], rows before offsets[0]
+ * and from offsets[E] on become zeros; NULL: E is 1.  K a multiple of 16, a and w on 16-byte
  * addresses, E <= 1024. */
 int b200moe_fp8_matmul(void* stream, const void* a, const float* a_scale, int64_t a_scale_stride, const void* w,
                        const float* w_scale, const int32_t* offsets, int S, int N, int K, int E, void* out,

@@ -169,3 +169,25 @@ def test_long_product_gives_the_same_bits_every_time(ops):
     for _ in range(20):
         assert torch.equal(ops.fp8.matmul(q, scale, w, ws, out_dtype=torch.float32), first)
     ops.fp8.check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,head,tail", [([3, 0, 5], 4, 0), ([0, 0], 7, 3), ([200, 150], 130, 20),
+                                              ([3000, 0, 2500], 700, 11)])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_rows_before_the_first_expert_are_zeros(ops, counts, head, tail, out_dtype):
+    """A part of the experts' offsets: the rows of the experts before it have none here."""
+    n, k, rows = 1064, 144, head + sum(counts) + tail
+    off = torch.tensor([head, *counts], device="cuda").cumsum(0).to(torch.int32)
+    q, scale = ops.fp8.quantize(randn(rows, rows, k))
+    w, ws = packed(head, len(counts), n, k)
+    for r in (slice(0, head), slice(rows - tail, rows)):
+        q.view(torch.uint8)[r] = 0x7F
+    torch.full((rows, n), float("nan"), dtype=out_dtype, device="cuda")  # what the output's memory held before
+    got = ops.fp8.grouped_matmul(q, scale, off, w, ws, out_dtype=out_dtype)
+    assert not got[:head].any() and not got[rows - tail:].any()
+    for e in range(len(counts)):
+        r = slice(int(off[e]), int(off[e + 1]))
+        if counts[e]:
+            check_product(got[r], q[r], scale[r], w[e], ws[e])
+    ops.fp8.check_errors()

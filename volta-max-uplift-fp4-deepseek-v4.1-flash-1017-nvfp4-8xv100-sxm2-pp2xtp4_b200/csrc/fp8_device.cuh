@@ -97,10 +97,13 @@ __device__ __forceinline__ int tile_expert(const int* start, int E, int item) {
   return lo;
 }
 
-// Rows past the last expert's are zeros: rows first .. S of out [S][N].
+// Rows of out [S][N] without an expert, before the first expert's and past the last one's, are zeros.
 template <typename TO>
-__device__ __forceinline__ void zero_rows(TO* out, int64_t N, int first, int S, int tid, int threads) {
-  for (int64_t r = max(first, 0) + blockIdx.x; r < S; r += gridDim.x)
+__device__ __forceinline__ void zero_rows(TO* out, int64_t N, int first, int last, int S, int tid, int threads) {
+  const int before = min(max(first, 0), S);
+  for (int64_t r = blockIdx.x; r < before; r += gridDim.x)
+    for (int64_t c = tid; c < N; c += threads) out[r * N + c] = from_f32<TO>(0.f);
+  for (int64_t r = max(last, before) + int64_t(blockIdx.x); r < S; r += gridDim.x)
     for (int64_t c = tid; c < N; c += threads) out[r * N + c] = from_f32<TO>(0.f);
 }
 

@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (lane == 0) tma_stores_done();
-    if (a.offsets) zero_rows(static_cast<TO*>(a.out), a.N, off[a.E], a.S, threadIdx.x - kSumWarp0 * 32, kSumWarps * 32);
+    if (a.offsets) zero_rows(static_cast<TO*>(a.out), a.N, off[0], off[a.E], a.S, threadIdx.x - kSumWarp0 * 32, kSumWarps * 32);
   }
   fence_before();
   __syncthreads();

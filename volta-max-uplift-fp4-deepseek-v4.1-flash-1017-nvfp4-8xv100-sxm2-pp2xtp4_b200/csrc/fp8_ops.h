@@ -7,8 +7,8 @@
 namespace b200moe {
 
 // out [S][N] = rows of a [S][K] . w [E][N][K]^T; with offsets [E + 1] (device)
-// rows offsets[e] .. offsets[e + 1] use w[e] and rows from offsets[E] on become
-// zeros, without them E is 1.  K is a multiple of 16, a and w start on 16 bytes.
+// rows offsets[e] .. offsets[e + 1] use w[e] and rows before offsets[0] and from
+// offsets[E] on become zeros, without them E is 1.  K is a multiple of 16, a and w start on 16 bytes.
 struct Fp8Product {
   const void* a;
   const float* a_scale;  // [S][ceil(K / 128)]

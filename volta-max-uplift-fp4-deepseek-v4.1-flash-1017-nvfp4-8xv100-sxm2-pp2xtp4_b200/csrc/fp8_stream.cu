@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (row0 + i < end) out[int64_t(row0 + i) * a.N + col] = from_f32<TO>(acc[i]);
       }
     }
-    if (a.offsets) zero_rows(out, a.N, off[a.E], a.S, tid, 128);
+    if (a.offsets) zero_rows(out, a.N, off[0], off[a.E], a.S, tid, 128);
   }
   fence_before();
   __syncthreads();

@@ -61,7 +61,8 @@ def matmul(q: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_scale: torch
 def grouped_matmul(q: torch.Tensor, scale: torch.Tensor, offsets: torch.Tensor, w: torch.Tensor,
                    w_scale: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """Rows sorted by expert (``permute``) times each expert's weights [E, N, K]: rows
-    ``offsets[e] : offsets[e + 1]`` use ``w[e]``; rows from ``offsets[E]`` on become zeros."""
+    ``offsets[e] : offsets[e + 1]`` use ``w[e]``; rows before ``offsets[0]`` and from ``offsets[E]``
+    on become zeros.  Offsets that fall or pass the rows are reported; those experts' rows hold no result."""
     return _lib.ops().grouped_matmul(q, scale, offsets, w, w_scale, out_dtype)
 
 
