@@ -8,6 +8,8 @@ import pytest
 import torch
 
 E4M3 = torch.float8_e4m3fn
+U = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, torch.float32: 2.0**-24}
+TINY = {torch.bfloat16: 2.0**-134, torch.float16: 2.0**-25, torch.float32: 2.0**-150}
 
 
 @pytest.fixture(scope="module")
@@ -73,6 +75,67 @@ def test_swiglu_of_the_largest_finite_gates(ops, dtype, width, limit):
     assert not bool(grad.isnan().any())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("width", [256, 33])
+def test_swiglu_of_low_gates(ops, dtype, width):
+    """Down to -88.7 exp(-g) is finite in f32 and a large up makes the value count; below, the value is 0 (the 64-bit
+    one is under 1e-36 of up)."""
+    gates = [-80.0, -87.0, -87.5, -88.0, -88.25, -88.5, -89.0, -100.0, -1e4, -1e30, torch.finfo(dtype).min,
+             -float("inf")]
+    h = torch.zeros(len(gates), 2 * width, device="cuda", dtype=dtype)
+    h[:, 3] = torch.tensor(gates, device="cuda")
+    h[:, width + 3] = 1e37
+    g, u = h[:, 3].double(), h[:, width + 3].double()
+    s = torch.where(g < -88.7, 0.0, torch.sigmoid(g))
+    g = g.clamp_min(-1e3)
+    q, scale = ops.fp8.swiglu_quantize(h, limit=None)
+    got = q[:, 3].double() * scale[:, 0].double()
+    # the exponential's and four more roundings; below f32's normal numbers nothing is divided here
+    assert bool(((got - g * s * u).abs() <= 8 * 2.0**-24 * (g * s * u).abs()).all())
+    grad = ops.fp8.swiglu_grad(h, torch.ones(len(gates), width, dtype=dtype, device="cuda"), limit=None).double()
+    want = u * (s + g * s * (1 - s))
+    near = U[dtype] * want.abs() + 16 * 2.0**-24 * u * (s + g.abs() * s) + TINY[dtype]
+    assert bool(((grad[:, 3] - want).abs() <= near).all())
+    assert bool(((grad[:, width + 3] - g * s).abs() <= U[dtype] * (g * s).abs() + 2.0**-126).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("limit", [10.0, None])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("width", [256, 257])
+def test_swiglu_of_special_values(ops, dtype, limit, width):
+    """A NaN makes its block NaN and no other; an infinite value the same; a bound turns an infinity into itself."""
+    inf, nan, low = float("inf"), float("nan"), torch.finfo(dtype).min
+    cases = [(nan, 1.0), (1.0, nan), (inf, 1.0), (-inf, 1.0), (1.0, inf), (1.0, -inf), (low, 1.0), (low, low),
+             (-inf, 0.0), (0.0, 1.0), (1.0, 0.0), (torch.finfo(dtype).tiny, torch.finfo(dtype).tiny)]
+    h = torch.full((len(cases), 2 * width), 0.5, device="cuda", dtype=dtype)
+    h[:, 7] = torch.tensor([c[0] for c in cases], device="cuda")
+    h[:, width + 7] = torch.tensor([c[1] for c in cases], device="cuda")
+    q, scale = ops.fp8.swiglu_quantize(h, limit=limit)
+    v = q.double() * scale.double().repeat_interleave(128, 1)[:, :width]
+    d = torch.ones(len(cases), width, device="cuda", dtype=dtype)
+    grad = ops.fp8.swiglu_grad(h, d, limit=limit)
+    gate, up = h.double().chunk(2, 1)
+    lim = inf if limit is None else limit
+    g, u = gate.clamp(max=lim).clamp_min(-1e3), up.clamp(-lim, lim)
+    s = torch.sigmoid(g)
+    want = g * s * u
+    for r, (a, b) in enumerate(cases):
+        bad = not bool(torch.isfinite(want[r, 7]))
+        assert bool(v[r, :128].isnan().all()) == bad and not bool(v[r, 128:].isnan().any()), (a, b)
+        if not bad:
+            step = 2.0**-4 * want[r].abs() + 2.0**-10 * float(scale[r].max())
+            assert bool(((v[r] - want[r]).abs() <= step * (1 + 2.0**-18) + 2.0**-20 * float(scale[r].max()) * 448).all())
+        zero = torch.tensor([j not in (7, width + 7) for j in range(2 * width)], device="cuda")
+        assert not bool(grad[r][zero].isnan().any()), (a, b)
+    up_cut = [r for r, (_, b) in enumerate(cases) if abs(b) > lim]
+    gate_cut = [r for r, (a, _) in enumerate(cases) if a > lim]
+    assert not grad[up_cut, width + 7].any() and not grad[gate_cut, 7].any()
+    assert grad[[0, 1], 7].isnan().all() and grad[0, width + 7].isnan() and not grad[1, width + 7].isnan()
+    assert not grad[[3, 6, 8]][:, [7, width + 7]].any()  # the lowest gates: no slope
+
+
 # -------------------------------------------------------------------- refusals
 @pytest.mark.gpu
 def test_permute_refuses_gradients_of_quantized_rows(ops):
@@ -132,10 +195,6 @@ def test_weights_past_the_kernels_sizes_are_refused(ops, shape):
 
 
 # -------------------------------------------------------------------- products
-U = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, torch.float32: 2.0**-24}
-TINY = {torch.bfloat16: 2.0**-134, torch.float16: 2.0**-25, torch.float32: 2.0**-150}
-
-
 def packed(seed, *shape):
     """E4M3 values of any size with a scale per 128 x 128 block."""
     g = torch.Generator(device="cuda")

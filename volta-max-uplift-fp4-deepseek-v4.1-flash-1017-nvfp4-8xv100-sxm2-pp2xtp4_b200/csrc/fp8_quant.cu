@@ -33,9 +33,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return o;
 }
 
-// The limited gate: min(gate, limit), and -88 for what is below it (the lowest values of a type, -inf): the SwiGLU and
-// its gradient are 0 there, as g / (1 + e^-g) of any such g is in f32.
-__device__ __forceinline__ float limited_gate(float gate, float limit) { return max_nan(min_nan(gate, limit), -88.f); }
+// The limited gate: min(gate, limit), and a finite value for -inf: from -89 down e^-g is infinite in f32 and the SwiGLU
+// and its gradient are 0, where -inf itself would give NaN.
+__device__ __forceinline__ float limited_gate(float gate, float limit) { return max_nan(min_nan(gate, limit), -128.f); }
 __device__ __forceinline__ float limited_up(float up, float limit) { return max_nan(min_nan(up, limit), -limit); }
 
 // Limited SwiGLU (the framework's): g = min(gate, limit), u = clamp(up, +-limit), g / (1 + e^-g) * u.

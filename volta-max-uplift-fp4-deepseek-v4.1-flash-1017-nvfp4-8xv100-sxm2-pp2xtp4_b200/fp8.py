@@ -29,8 +29,8 @@ def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def swiglu_quantize(h: torch.Tensor, limit: float | None = 10.0) -> tuple[torch.Tensor, torch.Tensor]:
     """Limited SwiGLU of rows [M, 2 I] (gate columns, then up), quantized:
-    ``g / (1 + exp(-g)) * u`` with ``g = min(gate, limit)``, ``u = clamp(up, -limit, limit)``
-    (a gate of -inf or a type's lowest value gives 0)."""
+    ``g / (1 + exp(-g)) * u`` with ``g = min(gate, limit)``, ``u = clamp(up, -limit, limit)``,
+    each step one f32 operation (a gate of -inf or a type's lowest value gives 0)."""
     return _lib.ops().swiglu_quantize(h, limit)
 
 
