@@ -250,3 +250,30 @@ def test_rows_before_the_first_expert_are_zeros(ops, counts, head, tail, out_dty
         if counts[e]:
             check_product(got[r], q[r], scale[r], w[e], ws[e])
     ops.fp8.check_errors()
+
+
+# ---------------------------------------------------------------------- errors
+@pytest.mark.gpu
+def test_no_error_is_lost_between_streams(ops):
+    """An error that one stream's kernel reports while another stream reads the word is seen by that read or the next."""
+    from b200moe._lib import B200MoeError
+
+    rows, bad = torch.ones(2, 8, device="cuda"), torch.tensor([[0, 99]], dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+
+    def reported():
+        try:
+            ops.permute.check_errors()
+        except B200MoeError:
+            return 1
+        return 0
+
+    for i in range(2000):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(500 * (i % 100))  # up to some 25 us, past the read below
+            ops.permute.unpermute(rows, bad)
+        seen = reported()
+        side.synchronize()
+        assert seen + reported() == 1, i
+    assert reported() == 0

@@ -1,6 +1,7 @@
 // The device error word of the stateless operators (permute.cu, fp8_*.cu): no
 // layer object holds one for them.  One word per GPU, OR-ed by kernels that
-// found a row or offset out of range, read and cleared by b200moe_op_errors.
+// found a row or offset out of range; b200moe_op_errors reads it and clears the
+// bits that it read.
 #include <atomic>
 
 #include "common.cuh"
@@ -39,6 +40,12 @@ int sm_count() {
   return n;
 }
 
+namespace {
+
+// Clears what was read and nothing else: another stream's kernel may have set a bit since.
+__global__ void clear_errors_kernel(uint32_t* word, uint32_t seen) { atomicAnd(word, ~seen); }
+
+}  // namespace
 }  // namespace b200moe
 
 extern "C" int b200moe_op_errors(void* stream, uint32_t* bits) {
@@ -47,8 +54,14 @@ extern "C" int b200moe_op_errors(void* stream, uint32_t* bits) {
   if (!word) return B200MOE_ERR_CUDA;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint32_t b = 0;
-  if (cudaMemcpyAsync(&b, word, sizeof(b), cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-      cudaMemsetAsync(word, 0, sizeof(b), s) != cudaSuccess || cudaStreamSynchronize(s) != cudaSuccess) {
+  cudaError_t e = cudaMemcpyAsync(&b, word, sizeof(b), cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess && b) {
+    clear_errors_kernel<<<1, 1, 0, s>>>(word, b);
+    e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  }
+  if (e != cudaSuccess) {
     cudaGetLastError();
     return B200MOE_ERR_CUDA;
   }
