@@ -277,3 +277,22 @@ def test_no_error_is_lost_between_streams(ops):
         side.synchronize()
         assert seen + reported() == 1, i
     assert reported() == 0
+
+
+# --------------------------------------------------------------------- experts
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_router_weights_learn_without_transposed_weights(ops, dtype):
+    """Their gradient is <grad, y>: the same bits with and without the weights that only the tokens' gradient reads."""
+    t, k, e, h, i = 21, 3, 6, 128, 96
+    w13, w2 = 0.05 * randn(1, e, 2 * i, h), 0.05 * randn(2, e, h, i)
+    x, ids = randn(3, t, h, dtype=dtype), torch.randint(-1, e, (t, k), dtype=torch.int32, device="cuda")
+    grad, got = randn(4, t, h, dtype=dtype), []
+    for trainable in (False, True):
+        m = ops.experts.Fp8Experts.from_weights(w13, w2, trainable=trainable)
+        w = torch.rand(t, k, generator=torch.Generator("cuda").manual_seed(5), device="cuda").requires_grad_()
+        got += torch.autograd.grad(m(x, ids, w), w, grad)
+        if not trainable:
+            with pytest.raises(ValueError, match="trainable"):
+                m(x.clone().requires_grad_(), ids, w)
+    assert torch.equal(*got) and bool(got[0].any()) and not got[0][ids < 0].any()

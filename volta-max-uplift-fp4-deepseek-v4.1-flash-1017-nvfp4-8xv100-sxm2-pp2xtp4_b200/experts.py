@@ -20,7 +20,7 @@ SWIGLU_LIMIT = 10.0
 class Fp8Experts:
     """``w13`` E4M3 [E, 2 I, H] (gate rows, then up rows) and ``w2`` [E, H, I] with their
     scales (``fp8.quantize_weight``); H and I multiples of 16.  ``trainable`` also keeps
-    the transposed weights, which the gradients of tokens and router weights need."""
+    the transposed weights, which the tokens' gradient needs (the router weights' does not)."""
 
     def __init__(self, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor, w2_scale: torch.Tensor, *,
                  swiglu_limit: float | None = SWIGLU_LIMIT, trainable: bool = False):
@@ -62,8 +62,8 @@ class Fp8Experts:
         if topk_weights.shape != topk_ids.shape:
             raise ValueError(f"bad routing shape {tuple(topk_ids.shape)} with weights {tuple(topk_weights.shape)}")
         if torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad):
-            if self.w13_t is None:
-                raise ValueError("gradients need trainable=True (the transposed weights)")
+            if x.requires_grad and self.w13_t is None:
+                raise ValueError("the tokens' gradient needs trainable=True (the transposed weights)")
             return _Experts.apply(x, topk_weights, topk_ids, self)
         _, y, row_of_route, _ = self._products(x, topk_ids)
         return unpermute(y, row_of_route, topk_weights)
