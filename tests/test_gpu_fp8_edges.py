@@ -252,6 +252,67 @@ def test_rows_before_the_first_expert_are_zeros(ops, counts, head, tail, out_dty
     ops.fp8.check_errors()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(2500, 2049, 144), (2500, 2100, 256), (4801, 1000, 400), (2500, 2056, 2064)])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_wide_tiles_that_end_inside(ops, m, n, k, out_dtype):
+    """Tiles of 128 x 256 (148 of them at least) whose last columns, rows and K block are partial: whole pieces leave by
+    clipped copies, odd rows by elements."""
+    q, scale = ops.fp8.quantize(randn(m + n, m, k))
+    w, ws = packed(k, n, k)
+    check_product(ops.fp8.matmul(q, scale, w, ws, out_dtype=out_dtype), q, scale, w, ws)
+    ops.fp8.check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1023, 1064, 1280])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_wide_tiles_by_expert(ops, n, out_dtype):
+    """Experts that begin and end inside a tile's 32-row copies, every row looked at."""
+    counts, k, tail = [700, 1, 0, 129, 333, 2000, 31, 64, 95, 500, 32, 128], 272, 19
+    off = torch.tensor([0, *counts], device="cuda").cumsum(0).to(torch.int32)
+    rows = sum(counts) + tail
+    q, scale = ops.fp8.quantize(randn(n, rows, k))
+    w, ws = packed(n, len(counts), n, k)
+    got = ops.fp8.grouped_matmul(q, scale, off, w, ws, out_dtype=out_dtype)
+    for e, c in enumerate(counts):
+        r = slice(int(off[e]), int(off[e + 1]))
+        if c:
+            check_product(got[r], q[r], scale[r], w[e], ws[e])
+    assert not got[rows - tail:].any()
+    ops.fp8.check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 8, 20, 33])
+@pytest.mark.parametrize("k", [12544, 12560, 16384, 16400, 32768, 32784])
+def test_longest_k_of_each_kernel(ops, m, k):
+    """One matrix: eight rows' values fill shared memory up to K 12544, the scales of 32 rows up to 16384, of 16 up to
+    32768; past each the next kernel takes over."""
+    q, scale = ops.fp8.quantize(randn(m, m, k))
+    w, ws = packed(k, 200, k)
+    check_product(ops.fp8.matmul(q, scale, w, ws), q, scale, w, ws)
+    x = randn(k, m, k, dtype=torch.bfloat16)
+    q, scale = ops.fp8.quantize(x)
+    check_product(ops.fp8.linear(x, w, ws), q, scale, w, ws)
+    ops.fp8.check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [16384, 16400])
+def test_longest_k_by_expert(ops, k):
+    counts = [5, 0, 20, 33]
+    off = torch.tensor([0, *counts], device="cuda").cumsum(0).to(torch.int32)
+    q, scale = ops.fp8.quantize(randn(k, sum(counts), k))
+    w, ws = packed(k, len(counts), 300, k)
+    got = ops.fp8.grouped_matmul(q, scale, off, w, ws)
+    for e, c in enumerate(counts):
+        r = slice(int(off[e]), int(off[e + 1]))
+        if c:
+            check_product(got[r], q[r], scale[r], w[e], ws[e])
+    ops.fp8.check_errors()
+
+
 # ---------------------------------------------------------------------- errors
 @pytest.mark.gpu
 def test_no_error_is_lost_between_streams(ops):
@@ -296,3 +357,24 @@ def test_router_weights_learn_without_transposed_weights(ops, dtype):
             with pytest.raises(ValueError, match="trainable"):
                 m(x.clone().requires_grad_(), ids, w)
     assert torch.equal(*got) and bool(got[0].any()) and not got[0][ids < 0].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,k,e,h,i", [(1, 4, 16, 512, 256), (70, 6, 16, 512, 352), (900, 4, 8, 256, 128)])
+def test_fp8_experts_in_f16(ops, t, k, e, h, i):
+    """The whole path in f16, in the norm within 2^-8: f16's roundings take 2^-11 each, and the share of values whose
+    32-bit form falls on the other side of an E4M3 boundary (2^-20 / 2^-4 of them, 2^-3 off) less than that."""
+    from test_gpu_fp8_experts import dequantize, plain_experts, rng, routes
+
+    m = ops.experts.Fp8Experts.from_weights(0.05 * randn(1, e, 2 * i, h), 0.05 * randn(2, e, h, i), trainable=True)
+    x, ids = randn(3, t, h, dtype=torch.float16), routes(rng(t), t, k, e, 0.1)
+    w, grad = torch.rand(t, k, generator=rng(t + 1), device="cuda"), randn(4, t, h, dtype=torch.float16)
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = m(xr, ids, wr)
+    gx, gw = torch.autograd.grad(out, (xr, wr), grad)
+    assert out.dtype == gx.dtype == torch.float16 and torch.equal(out, m(x, ids, w))
+    wide = lambda q, s: dequantize(q, s.repeat_interleave(128, -2)[..., : q.shape[-2], :])  # noqa: E731
+    want = plain_experts(x, ids, w, wide(m.w13, m.w13_scale), wide(m.w2, m.w2_scale), 10.0, grad)
+    for got, ref in zip((out, gx, gw), want):
+        assert float((got.detach().double() - ref).norm()) <= 2.0**-8 * float(ref.norm())
+    ops.fp8.check_errors()
