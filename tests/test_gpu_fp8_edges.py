@@ -313,6 +313,19 @@ def test_longest_k_by_expert(ops, k):
     ops.fp8.check_errors()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 8])
+@pytest.mark.parametrize("n,k", [(4736, 2064), (4737, 2064), (9472, 272), (9473, 272), (2368, 6400), (2369, 6400)])
+def test_few_rows_at_the_end_of_a_wave(ops, m, n, k):
+    """The few-row kernel's last item that has a CTA of its own, and the first that has none."""
+    w, ws = packed(n, n, k)
+    x = randn(k, m, k, dtype=torch.bfloat16)
+    q, scale = ops.fp8.quantize(x)
+    check_product(ops.fp8.matmul(q, scale, w, ws, out_dtype=torch.float32), q, scale, w, ws)
+    check_product(ops.fp8.linear(x, w, ws), q, scale, w, ws)
+    ops.fp8.check_errors()
+
+
 # ---------------------------------------------------------------------- errors
 @pytest.mark.gpu
 def test_no_error_is_lost_between_streams(ops):

@@ -369,19 +369,23 @@ int product_status(const Fp8Product& p, int out_dtype) {
   return B200MOE_OK;
 }
 
-// The kernel by rows per matrix, as measured on B200 (us; kernels of 8, 16, 32 and 128 rows per tile):
-//   one matrix 4096 x 4096: 6.8 / 11.5 / 12.4 / 14.2 at 1 row, - / 11.9 / 13.0 / 14.5 at 32, - / 12.1 / 13.1 / 14.5
-//   at 64, - / 20.9 / 13.2 / 14.6 at 96, - / 29.7 / 23.1 / 15.4 at 192: a tile of fewer rows gives more CTAs, so the
-//   smallest whose tiles still run in one wave (the kernels' order, as each has become faster since: 5.6 at 1 row, 9.0
-//   at 32, 10.9 at 96, 13.6 at 192). The first is left where its bandwidth costs more than its latency saves: 8192 x
-//   4096 takes 11.3 / 11.6 with one row, 11264 x 4096 15.2 / 12.3;
-//   64 matrices 2816 x 2048: - / 67 / 64 / 71 at 8 rows each, - / 104 / 66 / 73 at 24, - / 112 / 91 / 74 at 32, where
-//   experts above 32 rows read their weights twice.
+// The kernel by rows per matrix, as measured on B200 (us; kernels of 8, 16, 32 and 128 rows per tile, weights from HBM):
+//   one matrix 4096 x 4096: 6.4 / 9.4 / 10.7 / 12.2 at 1 row, 8.0 / 9.5 / 10.8 / 12.0 at 8, - / 9.7 / 11.2 / 11.9 at 32,
+//   - / 9.9 / 11.2 / 12.0 at 64, - / 15.9 / 11.3 / 12.2 at 96, - / 22.4 / 18.4 / 12.4 at 192: a tile of fewer rows gives
+//   more CTAs, so the smallest whose tiles still run in one wave. So for the first too: 9472 x 2048 5.9 / 7.1 / 7.6 / -
+//   in one wave; 9504 x 2048 8.9 / 7.1 / 7.6 / - with CTAs that walk on to a second tile, 14336 x 4096 19.1 / 13.0 /
+//   13.7 / 21.5. The one wrong choice seen in one wave: 4096 x 6144, 13.7 / 12.6.
+//   64 matrices 2816 x 2048, kernels of 32 and 128: 63 / 69 at 8 rows each, 65 / 71 at 24, 66 / 71 at 32, 111 / 72 at 48,
+//   where experts above 32 rows read their weights twice; with rows as a Poisson draw 64 / 71 at 24 on average, 68 / 71
+//   at 28, 87 / 71 at 32. 64 matrices 4096 x 4096: 163 / 169 at 8, 167 / 172 at 24, 252 / 178 at 32 drawn. 384 matrices
+//   4096 x 4096: 900 / 1010 at 2, 1000 / 1020 at 8, 1070 / 1010 at 16, 1100 / 1015 at 24: there 24 is past the crossing.
+//   S counts rows without an expert too, and no spread is known here: 288 rows over 48 matrices 2816 x 2048 with 2,016
+//   rows dropped take 60 us and would take 56; 2,000 of 8,000 rows on one of 384 experts 1090 with either.
 // Returns 8, 16, 32 or 128.
 int choose(const Fp8Product& p) {
   if (!p.offsets) {
     const int64_t n_tiles = (p.N + 127) / 128;
-    if (fp8_skinny_fits(p) && int64_t(p.N) * p.K <= (32 << 20)) return 8;
+    if (fp8_skinny_fits(p)) return 8;
     for (int t = 16; t <= 32; t *= 2)
       if ((p.S + t - 1) / t * n_tiles <= sm_count() && fp8_stream_fits(p.K, t)) return t;
     // more columns than one wave holds, bound by their bytes as long as one tile has all rows

@@ -30,6 +30,7 @@ bool fp8_stream_fits(int K, int rows_per_tile);
 int launch_fp8_skinny(cudaStream_t s, const Fp8Product& p, int out_dtype);
 // the same on rows of f16 or bf16 (x [S][K], row stride ldx), quantized in the kernel
 int launch_fp8_skinny_x(cudaStream_t s, const Fp8Product& p, const void* x, int x_dtype, int64_t ldx, int out_dtype);
+// whether its rows fit in shared memory and its CTAs run in one wave
 bool fp8_skinny_fits(const Fp8Product& p);
 
 }  // namespace b200moe

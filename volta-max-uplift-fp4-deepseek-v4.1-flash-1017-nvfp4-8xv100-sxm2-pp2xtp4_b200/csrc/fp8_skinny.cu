@@ -13,8 +13,10 @@
 // shared memory in a fixed order.
 //
 // Bound: latency. All of a small matrix is in flight at once (16.8 MB for 4096 x
-// 4096: 8 KB per warp, two CTAs per SM): 5.7 us, where the copies and MMAs of the
-// streaming kernel (fp8_stream.cu) take 11.5; past 32 MB its bandwidth wins (14336 x 4096: 18.9 against 13.1).
+// 4096: 8 KB per warp, two CTAs per SM): 6.4 us at one row, 8.0 at eight, where the
+// copies and MMAs of the streaming kernel (fp8_stream.cu) take 9.4. It is taken as
+// long as all CTAs, of 16 or 32 weight rows, run at once (4736 x 4096: 6.7 us, 9.5
+// streamed): CTAs that walk on to a second tile take 9.9 us for 4752 x 4096, streamed 9.5.
 #include <algorithm>
 #include <atomic>
 
@@ -110,21 +112,21 @@ __device__ __forceinline__ void stage_tokens(const SkinnyArgs& A, uint8_t* xs, f
 
 template <typename TX, typename TO, int KS>
 __global__ void __launch_bounds__(kThreads, 2) fp8_skinny_kernel(const SkinnyArgs A) {
-  constexpr int RT = kWarps / KS;  // 16-row tiles of w per item
-  __shared__ float red[2][kWarps][4][32];
+  constexpr int RT = kWarps / KS;  // 16-row tiles of w per CTA
+  __shared__ float red[kWarps][4][32];
   extern __shared__ __align__(16) uint8_t skinny_smem[];
   uint8_t* xs = skinny_smem;                                                     // [8][row_pitch]
   float* ss = reinterpret_cast<float*>(skinny_smem + kTokens * row_pitch(A.KB));  // [8][KB]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int ksub = warp % KS, rsub = warp / KS;
-  const int n_items = (A.N + 16 * RT - 1) / (16 * RT);
+  const int n0 = (blockIdx.x * RT + rsub) * 16;
   const int per_warp = (A.KB + KS - 1) / KS, n_steps = (per_warp + kDeep - 1) / kDeep;
   pdl_wait();
 
   uint4 w[kDeep][4];
   float fb[kDeep];  // the blocks' weight scales, in flight with them
-  auto fetch = [&](int item, int step, int j) {
-    const int kb = (step * kDeep + j) * KS + ksub, n0 = (item * RT + rsub) * 16;
+  auto fetch = [&](int step, int j) {
+    const int kb = (step * kDeep + j) * KS + ksub;
     fb[j] = __ldg(A.w_scale + int64_t(min(n0 / kFp8Block, A.NB - 1)) * A.KB + min(kb, A.KB - 1));
     const uint8_t* p = A.w + int64_t(n0 + g) * A.K + kb * kFp8Block + q * 16;
 #pragma unroll
@@ -136,63 +138,65 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_skinny_kernel(const SkinnyArg
       }
   };
 
-  int item = blockIdx.x, flip = 0;
 #pragma unroll
-  for (int j = 0; j < kDeep; ++j) fetch(item, 0, j);
+  for (int j = 0; j < kDeep; ++j) fetch(0, j);
   stage_tokens<TX>(A, xs, ss);
   __syncthreads();
-  for (; item < n_items; item += gridDim.x, flip ^= 1) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int step = 0; step < n_steps; ++step) {
-      const bool last = step + 1 == n_steps;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int step = 0; step < n_steps; ++step) {
 #pragma unroll
-      for (int j = 0; j < kDeep; ++j) {
-        const int kb = (step * kDeep + j) * KS + ksub;
-        if (kb < A.KB) {  // the same for the whole warp
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < kDeep; ++j) {
+      const int kb = (step * kDeep + j) * KS + ksub;
+      if (kb < A.KB) {  // the same for the whole warp
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint32_t lo[4] = {w[j][c].x, w[j][c].y, w[j][c].z, w[j][c].w};
-            const uint32_t hi[4] = {w[j][2 + c].x, w[j][2 + c].y, w[j][2 + c].z, w[j][2 + c].w};
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t lo[4] = {w[j][c].x, w[j][c].y, w[j][c].z, w[j][c].w};
+          const uint32_t hi[4] = {w[j][2 + c].x, w[j][2 + c].y, w[j][2 + c].z, w[j][2 + c].w};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {  // eight columns of this lane: two MMAs of 16 columns
-              const uint2 l0 = e4m3x4_to_f16(lo[2 * h]), l1 = e4m3x4_to_f16(lo[2 * h + 1]);
-              const uint2 h0 = e4m3x4_to_f16(hi[2 * h]), h1 = e4m3x4_to_f16(hi[2 * h + 1]);
-              const uint4 x = *reinterpret_cast<const uint4*>(
-                  xs + g * row_pitch(A.KB) + (kb * kFp8Block + c * 64 + q * 16 + h * 8) * 2);
-              mma_16816(d, {l0.x, h0.x, l0.y, h0.y}, x.x, x.y);
-              mma_16816(d, {l1.x, h1.x, l1.y, h1.y}, x.z, x.w);
-            }
+          for (int h = 0; h < 2; ++h) {  // eight columns of this lane: two MMAs of 16 columns
+            const uint2 l0 = e4m3x4_to_f16(lo[2 * h]), l1 = e4m3x4_to_f16(lo[2 * h + 1]);
+            const uint2 h0 = e4m3x4_to_f16(hi[2 * h]), h1 = e4m3x4_to_f16(hi[2 * h + 1]);
+            const uint4 x = *reinterpret_cast<const uint4*>(
+                xs + g * row_pitch(A.KB) + (kb * kFp8Block + c * 64 + q * 16 + h * 8) * 2);
+            mma_16816(d, {l0.x, h0.x, l0.y, h0.y}, x.x, x.y);
+            mma_16816(d, {l1.x, h1.x, l1.y, h1.y}, x.z, x.w);
           }
-          const float* sp = ss + 2 * q * A.KB + kb;
-          const float s0 = sp[0] * fb[j], s1 = sp[A.KB] * fb[j];
-          acc[0] = fmaf(d[0], s0, acc[0]);
-          acc[1] = fmaf(d[1], s1, acc[1]);
-          acc[2] = fmaf(d[2], s0, acc[2]);
-          acc[3] = fmaf(d[3], s1, acc[3]);
         }
-        if (!last)
-          fetch(item, step + 1, j);
-        else if (item + gridDim.x < n_items)
-          fetch(item + gridDim.x, 0, j);
+        const float* sp = ss + 2 * q * A.KB + kb;
+        const float s0 = sp[0] * fb[j], s1 = sp[A.KB] * fb[j];
+        acc[0] = fmaf(d[0], s0, acc[0]);
+        acc[1] = fmaf(d[1], s1, acc[1]);
+        acc[2] = fmaf(d[2], s0, acc[2]);
+        acc[3] = fmaf(d[3], s1, acc[3]);
       }
+      if (step + 1 < n_steps) fetch(step + 1, j);
     }
+  }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) red[flip][warp][i][lane] = acc[i];
-    __syncthreads();  // the other buffer's readers have passed the last item's barrier
-    for (int o = ksub * 32 + lane; o < 16 * kTokens; o += KS * 32) {
-      const int t = o >> 4, r = o & 15, col = (item * RT + rsub) * 16 + r;
-      const int slot = (r >> 3) * 2 + (t & 1), src = (r & 7) * 4 + (t >> 1);
-      float sum = 0.f;
+  for (int i = 0; i < 4; ++i) red[warp][i][lane] = acc[i];
+  __syncthreads();
+  for (int o = ksub * 32 + lane; o < 16 * kTokens; o += KS * 32) {
+    const int t = o >> 4, r = o & 15, col = n0 + r;
+    const int slot = (r >> 3) * 2 + (t & 1), src = (r & 7) * 4 + (t >> 1);
+    float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < KS; ++k) sum += red[flip][rsub * KS + k][slot][src];
-      if (t < A.S && col < A.N) static_cast<TO*>(A.out)[int64_t(t) * A.N + col] = from_f32<TO>(sum);
-    }
+    for (int k = 0; k < KS; ++k) sum += red[rsub * KS + k][slot][src];
+    if (t < A.S && col < A.N) static_cast<TO*>(A.out)[int64_t(t) * A.N + col] = from_f32<TO>(sum);
   }
   pdl_trigger();
 }
 
+// Eight warps along K where each still has four K blocks, else two row tiles of four warps: one row of 4096 x 4096
+// takes 6.4 us with eight and 8.3 with four, of 4096 x 2176 4.2 and 5.0, of 2816 x 2048 3.9 and 3.5.
+bool deep(int KB) { return KB > 4 * kDeep; }
+int skinny_grid(int N, int KB) {
+  const int rows = 16 * (deep(KB) ? 1 : 2);
+  return (N + rows - 1) / rows;
+}
+
 size_t skinny_smem_bytes(int KB) { return size_t(kTokens) * (row_pitch(KB) + KB * sizeof(float)); }
+int skinny_ctas(int KB) { return sm_count() * (skinny_smem_bytes(KB) <= 100 * 1024 ? 2 : 1); }  // that run at once
 
 template <typename TX, typename TO, int KS>
 int launch_one(cudaStream_t s, const SkinnyArgs& a) {
@@ -205,21 +209,18 @@ int launch_one(cudaStream_t s, const SkinnyArgs& a) {
       return -1;
     attr_set.fetch_or(uint64_t(1) << dev);
   }
-  const int items = (a.N + 16 * (kWarps / KS) - 1) / (16 * (kWarps / KS));
-  const size_t smem = skinny_smem_bytes(a.KB);
-  const int ctas = sm_count() * (smem <= 100 * 1024 ? 2 : 1);
-  return launch_chain(kernel, dim3(std::min(ctas, items)), dim3(kThreads), smem, s, a) == cudaSuccess ? 0 : -1;
+  return launch_chain(kernel, dim3(skinny_grid(a.N, a.KB)), dim3(kThreads), skinny_smem_bytes(a.KB), s, a) == cudaSuccess
+             ? 0
+             : -1;
 }
 
-// Eight warps along K where each still has four K blocks, else two row tiles of four warps: 4096 x 4096 takes 6.8 us
-// with eight and 7.5 with four.
 template <typename TX>
 int launch_out(cudaStream_t s, const SkinnyArgs& a, int out_dtype) {
-  const bool deep = a.KB > 4 * kDeep;
-  if (out_dtype == B200MOE_F16) return deep ? launch_one<TX, __half, 8>(s, a) : launch_one<TX, __half, 4>(s, a);
+  const bool d = deep(a.KB);
+  if (out_dtype == B200MOE_F16) return d ? launch_one<TX, __half, 8>(s, a) : launch_one<TX, __half, 4>(s, a);
   if (out_dtype == B200MOE_BF16)
-    return deep ? launch_one<TX, __nv_bfloat16, 8>(s, a) : launch_one<TX, __nv_bfloat16, 4>(s, a);
-  return deep ? launch_one<TX, float, 8>(s, a) : launch_one<TX, float, 4>(s, a);
+    return d ? launch_one<TX, __nv_bfloat16, 8>(s, a) : launch_one<TX, __nv_bfloat16, 4>(s, a);
+  return d ? launch_one<TX, float, 8>(s, a) : launch_one<TX, float, 4>(s, a);
 }
 
 SkinnyArgs args_of(const Fp8Product& p) {
@@ -241,8 +242,9 @@ SkinnyArgs args_of(const Fp8Product& p) {
 }  // namespace
 
 bool fp8_skinny_fits(const Fp8Product& p) {
-  return p.E == 1 && !p.offsets && p.S <= kTokens &&
-         skinny_smem_bytes((p.K + kFp8Block - 1) / kFp8Block) <= size_t(kSkinnySmem);
+  const int KB = (p.K + kFp8Block - 1) / kFp8Block;
+  return p.E == 1 && !p.offsets && p.S <= kTokens && skinny_smem_bytes(KB) <= size_t(kSkinnySmem) &&
+         skinny_grid(p.N, KB) <= skinny_ctas(KB);
 }
 
 int launch_fp8_skinny(cudaStream_t s, const Fp8Product& p, int out_dtype) {
