@@ -326,9 +326,10 @@ __device__ __forceinline__ float warp_sum8(const float (&v)[8], int lane) {
 
 // A CTA per token: g[t] is read once for up to eight slots; each slot's row is
 // read for the dot product and its gradient row written in the same pass.
-// Three CTAs per SM where the registers allow it: 95 us at 4096 tokens of 8 x 4096, 99 with two.
+// CTAs per SM, for 4096 tokens of 8 x 4096: 16-bit rows and gradients take 98 us with three, 114 with two (although
+// the 80 registers of three spill 72 to 80 bytes); f32 gradients of 16-bit rows 132 with three (160 bytes), 105 with two.
 template <typename TG, typename TI, int V, bool WIDE>
-__global__ void __launch_bounds__(256, WIDE && sizeof(TI) == 2 ? 3 : 2) unpermute_grad_kernel(const TG* __restrict__ grad, int64_t grad_stride,
+__global__ void __launch_bounds__(256, WIDE && sizeof(TG) == 2 ? 3 : 2) unpermute_grad_kernel(const TG* __restrict__ grad, int64_t grad_stride,
                                                              const TI* __restrict__ rows,
                                                              const int32_t* __restrict__ row_of_route,
                                                              const float* __restrict__ weights, int T, int k, int H,
