@@ -52,6 +52,21 @@ def test_swiglu_gives_the_bits_of_its_definition(ops, dtype, rows, width):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,width", [(2000, 1408), (1500, 1401), (1, 2048)])
+def test_swiglu_gradient_by_the_steps_of_its_formula(ops, dtype, rows, width):
+    """d u (s (1 + g (1 - s))) and d (g s), each operation rounded to f32, the result once more: no bit may differ."""
+    h, d = randn(rows, rows, 2 * width, dtype=dtype) * 4, randn(width, rows, width, dtype=dtype)
+    gate, up = h.float().chunk(2, 1)
+    g, u = gate.clamp(max=10.0), up.clamp(-10.0, 10.0)
+    one = torch.ones((), device="cuda")
+    s = one / (1 + torch.exp(-g))
+    dg = torch.where(gate > 10.0, 0.0, d.float() * u * (s * (1 + g * (1 - s))))
+    du = torch.where(up.abs() > 10.0, 0.0, d.float() * (g * s))
+    assert torch.equal(ops.fp8.swiglu_grad(h, d), torch.cat([dg, du], 1).to(dtype))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("limit", [None, 3e38])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("width", [128, 33])

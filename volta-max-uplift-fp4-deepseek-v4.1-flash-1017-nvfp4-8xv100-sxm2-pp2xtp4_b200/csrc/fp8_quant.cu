@@ -201,7 +201,8 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_rows_any_kernel(const T* __
   }
 }
 
-// d gate = d u s (1 + g (1 - s)) where gate <= limit, d up = d g s where |up| <= limit, s = 1 / (1 + e^-g).
+// d gate = d u (s (1 + g (1 - s))) where gate <= limit, d up = d (g s) where |up| <= limit, s = 1 / (1 + e^-g), one f32
+// operation at a time: the bits do not depend on which products the compiler fuses.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kQuantThreads) swiglu_grad_kernel(const T* __restrict__ h, int64_t h_stride,
                                                                     const T* __restrict__ grad, int64_t grad_stride,
@@ -225,9 +226,9 @@ __global__ void __launch_bounds__(kQuantThreads) swiglu_grad_kernel(const T* __r
       const float g0 = gate.get(i), u0 = up.get(i), di = d.get(i);
       const float g = limited_gate(g0, limit), u = limited_up(u0, limit);
       const float s = __frcp_rn(1.f + expf(-g));
-      const float gs = g * s;
-      dg[i] = g0 > limit ? 0.f : di * u * fmaf(gs, 1.f - s, s);
-      du[i] = fabsf(u0) > limit ? 0.f : di * gs;
+      const float slope = __fmul_rn(s, __fadd_rn(1.f, __fmul_rn(g, __fsub_rn(1.f, s))));
+      dg[i] = g0 > limit ? 0.f : __fmul_rn(__fmul_rn(di, u), slope);
+      du[i] = fabsf(u0) > limit ? 0.f : __fmul_rn(di, __fmul_rn(g, s));
     }
     T* dst = grad_h + at.row * 2 * width;
     store_columns<WIDE>(dst, c, step, width, dg);
