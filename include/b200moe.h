@@ -347,8 +347,8 @@ int b200moe_fold_nvfp4_to_mxfp4(void* stream, const uint8_t* codes, const uint8_
  * the reference, whose experts are FP4 and GGUF only and are never trained).
  * They run on the current device, allocate nothing and never wait for the
  * host.  A row or offset out of range is left out and sets a bit in the current
- * device's operator error word, read and cleared (after `stream`) by
- * b200moe_op_errors. */
+ * device's operator error word; b200moe_op_errors reads it (after `stream`) and
+ * clears the bits that it read. */
 int b200moe_op_errors(void* stream, uint32_t* bits);
 
 /* Routes sorted by expert (stable; ids int32 [routes], routes = T * k <= 2^26,
@@ -377,7 +377,8 @@ int b200moe_unpermute(void* stream, const void* rows, int dtype, const int32_t* 
 
 /* Its gradients: grad_rows[row] = weights[t][s] * grad[t] (zeros in the row of a
  * route without an expert), grad_weights[t][s] = <grad[t], rows[row]> in f32.
- * Either may be NULL.  grad: dtype or F32, grad_stride elements between tokens. */
+ * A row's gradient is written by the route that names it, so row_of_route has to
+ * name every row once (~row for a route without an expert).  Either may be NULL.  grad: dtype or F32, grad_stride elements between tokens. */
 int b200moe_unpermute_grad(void* stream, const void* grad, int grad_dtype, int64_t grad_stride, const void* rows,
                            int dtype, const int32_t* row_of_route, const float* weights, int T, int k, int H,
                            void* grad_rows, float* grad_weights);
@@ -409,7 +410,7 @@ int b200moe_fp8_matmul(void* stream, const void* a, const float* a_scale, int64_
                        int out_dtype);
 /* The same for one matrix and rows x of f16, bf16 or f32 (ldx elements between
  * them), quantized in the call: inside the product's kernel for up to 8 rows of
- * 16 bits on 16-byte addresses, else into the workspace
+ * 16 bits on 16-byte addresses (and a matrix of one wave of its CTAs), else into the workspace
  * (b200moe_fp8_linear_workspace_bytes, on a 16-byte address; the 0 it gives for
  * few rows holds for such x only, S * (K + 4 ceil(K / 128)) + 16 always suffices). */
 size_t b200moe_fp8_linear_workspace_bytes(int S, int N, int K);

@@ -6,7 +6,12 @@
 // Row blocks are 1 x 128: eight lanes hold a block, sixteen columns each (two
 // 16-byte loads of 16-bit values), so the maximum is three shuffles and a block
 // is read once.  Weight blocks are 128 x 128: a CTA holds one in registers.
-// Bound: HBM (f32 or 16-bit columns in, one byte out).
+// Bound: HBM (f32 or 16-bit columns in, one byte out) for rows as they are: 8192 x
+// 4096 bf16 in 18 to 19 us; instruction issue for the SwiGLU: 39 per value with f32's
+// own exponential and division, 74 % of the slots, 49152 x 1408 in 96 us (floor 53).
+// Its gradient issues 47 per value and takes 115 us (floor 106). The hardware's
+// power of two and reciprocal in their place took 66 and 102 us and moved single
+// codes off the definition's; launch bounds of five or six CTAs per SM 96 and 106.
 #include <algorithm>
 
 #include "fp8_device.cuh"
@@ -17,8 +22,8 @@ namespace {
 
 constexpr int kQuantThreads = 256;
 constexpr int kQuantBlocks = kQuantThreads / 8;  // row blocks of a CTA's turn
-// CTAs at most, for walks of several turns: SwiGLU of 49152 x 1408 takes 70 us with 16 per SM, 72 with 8 and 77
-// without a cap, its gradient 102 us with 48 per SM, 116 without a cap and 108 with 16
+// CTAs at most, for walks of several turns: SwiGLU of 49152 x 1408 takes 97 us with 16 per SM, 102 with 8 and 99
+// without a cap, its gradient 113 us with 48 per SM, 128 without a cap and 116 with 16 (115 now, its steps fixed since)
 constexpr int64_t kCtaCap = 148 * 16, kGradCap = 148 * 48, kAnyCap = 148 * 32;
 
 // Minimum / maximum that keep a NaN.

@@ -13,11 +13,12 @@
 //   warps 2-5 (sums): a thread holds one weight row; product times the weight
 //     block's scale and each token's (in shared memory, four per load) joins the
 //     f32 sums of its NTOK columns.
-// 190 experts of 4096 x 4096 for 256 rows: 461 us, 6.95 TB/s, the rate of a plain
-// copy and a little more (it reads only). Streaming the weights through registers
+// 192 experts of 4096 x 4096 for 256 rows: 456 us, 7.06 TB/s (it reads only; a plain
+// copy reaches 6.55). Streaming the weights through registers
 // into mma.sync instead reached 4.9 TB/s at best. One matrix of 4096 x 4096 for 64
-// rows has 32 x 4 items and takes 9.2 us: 0.18 per K block, 3 for launch, first
-// bytes and stores; with one MMA warp 10.7.
+// rows has 32 x 4 items, so 20 SMs idle and each of the others walks K alone: 9.8 us,
+// 0.18 per K block, the rest launch, first bytes and stores; one MMA warp took 1.5
+// more. Up to 16 rows it has 32 items only and takes 9.6 us: K is not split.
 #include <cuda.h>
 
 #include <algorithm>

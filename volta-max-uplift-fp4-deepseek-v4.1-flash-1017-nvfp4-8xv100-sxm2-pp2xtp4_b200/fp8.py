@@ -5,9 +5,11 @@ Activations carry a scale per row and 128 columns, weights one per 128 x 128 blo
     amax = max(max |x|, 1e-30)    scale = amax / 448    q = e4m3(x * (448 / amax))
 
 A NaN or an infinity in a block makes the whole block, and so its product's row,
-NaN.  Products sum in f32.  Weights are frozen: gradients flow to activations (a
-second product, of the quantized gradient with the transposed weights), never to
-the packed weights.  Arguments that do not fit raise ``ValueError`` (an address off
+NaN.  Products sum in f32.  Weights are frozen: ``linear`` has a gradient in its rows (a
+second product, of the quantized gradient with the transposed weights), never in
+the packed weights.  The quantizers, ``matmul`` and ``grouped_matmul`` return values
+without a graph; ``experts.Fp8Experts`` puts the gradients of the whole path together.
+Arguments that do not fit raise ``ValueError`` (an address off
 16 bytes ``B200MoeError``); offsets out of range are cut and reported by
 ``check_errors``.
 """

@@ -36,7 +36,9 @@ class Permuted(NamedTuple):
 
 def sort_routes(topk_ids: torch.Tensor, num_experts: int) -> tuple[torch.Tensor, torch.Tensor]:
     """int32 ids [T, k] -> (row_of_route int32 [T, k], offsets int32 [num_experts + 1]).
-    At most 1024 experts and 2^26 routes."""
+    At most 1024 experts and 2^26 routes.  Every 2048 routes read the counts of all the
+    others, so the time grows with the square of the routes: 13 us at 131,072 of them
+    (384 experts), 88 us at 2^20, 3.7 ms at 2^23."""
     return _lib.ops().sort_routes(topk_ids, num_experts)
 
 
@@ -50,7 +52,10 @@ def permute(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int, scale: to
 def unpermute(rows: torch.Tensor, row_of_route: torch.Tensor, weights: torch.Tensor | None = None,
               out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``out[t] = sum_s weights[t, s] * rows[row_of_route[t, s]]`` over the routes that
-    have an expert (``weights`` f32 [T, k], None: ones); ``out_dtype``: the rows' or f32."""
+    have an expert (``weights`` f32 [T, k], None: ones); ``out_dtype``: the rows' or f32.
+    ``row_of_route`` is ``permute``'s or another map of the same form: the gradients
+    need every row named exactly once, also those of dropped routes (``~row``, not any
+    negative number), since each row's gradient is written by the route that names it."""
     return _lib.ops().unpermute(rows, row_of_route, weights, out_dtype)
 
 
