@@ -417,6 +417,66 @@ size_t b200moe_fp8_linear_workspace_bytes(int S, int N, int K);
 int b200moe_fp8_linear(void* stream, const void* x, int x_dtype, int64_t ldx, const void* w, const float* w_scale,
                        int S, int N, int K, void* out, int out_dtype, void* workspace, size_t workspace_bytes);
 
+/* Rows to 4-bit floating point (E2M1) records of b200moe_fp4_record_bytes(format,
+ * k) bytes each, formats B200MOE_NVFP4 and B200MOE_MXFP4 (0: k is not a multiple
+ * of 32 or the format unknown).  A record: k / 2 bytes of codes (the even column
+ * in the low bits), k / 16 E4M3 or k / 32 E8M0 scales, for NVFP4 on the next
+ * multiple of 4 the row's f32 factor, zeros up to a multiple of 16.
+ *   NVFP4: factor = the smallest 2^e with 2688 * 2^e >= max |x| (at least 2^-100),
+ *     scale = e4m3(block max / (6 factor)), q = e2m1(x / (scale factor));
+ *   MXFP4: scale = 2^e, the smallest with 6 * 2^e >= block max, q = e2m1(x / 2^e).
+ * swiglu: x holds 2 k columns, the SwiGLU of b200moe_fp8_quantize is quantized.  A
+ * NaN or an infinity makes the factor, or the block's scale, a NaN.  records on 16
+ * bytes. */
+int b200moe_fp4_record_bytes(int format, int k);
+int b200moe_fp4_quantize(void* stream, const void* x, int dtype, int64_t x_stride, int rows, int k, int format,
+                         int swiglu, float limit, void* records);
+/* Weights w [mats][n][k] by the same steps, an NVFP4 factor per matrix: codes
+ * [mats][n][k / 2] on 16 bytes, scale [mats][n][k / 16 or k / 32], factor [mats]
+ * (MXFP4: NULL). */
+int b200moe_fp4_quantize_weight(void* stream, const void* w, int dtype, int mats, int n, int k, int format, void* codes,
+                                void* scale, float* factor);
+/* What codes, scales and factors (NULL: 1) stand for: out [rows][k] = value *
+ * scale * factor, rounded once.  ld_*: bytes between rows (ld_factor 0: one factor
+ * for all); codes on 8 bytes, ld_codes a multiple of 8. */
+int b200moe_fp4_values(void* stream, const void* codes, int64_t ld_codes, const void* scale, int64_t ld_scale,
+                       const void* factor, int64_t ld_factor, int64_t rows, int k, int format, void* out, int dtype);
+/* out [S][N] = records a [S] . w^T with scales and factors, f32 sums: w [E][N][K / 2]
+ * codes, w_scale [E][N][K / 16 or K / 32], w_factor [E] (MXFP4: not read).  offsets
+ * as in b200moe_fp8_matmul.  K a multiple of 32, a and w on 16 bytes, E <= 1024. */
+int b200moe_fp4_matmul(void* stream, const void* a, const void* w, const void* w_scale, const float* w_factor,
+                       const int32_t* offsets, int S, int N, int K, int E, int format, void* out, int out_dtype);
+/* The same for one matrix and rows x of f16, bf16 or f32 (ldx elements between
+ * them), quantized in the call, into the workspace where b200moe_fp4_linear_workspace_bytes
+ * is not 0 (on a 16-byte address; S * b200moe_fp4_record_bytes always suffices).  0
+ * holds for 16-bit x on 16 bytes, rows a multiple of 16 bytes apart. */
+size_t b200moe_fp4_linear_workspace_bytes(int S, int N, int K, int format);
+int b200moe_fp4_linear(void* stream, const void* x, int x_dtype, int64_t ldx, const void* w, const void* w_scale,
+                       const float* w_factor, int S, int N, int K, int format, void* out, int out_dtype, void* workspace,
+                       size_t workspace_bytes);
+
+/* Root-mean-square norm of rows [rows][width], width <= 16384:
+ *   s = x + residual, rounded to the residual's type and stored in sum [rows][width]
+ *   (residual NULL: s = x, sum not written); y = s / sqrt(mean(s^2) + eps) * weight.
+ * residual_f32 / weight_f32: f32 instead of x's type.  eps: 1e-20 or more.
+ * out 0: y [rows][width] of x's type.  out 1, 2, 3: y in f32, quantized to E4M3 with a
+ * scale per 128 columns (q, scale as b200moe_fp8_quantize), or to NVFP4 or MXFP4
+ * records (q; width a multiple of 32); y is written too where it is not NULL.  q on
+ * 16 bytes. */
+int b200moe_rms_norm(void* stream, const void* x, int dtype, int64_t x_stride, const void* residual, int residual_f32,
+                     int64_t residual_stride, const void* weight, int weight_f32, float eps, int rows, int width, void* sum,
+                     void* y, int out, void* q, float* scale);
+/* Its gradient from the stored sum s (f32 where s_f32, else of dtype): with u = s rstd, g = weight grad_y,
+ *   grad_s' = rstd (g - u mean(g u)) + grad_s (grad_s NULL: 0), of s's type in grad_sum, of dtype in grad_x;
+ *   grad_weight = sum over rows of grad_y u, of the weight's type, joined in a fixed order through the
+ *   workspace (b200moe_rms_norm_grad_workspace_bytes, on 16 bytes).
+ * Any of grad_x, grad_sum, grad_weight may be NULL. */
+size_t b200moe_rms_norm_grad_workspace_bytes(int rows, int width);
+int b200moe_rms_norm_grad(void* stream, const void* s, int s_f32, int64_t s_stride, const void* grad_y, int dtype,
+                          int64_t grad_y_stride, const void* grad_s, int64_t grad_s_stride, const void* weight,
+                          int weight_f32, float eps, int rows, int width, void* grad_x, void* grad_sum, void* grad_weight,
+                          void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

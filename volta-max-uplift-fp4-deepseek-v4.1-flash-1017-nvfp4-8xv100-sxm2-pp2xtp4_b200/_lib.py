@@ -109,6 +109,16 @@ SIGNATURES = {
     "b200moe_fp8_matmul": ([P, P, P, I64, P, P, P, I32, I32, I32, I32, P, I32], I32),
     "b200moe_fp8_linear_workspace_bytes": ([I32, I32, I32], SIZE),
     "b200moe_fp8_linear": ([P, P, I32, I64, P, P, I32, I32, I32, P, I32, P, SIZE], I32),
+    "b200moe_fp4_record_bytes": ([I32, I32], I32),
+    "b200moe_fp4_quantize": ([P, P, I32, I64, I32, I32, I32, I32, F32, P], I32),
+    "b200moe_fp4_quantize_weight": ([P, P, I32, I32, I32, I32, I32, P, P, P], I32),
+    "b200moe_fp4_values": ([P, P, I64, P, I64, P, I64, I64, I32, I32, P, I32], I32),
+    "b200moe_fp4_matmul": ([P, P, P, P, P, P, I32, I32, I32, I32, I32, P, I32], I32),
+    "b200moe_fp4_linear_workspace_bytes": ([I32, I32, I32, I32], SIZE),
+    "b200moe_fp4_linear": ([P, P, I32, I64, P, P, P, I32, I32, I32, I32, P, I32, P, SIZE], I32),
+    "b200moe_rms_norm": ([P, P, I32, I64, P, I32, I64, P, I32, F32, I32, I32, P, P, I32, P, P], I32),
+    "b200moe_rms_norm_grad_workspace_bytes": ([I32, I32], SIZE),
+    "b200moe_rms_norm_grad": ([P, P, I32, I64, P, I32, I64, P, I64, P, I32, F32, I32, I32, P, P, P, P, SIZE], I32),
     "b200moe_mma_peak": ([I32, I32, I32, ctypes.POINTER(F32), ctypes.POINTER(F32)], I32),
 }
 
@@ -149,7 +159,7 @@ _OPS = None
 
 
 def ops():
-    """The torch binding of the stateless operators (``permute``, ``fp8``), which calls
+    """The torch binding of the stateless operators (``permute``, ``fp8``, ``fp4``, ``norm``), which calls
     the library; built and pinned with it (raises when missing: no fallback exists)."""
     global _OPS
     if _OPS is None:

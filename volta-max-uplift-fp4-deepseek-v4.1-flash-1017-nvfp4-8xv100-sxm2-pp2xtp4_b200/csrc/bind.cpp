@@ -1,4 +1,4 @@
-// The stateless operators (permute, fp8) as torch calls: argument checks, output
+// The stateless operators (permute, fp8, fp4, norm) as torch calls: argument checks, output
 // tensors, the current stream and the gradients around the C entry points of
 // b200moe.h. Written against torch's C++ interface because these calls are short:
 // a decode step's operator runs 2-6 us on the GPU, where the same call through
@@ -44,7 +44,7 @@ void check(const char* where, int status) {
 }
 
 // ------------------------------------------------------------------ checks
-enum Kind { kFloats, kFloatsOrE4m3, kOnlyE4m3, kF32, kI32 };
+enum Kind { kFloats, kFloatsOrE4m3, kOnlyE4m3, kF32, kU8, kI32 };
 
 bool is_float(ScalarType t) {
   return t == ScalarType::BFloat16 || t == ScalarType::Half || t == ScalarType::Float;
@@ -55,12 +55,13 @@ bool fits(ScalarType t, Kind k) {
     case kFloatsOrE4m3: return is_float(t) || t == kE4m3;
     case kOnlyE4m3: return t == kE4m3;
     case kF32: return t == ScalarType::Float;
+    case kU8: return t == ScalarType::Byte;
     default: return t == ScalarType::Int;
   }
 }
 const char* kind_name(Kind k) {
   const char* names[] = {"bfloat16/float16/float32", "bfloat16/float16/float32/float8_e4m3fn", "float8_e4m3fn",
-                         "float32", "int32"};
+                         "float32", "uint8", "int32"};
   return names[k];
 }
 int code(ScalarType t) {
@@ -493,6 +494,325 @@ Tensor linear(const Tensor& x, const Tensor& w, const Tensor& w_scale, const Opt
   return run_linear(x, w, w_scale, dtype);
 }
 
+// ----------------------------------------------------- 4-bit rows and products
+constexpr int kNvfp4 = B200MOE_NVFP4, kMxfp4 = B200MOE_MXFP4;
+
+int64_t record_bytes(int64_t format, int64_t k) {
+  TORCH_CHECK_VALUE(format == kNvfp4 || format == kMxfp4, "unknown 4-bit format ", format);
+  TORCH_CHECK_VALUE(k >= 32 && k % 32 == 0 && k <= (1 << 24), "4-bit rows need a multiple of 32 columns, got ", k);
+  return b200moe_fp4_record_bytes(int(format), int(k));
+}
+int64_t fp4_scales(int64_t format, int64_t k) { return k / (format == kMxfp4 ? 32 : 16); }
+
+Tensor run_fp4_quantize(const Tensor& x, int64_t k, int64_t format, bool swiglu, float limit) {
+  const int64_t bytes = record_bytes(format, k), rows = x.size(0);
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor out = empty({rows, bytes}, ScalarType::Byte, x);
+  if (rows)
+    check("b200moe_fp4_quantize",
+          b200moe_fp4_quantize(stream(x), x.data_ptr(), code(x.scalar_type()), x.stride(0), int(rows), int(k),
+                               int(format), swiglu, limit, out.data_ptr()));
+  return out;
+}
+
+Tensor fp4_quantize(const Tensor& x, int64_t format) {
+  want("x", x, kFloats, 2, nullptr, true);
+  return run_fp4_quantize(x, x.size(1), format, false, 1.f);
+}
+
+Tensor fp4_swiglu_quantize(const Tensor& h, const std::optional<double>& limit, int64_t format) {
+  check_gate_up(h);
+  return run_fp4_quantize(h, h.size(1) / 2, format, true, check_limit(limit));
+}
+
+std::tuple<Tensor, Tensor, OptTensor> fp4_quantize_weight(const Tensor& w, int64_t format) {
+  const bool many = w.defined() && w.dim() == 3;
+  want("w", w, kFloats, many ? 3 : 2);
+  TORCH_CHECK_VALUE(w.numel() > 0, "w must not be empty, got ", w.sizes());
+  const int64_t n = w.size(-2), k = w.size(-1), mats = many ? w.size(0) : 1;
+  record_bytes(format, k);
+  TORCH_CHECK_VALUE(mats <= 65535, "w is too large: ", w.sizes());
+  const c10::cuda::CUDAGuard guard(w.device());
+  auto shaped = [&](int64_t last) {
+    return many ? empty({mats, n, last}, ScalarType::Byte, w) : empty({n, last}, ScalarType::Byte, w);
+  };
+  Tensor codes = shaped(k / 2), scale = shaped(fp4_scales(format, k)), factor;
+  if (format == kNvfp4) factor = empty({mats}, ScalarType::Float, w);
+  check("b200moe_fp4_quantize_weight",
+        b200moe_fp4_quantize_weight(stream(w), w.data_ptr(), code(w.scalar_type()), int(mats), int(n), int(k),
+                                    int(format), codes.data_ptr(), scale.data_ptr(), f32_mut(factor)));
+  return {codes, scale, factor.defined() ? OptTensor(factor) : std::nullopt};
+}
+
+void check_records(const Tensor& record, int64_t k, int64_t format) {
+  want("record", record, kU8, 2);
+  TORCH_CHECK_VALUE(record.size(1) == record_bytes(format, k), "a record of ", k, " columns has ",
+                    record_bytes(format, k), " bytes, got ", record.sizes());
+}
+
+// Packed weights [(E,) N, K]; returns their format: MXFP4 without a factor, NVFP4 with one per matrix.
+int64_t check_fp4_weight(const Tensor& codes, const Tensor& scale, const Tensor& factor, int64_t dim, const Tensor* like) {
+  want("codes", codes, kU8, dim, like);
+  want("scale", scale, kU8, dim, &codes);
+  TORCH_CHECK_VALUE(codes.numel() > 0, "codes must not be empty, got ", codes.sizes());
+  const int64_t format = factor.defined() ? kNvfp4 : kMxfp4, k = 2 * codes.size(-1), mats = dim == 3 ? codes.size(0) : 1;
+  record_bytes(format, k);
+  at::DimVector shape(codes.sizes());
+  shape.back() = fp4_scales(format, k);
+  TORCH_CHECK_VALUE(scale.sizes() == at::IntArrayRef(shape), "scale must have shape ", at::IntArrayRef(shape),
+                    factor.defined() ? " (NVFP4, which a factor makes it)" : " (MXFP4, which no factor makes it)",
+                    ", got ", scale.sizes());
+  if (factor.defined()) {
+    want("factor", factor, kF32, 1, &codes);
+    want_shape("factor", factor, {mats});
+  }
+  TORCH_CHECK_VALUE(mats * codes.size(-2) <= INT32_MAX - 256, "at most 2^31 weight rows, got ", codes.sizes());
+  return format;
+}
+
+int64_t fp4_weight_format(const Tensor& codes, const Tensor& scale, const OptTensor& factor) {
+  return check_fp4_weight(codes, scale, factor.value_or(Tensor()), codes.defined() && codes.dim() == 3 ? 3 : 2, nullptr);
+}
+
+Tensor run_fp4_values(const Tensor& like, const uint8_t* codes, int64_t ld_codes, const uint8_t* scale, int64_t ld_scale,
+                      const void* factor, int64_t ld_factor, int64_t rows, int64_t k, int64_t format, const Tensor& out) {
+  if (rows)
+    check("b200moe_fp4_values",
+          b200moe_fp4_values(stream(like), codes, ld_codes, scale, ld_scale, factor, ld_factor, rows, int(k), int(format),
+                             out.data_ptr(), code(out.scalar_type())));
+  return out;
+}
+
+Tensor fp4_rows_values(const Tensor& record, int64_t k, int64_t format, ScalarType dtype) {
+  check_records(record, k, format);
+  TORCH_CHECK_VALUE(is_float(dtype), "dtype must be bfloat16, float16 or float32, got ", dtype);
+  const c10::cuda::CUDAGuard guard(record.device());
+  const int64_t rows = record.size(0), ld = record.size(1), scales = k / 2;
+  const uint8_t* p = static_cast<const uint8_t*>(record.data_ptr());
+  const void* factor = format == kNvfp4 ? p + scales + (k / 16 + 3) / 4 * 4 : nullptr;
+  return run_fp4_values(record, p, ld, p + scales, ld, factor, ld, rows, k, format, empty({rows, k}, dtype, record));
+}
+
+Tensor fp4_weight_values(const Tensor& codes, const Tensor& scale, const OptTensor& factor_arg, ScalarType dtype) {
+  const Tensor factor = factor_arg.value_or(Tensor());
+  const bool many = codes.defined() && codes.dim() == 3;
+  const int64_t format = check_fp4_weight(codes, scale, factor, many ? 3 : 2, nullptr);
+  TORCH_CHECK_VALUE(is_float(dtype), "dtype must be bfloat16, float16 or float32, got ", dtype);
+  const c10::cuda::CUDAGuard guard(codes.device());
+  const int64_t n = codes.size(-2), half = codes.size(-1), mats = many ? codes.size(0) : 1, ns = scale.size(-1);
+  Tensor out = many ? empty({mats, n, 2 * half}, dtype, codes) : empty({n, 2 * half}, dtype, codes);
+  for (int64_t e = 0; e < mats; ++e)
+    run_fp4_values(codes, static_cast<const uint8_t*>(codes.data_ptr()) + e * n * half, half,
+                   static_cast<const uint8_t*>(scale.data_ptr()) + e * n * ns, ns,
+                   factor.defined() ? f32(factor) + e : nullptr, 0, n, 2 * half, format, many ? out.select(0, e) : out);
+  return out;
+}
+
+Tensor run_fp4_product(const Tensor& record, int64_t k, int64_t format, const Tensor& offsets, const Tensor& codes,
+                       const Tensor& scale, const Tensor& factor, ScalarType out_dtype) {
+  const c10::cuda::CUDAGuard guard(record.device());
+  const int64_t s = record.size(0), n = codes.size(-2);
+  Tensor out = empty({s, n}, out_dtype, record);
+  if (s)
+    check("b200moe_fp4_matmul",
+          b200moe_fp4_matmul(stream(record), record.data_ptr(), codes.data_ptr(), scale.data_ptr(), f32(factor),
+                             offsets.defined() ? i32(offsets) : nullptr, int(s), int(n), int(k),
+                             offsets.defined() ? int(codes.size(0)) : 1, int(format), out.data_ptr(), code(out_dtype)));
+  return out;
+}
+
+void check_fp4_product(const Tensor& record, int64_t k, int64_t format, const Tensor& codes, const Tensor& scale,
+                       const Tensor& factor, int64_t dim, ScalarType out_dtype) {
+  check_records(record, k, format);
+  TORCH_CHECK_VALUE(check_fp4_weight(codes, scale, factor, dim, &record) == format,
+                    "the rows and the weights have different formats");
+  TORCH_CHECK_VALUE(2 * codes.size(-1) == k, "the weights have ", 2 * codes.size(-1), " columns, the rows ", k);
+  check_out(out_dtype);
+}
+
+Tensor fp4_matmul(const Tensor& record, int64_t k, int64_t format, const Tensor& codes, const Tensor& scale,
+                  const OptTensor& factor, ScalarType out_dtype) {
+  check_fp4_product(record, k, format, codes, scale, factor.value_or(Tensor()), 2, out_dtype);
+  return run_fp4_product(record, k, format, Tensor(), codes, scale, factor.value_or(Tensor()), out_dtype);
+}
+
+Tensor fp4_grouped_matmul(const Tensor& record, int64_t k, int64_t format, const Tensor& offsets, const Tensor& codes,
+                          const Tensor& scale, const OptTensor& factor, ScalarType out_dtype) {
+  check_fp4_product(record, k, format, codes, scale, factor.value_or(Tensor()), 3, out_dtype);
+  want("offsets", offsets, kI32, 1, &record);
+  want_shape("offsets", offsets, {codes.size(0) + 1});
+  TORCH_CHECK_VALUE(codes.size(0) <= kMaxExperts, "at most ", kMaxExperts, " experts, got ", codes.sizes());
+  return run_fp4_product(record, k, format, offsets, codes, scale, factor.value_or(Tensor()), out_dtype);
+}
+
+Tensor fp4_linear(const Tensor& x, const Tensor& codes, const Tensor& scale, const OptTensor& factor_arg,
+                  const OptDtype& out_dtype) {
+  const Tensor factor = factor_arg.value_or(Tensor());
+  want("x", x, kFloats, 2, nullptr, true);
+  const int64_t format = check_fp4_weight(codes, scale, factor, 2, &x), m = x.size(0), k = x.size(1), n = codes.size(0);
+  TORCH_CHECK_VALUE(2 * codes.size(1) == k, "the weights have ", 2 * codes.size(1), " columns, the rows ", k);
+  const ScalarType dtype = out_dtype.value_or(x.scalar_type());
+  check_out(dtype);
+  TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !x.requires_grad(), "4-bit products have no gradient");
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor out = empty({m, n}, dtype, x), ws;
+  if (m == 0) return out;
+  int64_t bytes = m * record_bytes(format, k);
+  if (x.scalar_type() != ScalarType::Float && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && x.stride(0) % 8 == 0)
+    bytes = int64_t(b200moe_fp4_linear_workspace_bytes(int(m), int(n), int(k), int(format)));
+  if (bytes) ws = empty({bytes}, ScalarType::Byte, x);
+  check("b200moe_fp4_linear",
+        b200moe_fp4_linear(stream(x), x.data_ptr(), code(x.scalar_type()), x.stride(0), codes.data_ptr(),
+                           scale.data_ptr(), f32(factor), int(m), int(n), int(k), int(format), out.data_ptr(), code(dtype),
+                           mut(ws), size_t(bytes)));
+  return out;
+}
+
+// ---------------------------------------------------------------------- norm
+bool is_f32(const Tensor& t) { return t.scalar_type() == ScalarType::Float; }
+
+void check_norm(const Tensor& x, const Tensor& weight, const Tensor& residual, double eps) {
+  want("x", x, kFloats, 2, nullptr, true);
+  const int64_t width = x.size(1);
+  TORCH_CHECK_VALUE(width >= 1 && width <= 16384, "x must have 1 to 16384 columns, got ", x.sizes());
+  want("weight", weight, kFloats, 1, &x);
+  want_shape("weight", weight, {width});
+  TORCH_CHECK_VALUE(weight.scalar_type() == x.scalar_type() || is_f32(weight), "weight must be ", x.scalar_type(),
+                    " or Float, got ", weight.scalar_type());
+  if (residual.defined()) {
+    want("residual", residual, kFloats, 2, &x, true);
+    want_shape("residual", residual, x.sizes());
+    TORCH_CHECK_VALUE(residual.scalar_type() == x.scalar_type() || is_f32(residual), "residual must be ",
+                      x.scalar_type(), " or Float, got ", residual.scalar_type());
+  }
+  TORCH_CHECK_VALUE(eps >= 1e-20 && eps <= 1e30, "eps must be from 1e-20 to 1e30, got ", eps);
+}
+
+struct NormOut {
+  Tensor q, scale, sum, y;  // undefined: not asked for
+};
+
+// out: 0 y alone, 1 E4M3, 2 + format records
+NormOut run_norm(const Tensor& x, const Tensor& weight, const Tensor& residual, double eps, int out, bool keep) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t rows = x.size(0), width = x.size(1);
+  NormOut o;
+  if (residual.defined()) o.sum = empty({rows, width}, residual.scalar_type(), x);
+  if (out == 0 || keep) o.y = empty({rows, width}, x.scalar_type(), x);
+  if (out == 1) {
+    o.q = empty({rows, width}, kE4m3, x);
+    o.scale = empty({rows, blocks(width)}, ScalarType::Float, x);
+  } else if (out > 1) {
+    o.q = empty({rows, record_bytes(out - 2, width)}, ScalarType::Byte, x);
+  }
+  if (rows)
+    check("b200moe_rms_norm",
+          b200moe_rms_norm(stream(x), x.data_ptr(), code(x.scalar_type()), x.stride(0), mut(residual),
+                           residual.defined() && is_f32(residual), residual.defined() ? residual.stride(0) : 0,
+                           weight.data_ptr(), is_f32(weight), float(eps), int(rows), int(width), mut(o.sum), mut(o.y), out,
+                           mut(o.q), f32_mut(o.scale)));
+  return o;
+}
+
+struct NormGrads {
+  Tensor x, residual, weight;
+};
+
+// s: the stored sum (or x); grad_y of dtype; grad_s of s's type or undefined.
+NormGrads run_norm_grad(const Tensor& s, const Tensor& grad_y, const Tensor& grad_s, const Tensor& weight, double eps,
+                        bool need_x, bool need_residual, bool need_weight) {
+  const c10::cuda::CUDAGuard guard(s.device());
+  const int64_t rows = s.size(0), width = s.size(1);
+  const ScalarType dtype = grad_y.scalar_type();
+  const bool one = dtype == s.scalar_type();  // both inputs' gradients have the same values and type
+  NormGrads g;
+  Tensor ws;
+  if (need_x || (one && need_residual)) g.x = empty({rows, width}, dtype, s);
+  if (!one && need_residual) g.residual = empty({rows, width}, s.scalar_type(), s);
+  if (need_weight) g.weight = empty({width}, weight.scalar_type(), s);
+  const int64_t bytes = need_weight && rows ? int64_t(b200moe_rms_norm_grad_workspace_bytes(int(rows), int(width))) : 0;
+  if (bytes) ws = empty({bytes}, ScalarType::Byte, s);
+  if (rows == 0) {
+    if (need_weight) g.weight.zero_();
+  } else if (need_x || need_residual || need_weight) {
+    check("b200moe_rms_norm_grad",
+          b200moe_rms_norm_grad(stream(s), s.data_ptr(), is_f32(s), s.stride(0), grad_y.data_ptr(), code(dtype),
+                                grad_y.stride(0), mut(grad_s), grad_s.defined() ? grad_s.stride(0) : 0, weight.data_ptr(),
+                                is_f32(weight), float(eps), int(rows), int(width), mut(g.x), mut(g.residual),
+                                mut(g.weight), mut(ws), size_t(bytes)));
+  }
+  if (one && need_residual) g.residual = g.x;
+  if (!need_x) g.x = Tensor();
+  return g;
+}
+
+struct RmsNormFn : torch::autograd::Function<RmsNormFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& residual,
+                               double eps) {
+    const NormOut o = run_norm(x, weight, residual.value_or(Tensor()), eps, 0, false);
+    ctx->save_for_backward({o.sum.defined() ? o.sum : x, weight});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["dtype"] = int64_t(x.scalar_type());
+    ctx->set_materialize_grads(false);
+    return o.sum.defined() ? variable_list{o.y, o.sum} : variable_list{o.y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    for (const Tensor& g : grads) once_differentiable(g);
+    const bool added = grads.size() == 2;
+    const Tensor grad_s = added && grads[1].defined() ? as_rows(grads[1]) : Tensor();
+    if (!grads[0].defined() && !grad_s.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    const Tensor& s = saved[0];
+    const auto dtype = ScalarType(ctx->saved_data["dtype"].toInt());
+    const Tensor grad_y = grads[0].defined() ? as_rows(grads[0]) : at::zeros(s.sizes(), s.options().dtype(dtype));
+    const NormGrads g = run_norm_grad(s, grad_y, grad_s, saved[1], ctx->saved_data["eps"].toDouble(),
+                                      ctx->needs_input_grad(0), added && ctx->needs_input_grad(2), ctx->needs_input_grad(1));
+    return {g.x, g.weight, g.residual, Tensor()};
+  }
+};
+
+std::tuple<Tensor, OptTensor> rms_norm(const Tensor& x, const Tensor& weight, const OptTensor& residual_arg, double eps) {
+  const Tensor residual = residual_arg.value_or(Tensor());
+  check_norm(x, weight, residual, eps);
+  if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || differentiable(residual))) {
+    const variable_list out = RmsNormFn::apply(x, weight, residual_arg, eps);
+    return {out[0], out.size() == 2 ? OptTensor(out[1]) : std::nullopt};
+  }
+  const NormOut o = run_norm(x, weight, residual, eps, 0, false);
+  return {o.y, o.sum.defined() ? OptTensor(o.sum) : std::nullopt};
+}
+
+using OptTensors = std::tuple<Tensor, OptTensor, OptTensor, OptTensor>;
+OptTensors rms_norm_quantize(const Tensor& x, const Tensor& weight, const OptTensor& residual_arg, double eps, int64_t out,
+                             bool keep) {
+  const Tensor residual = residual_arg.value_or(Tensor());
+  check_norm(x, weight, residual, eps);
+  TORCH_CHECK_VALUE(out >= 1 && out <= 3, "unknown format ", out);
+  if (out > 1) record_bytes(out - 2, x.size(1));
+  TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(x.requires_grad() || weight.requires_grad() || differentiable(residual)),
+                    "quantized rows have no gradient: use rms_norm");
+  const NormOut o = run_norm(x, weight, residual, eps, int(out), keep);
+  auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; };
+  return {o.q, opt(o.scale), opt(o.sum), opt(o.y)};
+}
+
+std::tuple<OptTensor, OptTensor, OptTensor> rms_norm_grad(const Tensor& s, const Tensor& grad_y, const OptTensor& grad_s_arg,
+                                                          const Tensor& weight, double eps, bool need_x, bool need_residual,
+                                                          bool need_weight) {
+  const Tensor grad_s = grad_s_arg.value_or(Tensor());
+  want("grad_y", grad_y, kFloats, 2, nullptr, true);
+  check_norm(grad_y, weight, s, eps);
+  if (grad_s.defined()) {
+    want("grad_s", grad_s, kFloats, 2, &s, true);
+    want_shape("grad_s", grad_s, s.sizes());
+    TORCH_CHECK_VALUE(grad_s.scalar_type() == s.scalar_type(), "grad_s must be ", s.scalar_type(), ", got ",
+                      grad_s.scalar_type());
+  }
+  const NormGrads g = run_norm_grad(s, grad_y, grad_s, weight, eps, need_x, need_residual, need_weight);
+  auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; };
+  return {opt(g.x), opt(g.residual), opt(g.weight)};
+}
+
 PyObject* g_error_class = nullptr;  // b200moe._lib.B200MoeError
 
 }  // namespace
@@ -526,4 +846,17 @@ PYBIND11_MODULE(b200moe_ops, m) {
   m.def("matmul", &matmul);
   m.def("grouped_matmul", &grouped_matmul);
   m.def("linear", &linear);
+  m.def("fp4_quantize", &fp4_quantize);
+  m.def("fp4_swiglu_quantize", &fp4_swiglu_quantize);
+  m.def("fp4_quantize_weight", &fp4_quantize_weight);
+  m.def("fp4_weight_format", &fp4_weight_format);
+  m.def("fp4_rows_values", &fp4_rows_values);
+  m.def("fp4_weight_values", &fp4_weight_values);
+  m.def("fp4_matmul", &fp4_matmul);
+  m.def("fp4_grouped_matmul", &fp4_grouped_matmul);
+  m.def("fp4_linear", &fp4_linear);
+  m.def("check_records", &check_records);
+  m.def("rms_norm", &rms_norm);
+  m.def("rms_norm_quantize", &rms_norm_quantize);
+  m.def("rms_norm_grad", &rms_norm_grad);
 }

@@ -1,0 +1,286 @@
+// Rows and weights to 4-bit floating point (fp4_rows.cuh), the limited SwiGLU
+// fused in front of the rows' quantizer, and the values that records stand for.
+//
+// A thread holds 16 columns.  NVFP4 needs the row's maximum before its first
+// code: a CTA (up to 512 columns a warp) holds a row in registers, so that it is
+// read once; longer rows than a CTA holds are read twice.  MXFP4's blocks stand
+// alone and take two threads each, whatever their row.
+// Bound: HBM for rows as they are, instruction issue for the SwiGLU.
+#include <algorithm>
+
+#include "fp4_rows.cuh"
+#include "internal.h"
+
+namespace b200moe {
+namespace {
+
+constexpr int kMaxRowThreads = 512;
+
+// 16 columns from c of a row (SWIGLU: of its product with the row's second half).
+template <typename T, bool SWIGLU, bool WIDE>
+__device__ __forceinline__ void load16(const T* row, int c, int width, float limit, float (&v)[16]) {
+  Vec<T, 16> a, b;
+  if constexpr (WIDE) {
+    a.load(row + c);
+    if constexpr (SWIGLU) b.load(row + width + c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      a.v[i] = row[c + i];
+      if constexpr (SWIGLU) b.v[i] = row[width + c + i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    v[i] = a.get(i);
+    if constexpr (SWIGLU) v[i] = swiglu(v[i], b.get(i), limit);
+  }
+}
+
+// A row per CTA, or per warp (blockDim.x / 32 of them) where per_warp is set.
+template <typename T, bool SWIGLU, bool WIDE>
+__global__ void __launch_bounds__(kMaxRowThreads) nvfp4_rows_kernel(const T* __restrict__ x, int64_t x_stride, int rows,
+                                                                    int width, float limit, int per_warp,
+                                                                    uint8_t* __restrict__ out) {
+  __shared__ uint32_t warp_max[kMaxRowThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = per_warp ? int64_t(blockIdx.x) * (blockDim.x / 32) + warp : blockIdx.x;
+  const int tid = per_warp ? lane : threadIdx.x, threads = per_warp ? 32 : blockDim.x;
+  pdl_wait();
+  pdl_trigger();
+  if (row >= rows) return;  // whole warps, and only where no barrier follows
+  const T* src = x + row * x_stride;
+  const int pieces = width / 16;
+  const bool once = pieces <= threads;  // the row stays in registers
+  float v[16];
+  uint32_t m = 0;
+  for (int p = tid; p < pieces; p += threads) {
+    load16<T, SWIGLU, WIDE>(src, p * 16, width, limit, v);
+    m = max(m, abs_bits(magnitude16(v)));
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (!per_warp) {
+    if (lane == 0) warp_max[warp] = m;
+    __syncthreads();
+    for (int i = 0; i < int(blockDim.x / 32); ++i) m = max(m, warp_max[i]);
+  }
+  const float factor = nvfp4_factor(m);
+  uint8_t* rec = out + row * fp4_stride(kNv, width);
+  for (int p = tid; p < pieces; p += threads) {
+    if (!once) load16<T, SWIGLU, WIDE>(src, p * 16, width, limit, v);
+    float unit;
+    const uint32_t s = nvfp4_scale(magnitude16(v), factor, unit);
+    *reinterpret_cast<uint2*>(rec + p * 8) = nvfp4_codes(v, unit);
+    rec[width / 2 + p] = uint8_t(s);
+  }
+  if (tid == 0) finish_record(rec, kNv, width, factor);
+}
+
+// Two neighbouring threads per block of 32 columns of any row.
+template <typename T, bool SWIGLU, bool WIDE>
+__global__ void __launch_bounds__(256) mxfp4_rows_kernel(const T* __restrict__ x, int64_t x_stride, int rows, int width,
+                                                         float limit, uint8_t* __restrict__ out) {
+  const int pieces = width / 16, stride = fp4_stride(kMx, width);
+  const int64_t total = int64_t(rows) * pieces, step = int64_t(gridDim.x) * blockDim.x;
+  pdl_wait();
+  pdl_trigger();
+  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; __any_sync(0xffffffffu, i < total); i += step) {
+    const bool in = i < total;  // the same for both threads of a block: pieces is even
+    const int64_t row = in ? (i <= INT32_MAX ? int64_t(uint32_t(i) / uint32_t(pieces)) : i / pieces) : 0;
+    const int p = in ? int(i - row * pieces) : 0;
+    float v[16], inv;
+    if (in) load16<T, SWIGLU, WIDE>(x + row * x_stride, p * 16, width, limit, v);
+    float m = in ? magnitude16(v) : 0.f;
+    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    if (!in) continue;
+    const uint32_t s = mxfp4_scale(m, inv);
+    uint8_t* rec = out + row * stride;
+    *reinterpret_cast<uint2*>(rec + p * 8) = mxfp4_codes(v, inv);
+    if (!(p & 1)) rec[width / 2 + p / 2] = uint8_t(s);
+    if (p == pieces - 1) finish_record(rec, kMx, width, 1.f);
+  }
+}
+
+// ------------------------------------------------------------------ weights
+// Largest magnitude of each matrix, as bits, into its factor's place (zero before).
+template <typename T>
+__global__ void __launch_bounds__(256) fp4_weight_max_kernel(const T* __restrict__ w, int64_t n, uint32_t* __restrict__ top) {
+  const T* src = w + int64_t(blockIdx.y) * n;
+  uint32_t m = 0;
+  pdl_wait();
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256)
+    m = max(m, abs_bits(to_f32(src[i])));
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0 && m) atomicMax(top + blockIdx.y, m);  // a maximum: any order gives the same
+  pdl_trigger();
+}
+__global__ void fp4_weight_factor_kernel(uint32_t* top, int mats) {
+  pdl_wait();
+  for (int i = threadIdx.x; i < mats; i += blockDim.x) top[i] = __float_as_uint(nvfp4_factor(top[i]));
+  pdl_trigger();
+}
+
+// A thread per 16 columns of any matrix; codes and scales in arrays of their own.
+template <typename T, int FMT>
+__global__ void __launch_bounds__(256) fp4_weight_kernel(const T* __restrict__ w, int64_t per_mat, int64_t total,
+                                                         const float* __restrict__ factor, uint8_t* __restrict__ codes,
+                                                         uint8_t* __restrict__ scale) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t step = int64_t(gridDim.x) * 256;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; __any_sync(0xffffffffu, i < total); i += step) {
+    const bool in = i < total;
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = in ? to_f32(w[i * 16 + j]) : 0.f;
+    float m = magnitude16(v);
+    if constexpr (FMT == kMx) {
+      float inv;
+      m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      if (!in) continue;
+      const uint32_t s = mxfp4_scale(m, inv);
+      reinterpret_cast<uint2*>(codes)[i] = mxfp4_codes(v, inv);
+      if (!(i & 1)) scale[i / 2] = uint8_t(s);
+    } else {
+      if (!in) continue;
+      float unit;
+      scale[i] = uint8_t(nvfp4_scale(m, factor[i / per_mat], unit));
+      reinterpret_cast<uint2*>(codes)[i] = nvfp4_codes(v, unit);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- read back
+// A thread per 16 columns: value * scale * factor, rounded once.
+template <typename T, int FMT>
+__global__ void __launch_bounds__(256) fp4_values_kernel(const uint8_t* __restrict__ codes, int64_t ld_codes,
+                                                         const uint8_t* __restrict__ scale, int64_t ld_scale,
+                                                         const uint8_t* __restrict__ factor, int64_t ld_factor,
+                                                         int64_t rows, int width, T* __restrict__ out) {
+  const int pieces = width / 16;
+  const int64_t total = rows * pieces, step = int64_t(gridDim.x) * 256;
+  pdl_wait();
+  pdl_trigger();
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += step) {
+    const int64_t row = i <= INT32_MAX ? int64_t(uint32_t(i) / uint32_t(pieces)) : i / pieces;
+    const int p = int(i - row * pieces);
+    const uint2 c = *reinterpret_cast<const uint2*>(codes + row * ld_codes + p * 8);
+    const uint32_t sb = scale[row * ld_scale + (FMT == kMx ? p / 2 : p)];
+    const float s = FMT == kMx ? e8m0_f32(sb) : e4m3_f32(sb);
+    const float f = factor ? *reinterpret_cast<const float*>(factor + row * ld_factor) : 1.f;
+    float v[16];
+    float(&lo)[8] = *reinterpret_cast<float(*)[8]>(v);
+    float(&hi)[8] = *reinterpret_cast<float(*)[8]>(v + 8);
+    e2m1x8_values(c.x, s, lo);
+    e2m1x8_values(c.y, s, hi);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] *= f;
+    store_vec<T, 16>(out + i * 16, v);
+  }
+}
+
+int status(cudaError_t e) {
+  if (e == cudaSuccess) return B200MOE_OK;
+  cudaGetLastError();
+  return B200MOE_ERR_CUDA;
+}
+
+bool on(const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+unsigned grid_of(int64_t threads) { return unsigned(std::min<int64_t>((threads + 255) / 256, int64_t(sm_count()) * 32)); }
+
+template <typename T, bool SWIGLU>
+cudaError_t run_rows(cudaStream_t s, int fmt, const void* x, int64_t x_stride, int rows, int width, float limit,
+                     uint8_t* out) {
+  const bool wide = on(x, 16) && x_stride * int64_t(sizeof(T)) % 16 == 0;
+  const T* src = static_cast<const T*>(x);
+  if (fmt == kMx) {
+    auto kernel = wide ? mxfp4_rows_kernel<T, SWIGLU, true> : mxfp4_rows_kernel<T, SWIGLU, false>;
+    return launch_chain(kernel, dim3(grid_of(int64_t(rows) * (width / 16))), dim3(256), 0, s, src, x_stride, rows, width,
+                        limit, out);
+  }
+  const int pieces = width / 16, per_warp = pieces <= 32;
+  const int threads = per_warp ? 256 : std::min(kMaxRowThreads, (pieces + 31) / 32 * 32);
+  const int64_t grid = per_warp ? (int64_t(rows) + 7) / 8 : rows;
+  auto kernel = wide ? nvfp4_rows_kernel<T, SWIGLU, true> : nvfp4_rows_kernel<T, SWIGLU, false>;
+  return launch_chain(kernel, dim3(unsigned(grid)), dim3(threads), 0, s, src, x_stride, rows, width, limit, per_warp, out);
+}
+
+template <typename T>
+cudaError_t run_weight(cudaStream_t s, int fmt, const void* w, int mats, int64_t n, uint8_t* codes, uint8_t* scale,
+                       float* factor) {
+  const T* src = static_cast<const T*>(w);
+  const int64_t total = mats * (n / 16);
+  if (fmt == kMx)
+    return launch_chain(fp4_weight_kernel<T, kMx>, dim3(grid_of(total)), dim3(256), 0, s, src, n / 16, total,
+                        static_cast<const float*>(nullptr), codes, scale);
+  cudaError_t e = cudaMemsetAsync(factor, 0, mats * sizeof(float), s);
+  uint32_t* top = reinterpret_cast<uint32_t*>(factor);
+  const unsigned per = unsigned(std::min<int64_t>((n + 4095) / 4096, std::max(1, sm_count() * 8 / mats)));
+  if (e == cudaSuccess)
+    e = launch_chain(fp4_weight_max_kernel<T>, dim3(per, mats), dim3(256), 0, s, src, n, top);
+  if (e == cudaSuccess) e = launch_chain(fp4_weight_factor_kernel, dim3(1), dim3(256), 0, s, top, mats);
+  if (e == cudaSuccess)
+    e = launch_chain(fp4_weight_kernel<T, kNv>, dim3(grid_of(total)), dim3(256), 0, s, src, n / 16, total,
+                     static_cast<const float*>(factor), codes, scale);
+  return e;
+}
+
+template <typename T>
+cudaError_t run_values(cudaStream_t s, int fmt, const uint8_t* codes, int64_t ld_codes, const uint8_t* scale,
+                       int64_t ld_scale, const uint8_t* factor, int64_t ld_factor, int64_t rows, int width, void* out) {
+  auto kernel = fmt == kMx ? fp4_values_kernel<T, kMx> : fp4_values_kernel<T, kNv>;
+  return launch_chain(kernel, dim3(grid_of(rows * (width / 16))), dim3(256), 0, s, codes, ld_codes, scale, ld_scale,
+                      factor, ld_factor, rows, width, static_cast<T*>(out));
+}
+
+bool bad_format(int fmt) { return fmt != kNv && fmt != kMx; }
+
+}  // namespace
+}  // namespace b200moe
+
+using namespace b200moe;
+
+extern "C" int b200moe_fp4_record_bytes(int format, int k) {
+  return bad_format(format) || k < 32 || k % 32 || k > (1 << 28) ? 0 : fp4_stride(format, k);
+}
+
+extern "C" int b200moe_fp4_quantize(void* stream, const void* x, int dtype, int64_t x_stride, int rows, int k, int format,
+                                    int swiglu, float limit, void* records) {
+  if (!x || !records || rows < 1 || !b200moe_fp4_record_bytes(format, k) || x_stride < 0 || !(limit > 0.f))
+    return B200MOE_ERR_INVALID_ARG;
+  if (dtype < 0 || dtype > B200MOE_F32) return B200MOE_ERR_DTYPE;
+  if (!on(records, 16)) return B200MOE_ERR_ALIGN;
+  auto run = dtype == B200MOE_F16    ? (swiglu ? run_rows<__half, true> : run_rows<__half, false>)
+             : dtype == B200MOE_BF16 ? (swiglu ? run_rows<__nv_bfloat16, true> : run_rows<__nv_bfloat16, false>)
+                                     : (swiglu ? run_rows<float, true> : run_rows<float, false>);
+  return status(run(static_cast<cudaStream_t>(stream), format, x, x_stride, rows, k, limit, static_cast<uint8_t*>(records)));
+}
+
+extern "C" int b200moe_fp4_quantize_weight(void* stream, const void* w, int dtype, int mats, int n, int k, int format,
+                                           void* codes, void* scale, float* factor) {
+  if (!w || !codes || !scale || mats < 1 || mats > 65535 || n < 1 || !b200moe_fp4_record_bytes(format, k) ||
+      (format == kNv && !factor))
+    return B200MOE_ERR_INVALID_ARG;
+  if (dtype < 0 || dtype > B200MOE_F32) return B200MOE_ERR_DTYPE;
+  if (!on(codes, 16)) return B200MOE_ERR_ALIGN;
+  auto run = dtype == B200MOE_F16 ? run_weight<__half> : dtype == B200MOE_BF16 ? run_weight<__nv_bfloat16>
+                                                                               : run_weight<float>;
+  return status(run(static_cast<cudaStream_t>(stream), format, w, mats, int64_t(n) * k, static_cast<uint8_t*>(codes),
+                    static_cast<uint8_t*>(scale), factor));
+}
+
+extern "C" int b200moe_fp4_values(void* stream, const void* codes, int64_t ld_codes, const void* scale, int64_t ld_scale,
+                                  const void* factor, int64_t ld_factor, int64_t rows, int k, int format, void* out,
+                                  int dtype) {
+  if (!codes || !scale || !out || rows < 1 || !b200moe_fp4_record_bytes(format, k) || ld_codes < 0 || ld_scale < 0 ||
+      ld_factor < 0)
+    return B200MOE_ERR_INVALID_ARG;
+  if (dtype < 0 || dtype > B200MOE_F32) return B200MOE_ERR_DTYPE;
+  if (!on(codes, 8) || ld_codes % 8 || !on(factor, 4) || ld_factor % 4 || !on(out, 16)) return B200MOE_ERR_ALIGN;
+  auto run = dtype == B200MOE_F16 ? run_values<__half> : dtype == B200MOE_BF16 ? run_values<__nv_bfloat16>
+                                                                               : run_values<float>;
+  return status(run(static_cast<cudaStream_t>(stream), format, static_cast<const uint8_t*>(codes), ld_codes,
+                    static_cast<const uint8_t*>(scale), ld_scale, static_cast<const uint8_t*>(factor), ld_factor, rows, k,
+                    out));
+}

@@ -16,6 +16,7 @@
 
 #include "fp8_device.cuh"
 #include "internal.h"
+#include "swiglu.cuh"
 
 namespace b200moe {
 namespace {
@@ -25,29 +26,6 @@ constexpr int kQuantBlocks = kQuantThreads / 8;  // row blocks of a CTA's turn
 // CTAs at most, for walks of several turns: SwiGLU of 49152 x 1408 takes 97 us with 16 per SM, 102 with 8 and 99
 // without a cap, its gradient 113 us with 48 per SM, 128 without a cap and 116 with 16 (115 now, its steps fixed since)
 constexpr int64_t kCtaCap = 148 * 16, kGradCap = 148 * 48, kAnyCap = 148 * 32;
-
-// Minimum / maximum that keep a NaN.
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float o;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(o) : "f"(a), "f"(b));
-  return o;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float o;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(o) : "f"(a), "f"(b));
-  return o;
-}
-
-// The limited gate: min(gate, limit), and a finite value for -inf: from -89 down e^-g is infinite in f32 and the SwiGLU
-// and its gradient are 0, where -inf itself would give NaN.
-__device__ __forceinline__ float limited_gate(float gate, float limit) { return max_nan(min_nan(gate, limit), -128.f); }
-__device__ __forceinline__ float limited_up(float up, float limit) { return max_nan(min_nan(up, limit), -limit); }
-
-// Limited SwiGLU (the framework's): g = min(gate, limit), u = clamp(up, +-limit), g / (1 + e^-g) * u.
-__device__ __forceinline__ float swiglu(float gate, float up, float limit) {
-  const float g = limited_gate(gate, limit);
-  return __fdiv_rn(g, 1.f + expf(-g)) * limited_up(up, limit);
-}
 
 // Position (row, block) of a walk over rows x blocks in steps of d_row rows and d_b blocks: one division at its start.
 struct Walk {

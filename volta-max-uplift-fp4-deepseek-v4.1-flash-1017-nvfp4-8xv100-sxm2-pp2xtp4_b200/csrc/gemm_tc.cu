@@ -545,12 +545,14 @@ static int launch_tc_one(cudaStream_t s, const TcArgs& a, const void* map, int g
              : -1;
 }
 
-int make_u8_tile_map(void* map_out, const void* base, int64_t rows, int64_t row_bytes, int box_bytes, int box_rows) {
+int make_u8_tile_map(void* map_out, const void* base, int64_t rows, int64_t row_bytes, int box_bytes, int box_rows,
+                     int64_t stride) {
   auto fn = encode_fn();
-  if (!fn || row_bytes % 16 || box_bytes > 128 || (reinterpret_cast<uintptr_t>(base) & 15)) return -1;
+  if (stride == 0) stride = row_bytes;
+  if (!fn || row_bytes % 16 || stride % 16 || box_bytes > 128 || (reinterpret_cast<uintptr_t>(base) & 15)) return -1;
   CUtensorMap* m = static_cast<CUtensorMap*>(map_out);
   cuuint64_t dims[2] = {cuuint64_t(row_bytes), cuuint64_t(rows)};
-  cuuint64_t strides[1] = {cuuint64_t(row_bytes)};
+  cuuint64_t strides[1] = {cuuint64_t(stride)};
   cuuint32_t box[2] = {cuuint32_t(box_bytes), cuuint32_t(box_rows)};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,

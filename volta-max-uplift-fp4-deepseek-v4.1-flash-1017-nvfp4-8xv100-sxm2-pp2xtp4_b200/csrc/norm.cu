@@ -1,0 +1,535 @@
+// Root-mean-square norm of rows after the residual's addition, with the rows
+// quantized for the product that follows or as they are, and its gradient:
+//
+//   s = round(x + r)    rstd = 1 / sqrt(mean(s^2) + eps)    y = (s rstd) w
+//   ds = rstd (g - u mean(g u)) + (the sum's own gradient),  g = w dy, u = s rstd
+//   dw = sum over rows of dy u
+//
+// s is rounded to the residual's type once, as it is stored, and the norm is that
+// of the stored sum, so the gradient that reads it again is the same function's.
+// Sums run in f32.  Where a row's squares pass f32's range the row is scaled by
+// 2^-100 first (both are uniform branches that ordinary rows do not take).
+//
+// Forward: a CTA per row (a warp up to 512 columns), 16 columns a thread, the row
+// kept in registers between its sum and its outputs, so every byte moves once.
+// The quantizers take y in f32: 128 columns' maximum for E4M3, the row's for
+// NVFP4 (a second sum over the CTA), 32 columns' for MXFP4.
+// Backward: a CTA walks rows (rows apart by the grid), holds its columns' part of
+// dw in registers, and loads the next row before it works on this one; the parts
+// are joined by a second launch in a fixed order, so equal inputs give equal bits.
+// Bound: HBM both ways.
+#include <algorithm>
+
+#include "fp4_rows.cuh"
+#include "internal.h"
+
+namespace b200moe {
+namespace {
+
+constexpr int kMaxThreads = 512;
+constexpr int kMaxWidth = kMaxThreads * 16 * 2;
+enum Out { kRows = 0, kFp8 = 1, kNvOut = 2, kMxOut = 3 };
+
+// Column i of a thread's 16: WIDE (a width of whole eights), consecutive ones; else single ones 32 apart, so that a
+// warp's access is one run of bytes.  The order of a row's sums goes by its width alone: whether WIDE columns move as
+// vectors (vec, where every address allows it) changes no bit.
+template <bool WIDE>
+__device__ __forceinline__ int column(int base, int lane, int i) {
+  return WIDE ? base + lane * 16 + i : base + lane + 32 * i;
+}
+
+// The thread's 16 values of a row of T from the warp's first column; zeros past the width.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load_raw(const T* row, int base, int lane, int width, int vec, Vec<T, 8> (&v)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (WIDE) {
+      const int c = base + lane * 16 + 8 * h;
+      if (c < width && vec) {
+        v[h].load(row + c);
+      } else if (c < width) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[h].v[i] = row[c + i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[h].v[i] = from_f32<T>(0.f);
+      }
+    } else {
+      load_columns<false>(v[h], row, base + lane + 256 * h, 32, width);
+    }
+  }
+}
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load_row(const T* row, int base, int lane, int width, int vec, float (&v)[16]) {
+  Vec<T, 8> r[2];
+  load_raw<T, WIDE>(row, base, lane, width, vec, r);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = r[i / 8].get(i % 8);
+}
+template <typename T, bool WIDE>
+__device__ __forceinline__ void store_row(T* row, int base, int lane, int width, int vec, const float (&v)[16]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float(&part)[8] = *reinterpret_cast<const float(*)[8]>(v + 8 * h);
+    if constexpr (WIDE) {
+      const int c = base + lane * 16 + 8 * h;
+      if (c < width && vec) {
+        store_vec<T, 8>(row + c, part);
+      } else if (c < width) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) row[c + i] = from_f32<T>(part[i]);
+      }
+    } else {
+      store_columns<false>(row, base + lane + 256 * h, 32, width, part);
+    }
+  }
+}
+// The same for a tensor of T or, where f32 is set, of float.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load_either(const void* p, int f32, int64_t offset, int base, int lane, int width,
+                                            int vec, float (&v)[16]) {
+  if (sizeof(T) == 4 || f32)
+    load_row<float, WIDE>(static_cast<const float*>(p) + offset, base, lane, width, vec, v);
+  else
+    load_row<T, WIDE>(static_cast<const T*>(p) + offset, base, lane, width, vec, v);
+}
+template <typename T, bool WIDE>
+__device__ __forceinline__ void store_either(void* p, int f32, int64_t offset, int base, int lane, int width,
+                                             int vec, const float (&v)[16]) {
+  if (sizeof(T) == 4 || f32)
+    store_row<float, WIDE>(static_cast<float*>(p) + offset, base, lane, width, vec, v);
+  else
+    store_row<T, WIDE>(static_cast<T*>(p) + offset, base, lane, width, vec, v);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+// The sum over the row's threads, the same bits in each; red: a place of kMaxThreads / 32 floats that no sum before used
+// since the last barrier.
+__device__ __forceinline__ float row_sum(float v, int per_warp, float* red) {
+  v = warp_sum(v);
+  if (per_warp) return v;
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.f;
+  for (int i = 0; i < int(blockDim.x / 32); ++i) v += red[i];
+  return v;
+}
+
+// What a row is scaled by before its squares are taken, and 1 / sqrt of their mean and eps.
+struct Rms {
+  float k, rstd;
+};
+constexpr float kFar = 0x1p-100f;
+
+struct NormArgs {
+  const void* x;
+  int64_t x_stride;
+  const void* residual;  // null: none
+  int64_t r_stride;
+  int r_f32;  // residual and sum are f32
+  const void* weight;
+  int w_f32;
+  float eps;
+  int rows, width, per_warp;
+  int vec;  // every address on 16 bytes
+  void* sum;         // [rows][width], with a residual
+  void* y;           // [rows][width] of x's type, or null
+  uint8_t* q;        // E4M3 [rows][width], or records
+  float* scale;      // E4M3: [rows][ceil(width / 128)]
+};
+
+template <typename T, int OUT, bool WIDE, int C>
+__global__ void __launch_bounds__(kMaxThreads, C == 1 ? 2 : 1) norm_kernel(const NormArgs a) {
+  __shared__ float red[3][kMaxThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = a.per_warp ? int64_t(blockIdx.x) * (blockDim.x / 32) + warp : blockIdx.x;
+  const int warps = a.per_warp ? 1 : blockDim.x / 32, first = a.per_warp ? 0 : warp;
+  pdl_wait();
+  pdl_trigger();
+  if (row >= a.rows) return;  // whole warps, and only where no barrier follows
+  float v[C][16];
+  float ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int base = (c * warps + first) * 512;
+    load_row<T, WIDE>(static_cast<const T*>(a.x) + row * a.x_stride, base, lane, a.width, a.vec, v[c]);
+    if (a.residual) {
+      float r[16];
+      load_either<T, WIDE>(a.residual, a.r_f32, row * a.r_stride, base, lane, a.width, a.vec, r);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        v[c][i] += r[i];
+        if (sizeof(T) == 2 && !a.r_f32) v[c][i] = to_f32(from_f32<T>(v[c][i]));
+      }
+      store_either<T, WIDE>(a.sum, a.r_f32, row * a.width, base, lane, a.width, a.vec, v[c]);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ss = fmaf(v[c][i], v[c][i], ss);
+  }
+  ss = row_sum(ss, a.per_warp, red[0]);
+  Rms n{1.f, 0.f};
+  if (!(ss < INFINITY)) {  // too large for f32, or not finite
+    n.k = kFar;
+    ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ss = fmaf(v[c][i] * kFar, v[c][i] * kFar, ss);
+    ss = row_sum(ss, a.per_warp, red[1]);
+  }
+  n.rstd = __frsqrt_rn(__fdiv_rn(ss, float(a.width)) + (n.k == 1.f ? a.eps : 0.f));
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int base = (c * warps + first) * 512;
+    float w[16];
+    load_either<T, WIDE>(a.weight, a.w_f32, 0, base, lane, a.width, a.vec, w);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[c][i] = v[c][i] * n.k * n.rstd * w[i];
+    if (a.y) store_row<T, WIDE>(static_cast<T*>(a.y) + row * a.width, base, lane, a.width, a.vec, v[c]);
+    if constexpr (OUT == kNvOut) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (column<WIDE>(base, lane, i) < a.width) top = max(top, abs_bits(v[c][i]));
+    }
+  }
+  if constexpr (OUT == kFp8) {
+    const int nb = (a.width + kFp8Block - 1) / kFp8Block;
+    uint8_t* q = a.q + row * a.width;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int base = (c * warps + first) * 512;
+      if constexpr (WIDE) {  // eight lanes hold a block
+        float m = magnitude16(v[c]);
+#pragma unroll
+        for (int d = 4; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+        const Fp8Scale s = fp8_scale(abs_bits(m));
+        const int col = base + lane * 16;
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          o[j] = e4m3x4(v[c][4 * j] * s.inv, v[c][4 * j + 1] * s.inv, v[c][4 * j + 2] * s.inv, v[c][4 * j + 3] * s.inv);
+        if (col < a.width) *reinterpret_cast<uint2*>(q + col) = make_uint2(o[0], o[1]);
+        if (col + 8 < a.width) *reinterpret_cast<uint2*>(q + col + 8) = make_uint2(o[2], o[3]);
+        if ((lane & 7) == 0 && col < a.width) a.scale[row * nb + col / kFp8Block] = s.scale;
+      } else {  // a warp's four columns of each lane are a block
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          uint32_t m = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) m = max(m, abs_bits(v[c][4 * b + i]));
+          const Fp8Scale s = fp8_scale(__reduce_max_sync(0xffffffffu, m));
+          const uint32_t o = e4m3x4(v[c][4 * b] * s.inv, v[c][4 * b + 1] * s.inv, v[c][4 * b + 2] * s.inv,
+                                    v[c][4 * b + 3] * s.inv);
+          const int col = base + 128 * b + lane;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (col + 32 * i < a.width) q[col + 32 * i] = uint8_t(o >> (8 * i));
+          if (lane == 0 && col < a.width) a.scale[row * nb + col / kFp8Block] = s.scale;
+        }
+      }
+    }
+  }
+  if constexpr (OUT == kNvOut) {
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (!a.per_warp) {
+      uint32_t* tops = reinterpret_cast<uint32_t*>(red[2]);
+      if (lane == 0) tops[warp] = top;
+      __syncthreads();
+      for (int i = 0; i < warps; ++i) top = max(top, tops[i]);
+    }
+    const float factor = nvfp4_factor(top);
+    uint8_t* rec = a.q + row * fp4_stride(kNv, a.width);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = (c * warps + first) * 512 + lane * 16;
+      if (col >= a.width) continue;
+      float unit;
+      const uint32_t s = nvfp4_scale(magnitude16(v[c]), factor, unit);
+      *reinterpret_cast<uint2*>(rec + col / 2) = nvfp4_codes(v[c], unit);
+      rec[a.width / 2 + col / 16] = uint8_t(s);
+    }
+    if (first == 0 && lane == 0) finish_record(rec, kNv, a.width, factor);
+  }
+  if constexpr (OUT == kMxOut) {
+    uint8_t* rec = a.q + row * fp4_stride(kMx, a.width);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = (c * warps + first) * 512 + lane * 16;
+      float m = magnitude16(v[c]), inv;
+      m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      if (col >= a.width) continue;
+      const uint32_t s = mxfp4_scale(m, inv);
+      *reinterpret_cast<uint2*>(rec + col / 2) = mxfp4_codes(v[c], inv);
+      if (!(lane & 1)) rec[a.width / 2 + col / 32] = uint8_t(s);
+    }
+    if (first == 0 && lane == 0) finish_record(rec, kMx, a.width, 1.f);
+  }
+}
+
+// ----------------------------------------------------------------- gradient
+struct GradArgs {
+  const void* s;  // the stored sum (or x), f32 where s_f32
+  int64_t s_stride;
+  int s_f32;
+  const void* dy;  // T
+  int64_t dy_stride;
+  const void* ds;  // the sum's own gradient, of the sum's type, or null
+  int64_t ds_stride;
+  const void* weight;
+  int w_f32;
+  float eps;
+  int rows, width, per_warp;
+  int vec;  // every address on 16 bytes
+  void* grad_x;    // T, or null
+  void* grad_sum;  // the sum's type, or null
+  float* parts;    // [slots][width], or null
+};
+
+template <typename T, bool WIDE, int C>
+__global__ void __launch_bounds__(kMaxThreads, 1) norm_grad_kernel(const GradArgs a) {
+  __shared__ float red[4][kMaxThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int warps = a.per_warp ? 1 : blockDim.x / 32, first = a.per_warp ? 0 : warp;
+  const int64_t slot = a.per_warp ? int64_t(blockIdx.x) * (blockDim.x / 32) + warp : blockIdx.x;
+  const int64_t slots = a.per_warp ? int64_t(gridDim.x) * (blockDim.x / 32) : gridDim.x;
+  float dw[C][16], w[C][16];
+  pdl_wait();
+  pdl_trigger();
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    load_either<T, WIDE>(a.weight, a.w_f32, 0, (c * warps + first) * 512, lane, a.width, a.vec, w[c]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dw[c][i] = 0.f;
+  }
+  const float inv_width = __fdiv_rn(1.f, float(a.width));
+  for (int64_t row = slot; row < a.rows; row += slots) {  // the same turns for every thread of a row
+    float s[C][16], dy[C][16];
+    float ss = 0.f, dot = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int base = (c * warps + first) * 512;
+      load_either<T, WIDE>(a.s, a.s_f32, row * a.s_stride, base, lane, a.width, a.vec, s[c]);
+      load_row<T, WIDE>(static_cast<const T*>(a.dy) + row * a.dy_stride, base, lane, a.width, a.vec, dy[c]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        ss = fmaf(s[c][i], s[c][i], ss);
+        dot = fmaf(dy[c][i] * w[c][i], s[c][i], dot);
+      }
+    }
+    // both sums at once; the places are those of the row before last, which every thread has read
+    ss = warp_sum(ss);
+    dot = warp_sum(dot);
+    if (!a.per_warp) {
+      const int turn = int((row - slot) / slots) & 1;
+      if (lane == 0) {
+        red[turn][warp] = ss;
+        red[2 + turn][warp] = dot;
+      }
+      __syncthreads();
+      ss = dot = 0.f;
+      for (int i = 0; i < warps; ++i) {
+        ss += red[turn][i];
+        dot += red[2 + turn][i];
+      }
+    }
+    float k = 1.f, rstd = __frsqrt_rn(__fmul_rn(ss, inv_width) + a.eps);
+    float mean = dot * rstd * inv_width;  // of g u
+    if (!(ss < INFINITY) || !(fabsf(dot) < INFINITY)) {
+      __shared__ float far[2][kMaxThreads / 32];
+      float s2 = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s2 = fmaf(s[c][i] * kFar, s[c][i] * kFar, s2);
+      if (!a.per_warp) __syncthreads();  // the places' last readers
+      s2 = row_sum(s2, a.per_warp, far[0]);
+      if (!(ss < INFINITY)) {
+        k = kFar;
+        rstd = __frsqrt_rn(__fmul_rn(s2, inv_width));
+      }
+      dot = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dot = fmaf(dy[c][i] * w[c][i], s[c][i] * k * rstd, dot);
+      mean = row_sum(dot, a.per_warp, far[1]) * inv_width;
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int base = (c * warps + first) * 512;
+      float d[16];
+      if (a.ds)
+        load_either<T, WIDE>(a.ds, a.s_f32, row * a.ds_stride, base, lane, a.width, a.vec, d);
+      else
+#pragma unroll
+        for (int i = 0; i < 16; ++i) d[i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float u = s[c][i] * k * rstd;
+        dw[c][i] = fmaf(dy[c][i], u, dw[c][i]);
+        d[i] = fmaf(rstd * k, dy[c][i] * w[c][i] - u * mean, d[i]);
+      }
+      if (a.grad_sum) store_either<T, WIDE>(a.grad_sum, a.s_f32, row * a.width, base, lane, a.width, a.vec, d);
+      if (a.grad_x) store_row<T, WIDE>(static_cast<T*>(a.grad_x) + row * a.width, base, lane, a.width, a.vec, d);
+    }
+  }
+  if (a.parts) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      store_row<float, WIDE>(a.parts + slot * a.width, (c * warps + first) * 512, lane, a.width, a.vec, dw[c]);
+  }
+}
+
+// dw[column] = sum over the slots in a fixed order: 32 columns per CTA, 32 runs of slots, joined by a tree.
+template <typename TW>
+__global__ void __launch_bounds__(1024) norm_parts_kernel(const float* __restrict__ parts, int64_t slots, int width,
+                                                          TW* __restrict__ out) {
+  __shared__ float sums[32][33];
+  const int lane = threadIdx.x & 31, run = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  pdl_wait();
+  pdl_trigger();
+  float v = 0.f;
+  if (col < width)
+    for (int64_t p = run; p < slots; p += 32) v += parts[p * width + col];
+  sums[run][lane] = v;
+  __syncthreads();
+  if (run == 0 && col < width) {
+    float t[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t[i] = sums[i][lane];
+#pragma unroll
+    for (int d = 16; d; d >>= 1)
+#pragma unroll
+      for (int i = 0; i < d; ++i) t[i] += t[i + d];
+    out[col] = from_f32<TW>(t[0]);
+  }
+}
+
+int status(cudaError_t e) {
+  if (e == cudaSuccess) return B200MOE_OK;
+  cudaGetLastError();
+  return B200MOE_ERR_CUDA;
+}
+
+bool whole(const void* p, int64_t stride, int size) {  // null, or rows on 16 bytes
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0;
+}
+
+// How a row's threads are laid out: a warp per row (8 rows per CTA), or a CTA per row with C pieces of 16 per thread.
+struct Shape {
+  int per_warp, threads, pieces;
+};
+Shape shape_of(int width) {
+  if (width <= 512) return {1, 256, 1};
+  const int c = width <= kMaxThreads * 16 ? 1 : 2;
+  return {0, (width + 512 * c - 1) / (512 * c) * 32, c};
+}
+
+template <typename T, int OUT>
+cudaError_t run_norm(cudaStream_t s, const NormArgs& a, const Shape& sh, bool wide) {
+  const int64_t grid = a.per_warp ? (int64_t(a.rows) + 7) / 8 : a.rows;
+  auto go = [&](auto kernel) { return launch_chain(kernel, dim3(unsigned(grid)), dim3(sh.threads), 0, s, a); };
+  if constexpr (OUT == kRows || OUT == kFp8) {  // 4-bit rows have whole blocks of 32 columns
+    if (!wide) return sh.pieces == 1 ? go(norm_kernel<T, OUT, false, 1>) : go(norm_kernel<T, OUT, false, 2>);
+  }
+  return sh.pieces == 1 ? go(norm_kernel<T, OUT, true, 1>) : go(norm_kernel<T, OUT, true, 2>);
+}
+
+template <typename T>
+cudaError_t run_out(cudaStream_t s, const NormArgs& a, const Shape& sh, bool wide, int out) {
+  return out == kRows    ? run_norm<T, kRows>(s, a, sh, wide)
+         : out == kFp8   ? run_norm<T, kFp8>(s, a, sh, wide)
+         : out == kNvOut ? run_norm<T, kNvOut>(s, a, sh, wide)
+                         : run_norm<T, kMxOut>(s, a, sh, wide);
+}
+
+// Slots of a gradient's walk: CTAs of the GPU's warps, at most one per row.
+int64_t grad_grid(int rows, const Shape& sh) {
+  const int64_t per_sm = std::max(1, 1024 / sh.threads);
+  const int64_t rows_per_cta = sh.per_warp ? sh.threads / 32 : 1;
+  return std::min<int64_t>((rows + rows_per_cta - 1) / rows_per_cta, per_sm * sm_count());
+}
+
+template <typename T>
+cudaError_t run_grad(cudaStream_t s, const GradArgs& a, const Shape& sh, bool wide) {
+  auto go = [&](auto kernel) {
+    return launch_chain(kernel, dim3(unsigned(grad_grid(a.rows, sh))), dim3(sh.threads), 0, s, a);
+  };
+  if (wide) return sh.pieces == 1 ? go(norm_grad_kernel<T, true, 1>) : go(norm_grad_kernel<T, true, 2>);
+  return sh.pieces == 1 ? go(norm_grad_kernel<T, false, 1>) : go(norm_grad_kernel<T, false, 2>);
+}
+
+template <typename TW>
+cudaError_t join(cudaStream_t s, const float* parts, int64_t slots, int width, void* out) {
+  return launch_chain(norm_parts_kernel<TW>, dim3((width + 31) / 32), dim3(1024), 0, s, parts, slots, width,
+                      static_cast<TW*>(out));
+}
+
+bool bad_sizes(int rows, int width, float eps) {
+  return rows < 1 || width < 1 || width > kMaxWidth || !(eps >= 1e-20f) || !(eps < INFINITY);
+}
+
+}  // namespace
+}  // namespace b200moe
+
+using namespace b200moe;
+
+extern "C" int b200moe_rms_norm(void* stream, const void* x, int dtype, int64_t x_stride, const void* residual,
+                                int residual_f32, int64_t residual_stride, const void* weight, int weight_f32, float eps,
+                                int rows, int width, void* sum, void* y, int out, void* q, float* scale) {
+  if (!x || !weight || bad_sizes(rows, width, eps) || x_stride < 0 || residual_stride < 0 || (residual && !sum) ||
+      out < kRows || out > kMxOut || (out == kRows ? !y : !q) || (out == kFp8 && !scale) ||
+      (out >= kNvOut && width % 32))
+    return B200MOE_ERR_INVALID_ARG;
+  if (dtype < 0 || dtype > B200MOE_F32) return B200MOE_ERR_DTYPE;
+  const int b = dtype == B200MOE_F32 ? 4 : 2, rb = residual_f32 ? 4 : b, wb = weight_f32 ? 4 : b;
+  const Shape sh = shape_of(width);
+  if (!whole(q, 0, 1)) return B200MOE_ERR_ALIGN;
+  const int vec = whole(x, x_stride, b) && whole(residual, residual_stride, rb) && whole(weight, 0, wb) &&
+                  whole(sum, width, rb) && whole(y, width, b);
+  const bool wide = width % 8 == 0;
+  const NormArgs a{x,   x_stride, residual, residual_stride, residual_f32, weight, weight_f32, eps, rows, width, sh.per_warp,
+                   vec, sum,      y,        static_cast<uint8_t*>(q), scale};
+  auto run = dtype == B200MOE_F16 ? run_out<__half> : dtype == B200MOE_BF16 ? run_out<__nv_bfloat16> : run_out<float>;
+  return status(run(static_cast<cudaStream_t>(stream), a, sh, wide, out));
+}
+
+extern "C" size_t b200moe_rms_norm_grad_workspace_bytes(int rows, int width) {
+  if (bad_sizes(rows, width, 1.f)) return 0;
+  const Shape sh = shape_of(width);
+  return size_t(grad_grid(rows, sh)) * (sh.per_warp ? sh.threads / 32 : 1) * width * sizeof(float);
+}
+
+extern "C" int b200moe_rms_norm_grad(void* stream, const void* s, int s_f32, int64_t s_stride, const void* grad_y,
+                                     int dtype, int64_t grad_y_stride, const void* grad_s, int64_t grad_s_stride,
+                                     const void* weight, int weight_f32, float eps, int rows, int width, void* grad_x,
+                                     void* grad_sum, void* grad_weight, void* workspace, size_t workspace_bytes) {
+  if (!s || !grad_y || !weight || bad_sizes(rows, width, eps) || s_stride < 0 || grad_y_stride < 0 || grad_s_stride < 0)
+    return B200MOE_ERR_INVALID_ARG;
+  if (dtype < 0 || dtype > B200MOE_F32) return B200MOE_ERR_DTYPE;
+  const Shape sh = shape_of(width);
+  const int64_t slots = grad_grid(rows, sh) * (sh.per_warp ? sh.threads / 32 : 1);
+  if (grad_weight && (!workspace || workspace_bytes < size_t(slots) * width * sizeof(float)))
+    return B200MOE_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return B200MOE_ERR_ALIGN;
+  const int b = dtype == B200MOE_F32 ? 4 : 2, sb = s_f32 ? 4 : b, wb = weight_f32 ? 4 : b;
+  const bool wide = width % 8 == 0;
+  const int vec = whole(s, s_stride, sb) && whole(grad_y, grad_y_stride, b) && whole(grad_s, grad_s_stride, sb) &&
+                  whole(weight, 0, wb) && whole(grad_x, width, b) && whole(grad_sum, width, sb);
+  float* parts = grad_weight ? static_cast<float*>(workspace) : nullptr;
+  const GradArgs a{s, s_stride, s_f32, grad_y, grad_y_stride, grad_s, grad_s_stride, weight, weight_f32, eps, rows, width,
+                   sh.per_warp, vec, grad_x, grad_sum, parts};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto run = dtype == B200MOE_F16 ? run_grad<__half> : dtype == B200MOE_BF16 ? run_grad<__nv_bfloat16> : run_grad<float>;
+  cudaError_t e = run(st, a, sh, wide);
+  if (e == cudaSuccess && grad_weight)
+    e = weight_f32 || dtype == B200MOE_F32 ? join<float>(st, parts, slots, width, grad_weight)
+        : dtype == B200MOE_F16             ? join<__half>(st, parts, slots, width, grad_weight)
+                                           : join<__nv_bfloat16>(st, parts, slots, width, grad_weight);
+  return status(e);
+}
