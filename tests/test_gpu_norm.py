@@ -1,6 +1,6 @@
 """The root-mean-square norm (``norm``) and its gradient against 64-bit forms.
 
-Tolerances.  A thread adds at most 32 squares, a warp 5 sums of them, a CTA 16: 53 roundings of 2^-24 in the mean,
+Tolerances.  A thread adds 16 squares and up to 4 such sums, a warp 5, a CTA 8: at most 53 roundings of 2^-24 in the mean,
 half of that in the root, 6 more operations to y: y is off by less than 2^-19 of itself before its own rounding.  A
 gradient adds the mean of g u, off by 2^-18 of the mean of magnitudes; the weight's adds one rounding per row."""
 

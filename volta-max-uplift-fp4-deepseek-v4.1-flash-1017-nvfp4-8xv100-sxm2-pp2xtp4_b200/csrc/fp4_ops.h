@@ -21,8 +21,10 @@ struct Fp4Product {
   int S, N, K, E;
 };
 
-// tcgen05 kernel (fp4_matmul.cu): rows the MMA's M, tiles of 128 rows x 128 or 256 columns
+// tcgen05 kernel (fp4_matmul.cu): rows the MMA's M, tiles of 128 rows x 128 columns
 int launch_fp4_tiles(cudaStream_t s, const Fp4Product& p, int out_dtype);
+// tcgen05 kernel of pairs of CTAs (fp4_pair.cu): tiles of 256 rows x 256 columns
+int launch_fp4_pairs(cudaStream_t s, const Fp4Product& p, int out_dtype);
 // the same with the weights as the MMA's M, for few rows per matrix: tiles of 16, 32 or 64 rows x 128 columns
 int launch_fp4_stream(cudaStream_t s, const Fp4Product& p, int rows_per_tile, int out_dtype);
 // kernel for one matrix and at most eight rows (fp4_skinny.cu): records, or rows x of f16 or bf16 (stride ldx) that it

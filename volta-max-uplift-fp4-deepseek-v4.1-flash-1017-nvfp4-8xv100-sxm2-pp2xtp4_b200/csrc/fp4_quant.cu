@@ -16,64 +16,88 @@ namespace {
 
 constexpr int kMaxRowThreads = 512;
 
-// 16 columns from c of a row (SWIGLU: of its product with the row's second half).
+// 16 columns of a row as loaded (SWIGLU: and of the row's second half), and their values.
 template <typename T, bool SWIGLU, bool WIDE>
-__device__ __forceinline__ void load16(const T* row, int c, int width, float limit, float (&v)[16]) {
+struct Piece {
   Vec<T, 16> a, b;
-  if constexpr (WIDE) {
-    a.load(row + c);
-    if constexpr (SWIGLU) b.load(row + width + c);
-  } else {
+  __device__ __forceinline__ void load(const T* row, int c, int width) {
+    if constexpr (WIDE) {
+      a.load(row + c);
+      if constexpr (SWIGLU) b.load(row + width + c);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      a.v[i] = row[c + i];
-      if constexpr (SWIGLU) b.v[i] = row[width + c + i];
+      for (int i = 0; i < 16; ++i) {
+        a.v[i] = row[c + i];
+        if constexpr (SWIGLU) b.v[i] = row[width + c + i];
+      }
     }
   }
+  __device__ __forceinline__ void values(float limit, float (&v)[16]) const {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    v[i] = a.get(i);
-    if constexpr (SWIGLU) v[i] = swiglu(v[i], b.get(i), limit);
+    for (int i = 0; i < 16; ++i) {
+      v[i] = a.get(i);
+      if constexpr (SWIGLU) v[i] = swiglu(v[i], b.get(i), limit);
+    }
   }
-}
+};
 
-// A row per CTA, or per warp (blockDim.x / 32 of them) where per_warp is set.
+// A walk over rows, a row per CTA, or per warp (blockDim.x / 32 of them) where per_warp is set. Where the row's threads
+// hold all of it (once), the next row is on its way while this one is worked on.
 template <typename T, bool SWIGLU, bool WIDE>
 __global__ void __launch_bounds__(kMaxRowThreads) nvfp4_rows_kernel(const T* __restrict__ x, int64_t x_stride, int rows,
                                                                     int width, float limit, int per_warp,
                                                                     uint8_t* __restrict__ out) {
-  __shared__ uint32_t warp_max[kMaxRowThreads / 32];
+  __shared__ uint32_t warp_max[2][kMaxRowThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = per_warp ? int64_t(blockIdx.x) * (blockDim.x / 32) + warp : blockIdx.x;
   const int tid = per_warp ? lane : threadIdx.x, threads = per_warp ? 32 : blockDim.x;
+  const int64_t slot = per_warp ? int64_t(blockIdx.x) * (blockDim.x / 32) + warp : blockIdx.x;
+  const int64_t slots = per_warp ? int64_t(gridDim.x) * (blockDim.x / 32) : gridDim.x;
+  const int pieces = width / 16;
+  const bool once = pieces <= threads, in = tid < pieces;
   pdl_wait();
   pdl_trigger();
-  if (row >= rows) return;  // whole warps, and only where no barrier follows
-  const T* src = x + row * x_stride;
-  const int pieces = width / 16;
-  const bool once = pieces <= threads;  // the row stays in registers
-  float v[16];
-  uint32_t m = 0;
-  for (int p = tid; p < pieces; p += threads) {
-    load16<T, SWIGLU, WIDE>(src, p * 16, width, limit, v);
-    m = max(m, abs_bits(magnitude16(v)));
+  Piece<T, SWIGLU, WIDE> next;
+  if (once && in && slot < rows) next.load(x + slot * x_stride, tid * 16, width);
+  int turn = 0;
+  for (int64_t row = slot; row < rows; row += slots, turn ^= 1) {
+    const T* src = x + row * x_stride;
+    float v[16], top = 0.f;
+    uint32_t m = 0;
+    if (once) {
+      if (in) {
+        next.values(limit, v);
+        top = magnitude16(v);
+        if (row + slots < rows) next.load(src + slots * x_stride, tid * 16, width);
+      }
+      m = abs_bits(top);
+    } else {
+      for (int p = tid; p < pieces; p += threads) {
+        next.load(src, p * 16, width);
+        next.values(limit, v);
+        m = max(m, abs_bits(magnitude16(v)));
+      }
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (!per_warp) {  // the places are those of the row before last, which every thread has read
+      if (lane == 0) warp_max[turn][warp] = m;
+      __syncthreads();
+      for (int i = 0; i < int(blockDim.x / 32); ++i) m = max(m, warp_max[turn][i]);
+    }
+    const float factor = nvfp4_factor(m);
+    uint8_t* rec = out + row * fp4_stride(kNv, width);
+    for (int p = tid; p < pieces; p += threads) {
+      if (!once) {
+        next.load(src, p * 16, width);
+        next.values(limit, v);
+        top = magnitude16(v);
+      }
+      float unit;
+      const uint32_t s = nvfp4_scale(top, factor, unit);
+      *reinterpret_cast<uint2*>(rec + p * 8) = nvfp4_codes(v, unit);
+      rec[width / 2 + p] = uint8_t(s);
+    }
+    if (tid == 0) finish_record(rec, kNv, width, factor);
   }
-  m = __reduce_max_sync(0xffffffffu, m);
-  if (!per_warp) {
-    if (lane == 0) warp_max[warp] = m;
-    __syncthreads();
-    for (int i = 0; i < int(blockDim.x / 32); ++i) m = max(m, warp_max[i]);
-  }
-  const float factor = nvfp4_factor(m);
-  uint8_t* rec = out + row * fp4_stride(kNv, width);
-  for (int p = tid; p < pieces; p += threads) {
-    if (!once) load16<T, SWIGLU, WIDE>(src, p * 16, width, limit, v);
-    float unit;
-    const uint32_t s = nvfp4_scale(magnitude16(v), factor, unit);
-    *reinterpret_cast<uint2*>(rec + p * 8) = nvfp4_codes(v, unit);
-    rec[width / 2 + p] = uint8_t(s);
-  }
-  if (tid == 0) finish_record(rec, kNv, width, factor);
 }
 
 // Two neighbouring threads per block of 32 columns of any row.
@@ -89,7 +113,11 @@ __global__ void __launch_bounds__(256) mxfp4_rows_kernel(const T* __restrict__ x
     const int64_t row = in ? (i <= INT32_MAX ? int64_t(uint32_t(i) / uint32_t(pieces)) : i / pieces) : 0;
     const int p = in ? int(i - row * pieces) : 0;
     float v[16], inv;
-    if (in) load16<T, SWIGLU, WIDE>(x + row * x_stride, p * 16, width, limit, v);
+    if (in) {
+      Piece<T, SWIGLU, WIDE> piece;
+      piece.load(x + row * x_stride, p * 16, width);
+      piece.values(limit, v);
+    }
     float m = in ? magnitude16(v) : 0.f;
     m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
     if (!in) continue;
@@ -151,31 +179,38 @@ __global__ void __launch_bounds__(256) fp4_weight_kernel(const T* __restrict__ w
 }
 
 // ---------------------------------------------------------------- read back
-// A thread per 16 columns: value * scale * factor, rounded once.
+// A thread per 32 columns: value * scale (exact in f32, and in f16 for NVFP4) * factor, rounded once.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) fp4_values_kernel(const uint8_t* __restrict__ codes, int64_t ld_codes,
                                                          const uint8_t* __restrict__ scale, int64_t ld_scale,
                                                          const uint8_t* __restrict__ factor, int64_t ld_factor,
                                                          int64_t rows, int width, T* __restrict__ out) {
-  const int pieces = width / 16;
+  const int pieces = width / 32;
   const int64_t total = rows * pieces, step = int64_t(gridDim.x) * 256;
   pdl_wait();
   pdl_trigger();
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += step) {
     const int64_t row = i <= INT32_MAX ? int64_t(uint32_t(i) / uint32_t(pieces)) : i / pieces;
     const int p = int(i - row * pieces);
-    const uint2 c = *reinterpret_cast<const uint2*>(codes + row * ld_codes + p * 8);
-    const uint32_t sb = scale[row * ld_scale + (FMT == kMx ? p / 2 : p)];
-    const float s = FMT == kMx ? e8m0_f32(sb) : e4m3_f32(sb);
-    const float f = factor ? *reinterpret_cast<const float*>(factor + row * ld_factor) : 1.f;
-    float v[16];
-    float(&lo)[8] = *reinterpret_cast<float(*)[8]>(v);
-    float(&hi)[8] = *reinterpret_cast<float(*)[8]>(v + 8);
-    e2m1x8_values(c.x, s, lo);
-    e2m1x8_values(c.y, s, hi);
+    const uint4 c = __ldg(reinterpret_cast<const uint4*>(codes + row * ld_codes) + p);
+    const uint8_t* sp = scale + row * ld_scale + (FMT == kMx ? p : 2 * p);
+    const float f = factor ? __ldg(reinterpret_cast<const float*>(factor + row * ld_factor)) : 1.f;
+    const uint32_t s0 = __ldg(sp), s1 = FMT == kMx ? s0 : __ldg(sp + 1);
+    const float m0 = FMT == kMx ? e8m0_f32(s0) : e4m3_f32(s0), m1 = FMT == kMx ? m0 : e4m3_f32(s1);
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] *= f;
-    store_vec<T, 16>(out + i * 16, v);
+    for (int j = 0; j < 4; ++j) {
+      const float m = j < 2 ? m0 : m1;
+      const uint32_t h[4] = {e2m1x2_byte<0>(w[j]), e2m1x2_byte<1>(w[j]), e2m1x2_byte<2>(w[j]), e2m1x2_byte<3>(w[j])};
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
+        v[2 * k] = q.x * m * f;
+        v[2 * k + 1] = q.y * m * f;
+      }
+      store_vec<T, 8>(out + i * 32 + j * 8, v);
+    }
   }
 }
 
@@ -201,8 +236,9 @@ cudaError_t run_rows(cudaStream_t s, int fmt, const void* x, int64_t x_stride, i
   }
   const int pieces = width / 16, per_warp = pieces <= 32;
   const int threads = per_warp ? 256 : std::min(kMaxRowThreads, (pieces + 31) / 32 * 32);
-  const int64_t grid = per_warp ? (int64_t(rows) + 7) / 8 : rows;
   auto kernel = wide ? nvfp4_rows_kernel<T, SWIGLU, true> : nvfp4_rows_kernel<T, SWIGLU, false>;
+  static Residents residents[2];  // by kernel
+  const int64_t grid = std::min<int64_t>(per_warp ? (int64_t(rows) + 7) / 8 : rows, residents[wide].ctas(kernel, threads));
   return launch_chain(kernel, dim3(unsigned(grid)), dim3(threads), 0, s, src, x_stride, rows, width, limit, per_warp, out);
 }
 
@@ -230,7 +266,7 @@ template <typename T>
 cudaError_t run_values(cudaStream_t s, int fmt, const uint8_t* codes, int64_t ld_codes, const uint8_t* scale,
                        int64_t ld_scale, const uint8_t* factor, int64_t ld_factor, int64_t rows, int width, void* out) {
   auto kernel = fmt == kMx ? fp4_values_kernel<T, kMx> : fp4_values_kernel<T, kNv>;
-  return launch_chain(kernel, dim3(grid_of(rows * (width / 16))), dim3(256), 0, s, codes, ld_codes, scale, ld_scale,
+  return launch_chain(kernel, dim3(grid_of(rows * (width / 32))), dim3(256), 0, s, codes, ld_codes, scale, ld_scale,
                       factor, ld_factor, rows, width, static_cast<T*>(out));
 }
 
@@ -277,7 +313,7 @@ extern "C" int b200moe_fp4_values(void* stream, const void* codes, int64_t ld_co
       ld_factor < 0)
     return B200MOE_ERR_INVALID_ARG;
   if (dtype < 0 || dtype > B200MOE_F32) return B200MOE_ERR_DTYPE;
-  if (!on(codes, 8) || ld_codes % 8 || !on(factor, 4) || ld_factor % 4 || !on(out, 16)) return B200MOE_ERR_ALIGN;
+  if (!on(codes, 16) || ld_codes % 16 || !on(factor, 4) || ld_factor % 4 || !on(out, 16)) return B200MOE_ERR_ALIGN;
   auto run = dtype == B200MOE_F16 ? run_values<__half> : dtype == B200MOE_BF16 ? run_values<__nv_bfloat16>
                                                                                : run_values<float>;
   return status(run(static_cast<cudaStream_t>(stream), format, static_cast<const uint8_t*>(codes), ld_codes,

@@ -126,16 +126,6 @@ __device__ __forceinline__ void finish_record(uint8_t* rec, int fmt, int K, floa
   if (fmt == kNv) *reinterpret_cast<float*>(rec + fp4_factor_at(K)) = factor;
 }
 
-// The values of eight codes times s.
-__device__ __forceinline__ void e2m1x8_values(uint32_t w, float s, float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t n = (w >> (4 * i)) & 15u, e = (n >> 1) & 3u, m = n & 1u;
-    const float mag = e ? __uint_as_float(((e + 126u) << 23) | (m << 22)) : 0.5f * float(m);
-    v[i] = (n & 8u ? -mag : mag) * s;
-  }
-}
-
 __device__ __forceinline__ float e4m3_f32(uint32_t byte) {  // 0x7f / 0xff are NaN
   if ((byte & 0x7fu) == 0x7fu) return fp4_nan();
   const uint32_t ex = (byte >> 3) & 15u, mn = byte & 7u;

@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 struct b200moe_ep;  // the expert-parallel exchange object of the C ABI (ep_p2p.cu)
 
 namespace b200moe {
@@ -202,7 +204,8 @@ int launch_route_combine(cudaStream_t s, const __half* y2, const int32_t* inv, c
                          int n_banks, const float* w, int T, int k, int H, float* out);
 int launch_fp4_tile(cudaStream_t s, bool mx, const uint8_t* codes, const uint8_t* scales, int n_slots,
                     int rows_per_slot, int K, bool gate_up, const float* globals, uint32_t* err, uint8_t* out);
-// 2D uint8 TMA map with 128-byte swizzle: rows x row_bytes, box box_bytes x box_rows, zero fill out of range
+// 2D uint8 TMA map, swizzled by the box's width (32, 64 or 128 bytes): rows x row_bytes, box box_bytes x box_rows, zero
+// fill out of range
 int make_u8_tile_map(void* map_out, const void* base, int64_t rows, int64_t row_bytes, int box_bytes, int box_rows,
                      int64_t stride = 0);  // bytes between rows, 0: row_bytes
 // the same for stores of 64-byte wide boxes with 64-byte swizzle; what lies out of range is not written
@@ -298,5 +301,26 @@ int launch_tc_gemm(cudaStream_t s, int fmt, int epi, const TcArgs& a, const void
 // ---- stateless operators (ops.cu): the current device's error word and SM count
 uint32_t* op_error_word();
 int sm_count();
+
+// CTAs of a kernel that run at once on the current device, by its threads (a multiple of 32 up to 1024): asked once per
+// kernel and size, as a static object beside the launch.
+class Residents {
+ public:
+  template <typename K>
+  int64_t ctas(K kernel, int threads) {
+    int n = per_sm_[threads / 32].load(std::memory_order_relaxed);
+    if (!n) {
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = 1;
+      }
+      per_sm_[threads / 32].store(n, std::memory_order_relaxed);
+    }
+    return int64_t(n) * sm_count();
+  }
+
+ private:
+  std::atomic<int> per_sm_[33] = {};
+};
 
 }  // namespace b200moe

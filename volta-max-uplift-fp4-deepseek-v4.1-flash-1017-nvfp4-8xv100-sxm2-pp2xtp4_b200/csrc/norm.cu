@@ -10,8 +10,9 @@
 // Sums run in f32.  Where a row's squares pass f32's range the row is scaled by
 // 2^-100 first (both are uniform branches that ordinary rows do not take).
 //
-// Forward: a CTA per row (a warp up to 512 columns), 16 columns a thread, the row
-// kept in registers between its sum and its outputs, so every byte moves once.
+// Forward: CTAs walk rows (a warp per row up to 512 columns), 16 columns a thread,
+// the row kept in registers between its sum and its outputs, so every byte moves
+// once, and the next row on its way meanwhile.
 // The quantizers take y in f32: 128 columns' maximum for E4M3, the row's for
 // NVFP4 (a second sum over the CTA), 32 columns' for MXFP4.
 // Backward: a CTA walks rows (rows apart by the grid), holds its columns' part of
@@ -26,8 +27,9 @@
 namespace b200moe {
 namespace {
 
-constexpr int kMaxThreads = 512;
-constexpr int kMaxWidth = kMaxThreads * 16 * 2;
+constexpr int kMaxThreads = 256;
+constexpr int kGradThreads = 512;  // of a gradient's CTAs per SM
+constexpr int kMaxWidth = kMaxThreads * 16 * 4;
 enum Out { kRows = 0, kFp8 = 1, kNvOut = 2, kMxOut = 3 };
 
 // Column i of a thread's 16: WIDE (a width of whole eights), consecutive ones; else single ones 32 apart, so that a
@@ -84,22 +86,13 @@ __device__ __forceinline__ void store_row(T* row, int base, int lane, int width,
     }
   }
 }
-// The same for a tensor of T or, where f32 is set, of float.
+// A row of the weight: T, or float where f32 is set.
 template <typename T, bool WIDE>
-__device__ __forceinline__ void load_either(const void* p, int f32, int64_t offset, int base, int lane, int width,
-                                            int vec, float (&v)[16]) {
+__device__ __forceinline__ void load_weight(const void* p, int f32, int base, int lane, int width, int vec, float (&v)[16]) {
   if (sizeof(T) == 4 || f32)
-    load_row<float, WIDE>(static_cast<const float*>(p) + offset, base, lane, width, vec, v);
+    load_row<float, WIDE>(static_cast<const float*>(p), base, lane, width, vec, v);
   else
-    load_row<T, WIDE>(static_cast<const T*>(p) + offset, base, lane, width, vec, v);
-}
-template <typename T, bool WIDE>
-__device__ __forceinline__ void store_either(void* p, int f32, int64_t offset, int base, int lane, int width,
-                                             int vec, const float (&v)[16]) {
-  if (sizeof(T) == 4 || f32)
-    store_row<float, WIDE>(static_cast<float*>(p) + offset, base, lane, width, vec, v);
-  else
-    store_row<T, WIDE>(static_cast<T*>(p) + offset, base, lane, width, vec, v);
+    load_row<T, WIDE>(static_cast<const T*>(p), base, lane, width, vec, v);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -130,7 +123,6 @@ struct NormArgs {
   int64_t x_stride;
   const void* residual;  // null: none
   int64_t r_stride;
-  int r_f32;  // residual and sum are f32
   const void* weight;
   int w_f32;
   float eps;
@@ -142,140 +134,154 @@ struct NormArgs {
   float* scale;      // E4M3: [rows][ceil(width / 128)]
 };
 
-template <typename T, int OUT, bool WIDE, int C>
-__global__ void __launch_bounds__(kMaxThreads, C == 1 ? 2 : 1) norm_kernel(const NormArgs a) {
-  __shared__ float red[3][kMaxThreads / 32];
+// T: x's type, TR: the residual's and the sum's.
+template <typename T, typename TR, int OUT, bool WIDE, int C>
+__global__ void __launch_bounds__(kMaxThreads, C == 1 ? 3 : 1) norm_kernel(const NormArgs a) {
+  __shared__ float red[3][2][kMaxThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = a.per_warp ? int64_t(blockIdx.x) * (blockDim.x / 32) + warp : blockIdx.x;
   const int warps = a.per_warp ? 1 : blockDim.x / 32, first = a.per_warp ? 0 : warp;
-  pdl_wait();
-  pdl_trigger();
-  if (row >= a.rows) return;  // whole warps, and only where no barrier follows
-  float v[C][16];
-  float ss = 0.f;
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int base = (c * warps + first) * 512;
-    load_row<T, WIDE>(static_cast<const T*>(a.x) + row * a.x_stride, base, lane, a.width, a.vec, v[c]);
-    if (a.residual) {
-      float r[16];
-      load_either<T, WIDE>(a.residual, a.r_f32, row * a.r_stride, base, lane, a.width, a.vec, r);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        v[c][i] += r[i];
-        if (sizeof(T) == 2 && !a.r_f32) v[c][i] = to_f32(from_f32<T>(v[c][i]));
-      }
-      store_either<T, WIDE>(a.sum, a.r_f32, row * a.width, base, lane, a.width, a.vec, v[c]);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) ss = fmaf(v[c][i], v[c][i], ss);
-  }
-  ss = row_sum(ss, a.per_warp, red[0]);
-  Rms n{1.f, 0.f};
-  if (!(ss < INFINITY)) {  // too large for f32, or not finite
-    n.k = kFar;
-    ss = 0.f;
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) ss = fmaf(v[c][i] * kFar, v[c][i] * kFar, ss);
-    ss = row_sum(ss, a.per_warp, red[1]);
-  }
-  n.rstd = __frsqrt_rn(__fdiv_rn(ss, float(a.width)) + (n.k == 1.f ? a.eps : 0.f));
-  uint32_t top = 0;
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int base = (c * warps + first) * 512;
-    float w[16];
-    load_either<T, WIDE>(a.weight, a.w_f32, 0, base, lane, a.width, a.vec, w);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[c][i] = v[c][i] * n.k * n.rstd * w[i];
-    if (a.y) store_row<T, WIDE>(static_cast<T*>(a.y) + row * a.width, base, lane, a.width, a.vec, v[c]);
-    if constexpr (OUT == kNvOut) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (column<WIDE>(base, lane, i) < a.width) top = max(top, abs_bits(v[c][i]));
-    }
-  }
-  if constexpr (OUT == kFp8) {
-    const int nb = (a.width + kFp8Block - 1) / kFp8Block;
-    uint8_t* q = a.q + row * a.width;
+  const int64_t slot = a.per_warp ? int64_t(blockIdx.x) * (blockDim.x / 32) + warp : blockIdx.x;
+  const int64_t slots = a.per_warp ? int64_t(gridDim.x) * (blockDim.x / 32) : gridDim.x;
+  Vec<T, 8> x[C][2];
+  Vec<TR, 8> r[C][2];
+  auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int base = (c * warps + first) * 512;
-      if constexpr (WIDE) {  // eight lanes hold a block
-        float m = magnitude16(v[c]);
+      load_raw<T, WIDE>(static_cast<const T*>(a.x) + row * a.x_stride, base, lane, a.width, a.vec, x[c]);
+      if (a.residual)
+        load_raw<TR, WIDE>(static_cast<const TR*>(a.residual) + row * a.r_stride, base, lane, a.width, a.vec, r[c]);
+    }
+  };
+  pdl_wait();
+  pdl_trigger();
+  if (slot < a.rows) fetch(slot);
+  int turn = 0;  // the sums' places are those of the row before last, which every thread has read
+  for (int64_t row = slot; row < a.rows; row += slots, turn ^= 1) {
+    float v[C][16];
+    float ss = 0.f;
 #pragma unroll
-        for (int d = 4; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
-        const Fp8Scale s = fp8_scale(abs_bits(m));
-        const int col = base + lane * 16;
-        uint32_t o[4];
+    for (int c = 0; c < C; ++c) {
+      const int base = (c * warps + first) * 512;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          o[j] = e4m3x4(v[c][4 * j] * s.inv, v[c][4 * j + 1] * s.inv, v[c][4 * j + 2] * s.inv, v[c][4 * j + 3] * s.inv);
-        if (col < a.width) *reinterpret_cast<uint2*>(q + col) = make_uint2(o[0], o[1]);
-        if (col + 8 < a.width) *reinterpret_cast<uint2*>(q + col + 8) = make_uint2(o[2], o[3]);
-        if ((lane & 7) == 0 && col < a.width) a.scale[row * nb + col / kFp8Block] = s.scale;
-      } else {  // a warp's four columns of each lane are a block
+      for (int i = 0; i < 16; ++i) v[c][i] = x[c][i / 8].get(i % 8);
+      if (a.residual) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          uint32_t m = 0;
+        for (int i = 0; i < 16; ++i) v[c][i] = to_f32(from_f32<TR>(v[c][i] + r[c][i / 8].get(i % 8)));
+        store_row<TR, WIDE>(static_cast<TR*>(a.sum) + row * a.width, base, lane, a.width, a.vec, v[c]);
+      }
+      float part = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) m = max(m, abs_bits(v[c][4 * b + i]));
-          const Fp8Scale s = fp8_scale(__reduce_max_sync(0xffffffffu, m));
-          const uint32_t o = e4m3x4(v[c][4 * b] * s.inv, v[c][4 * b + 1] * s.inv, v[c][4 * b + 2] * s.inv,
-                                    v[c][4 * b + 3] * s.inv);
-          const int col = base + 128 * b + lane;
+      for (int i = 0; i < 16; ++i) part = fmaf(v[c][i], v[c][i], part);
+      ss += part;
+    }
+    if (row + slots < a.rows) fetch(row + slots);
+    ss = row_sum(ss, a.per_warp, red[0][turn]);
+    Rms n{1.f, 0.f};
+    if (!(ss < INFINITY)) {  // too large for f32, or not finite
+      n.k = kFar;
+      ss = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (col + 32 * i < a.width) q[col + 32 * i] = uint8_t(o >> (8 * i));
-          if (lane == 0 && col < a.width) a.scale[row * nb + col / kFp8Block] = s.scale;
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ss = fmaf(v[c][i] * kFar, v[c][i] * kFar, ss);
+      ss = row_sum(ss, a.per_warp, red[1][turn]);
+    }
+    n.rstd = __frsqrt_rn(__fdiv_rn(ss, float(a.width)) + (n.k == 1.f ? a.eps : 0.f));
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int base = (c * warps + first) * 512;
+      float w[16];
+      load_weight<T, WIDE>(a.weight, a.w_f32, base, lane, a.width, a.vec, w);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[c][i] = v[c][i] * n.k * n.rstd * w[i];
+      if (a.y) store_row<T, WIDE>(static_cast<T*>(a.y) + row * a.width, base, lane, a.width, a.vec, v[c]);
+      if constexpr (OUT == kNvOut) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (column<WIDE>(base, lane, i) < a.width) top = max(top, abs_bits(v[c][i]));
+      }
+    }
+    if constexpr (OUT == kFp8) {
+      const int nb = (a.width + kFp8Block - 1) / kFp8Block;
+      uint8_t* q = a.q + row * a.width;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int base = (c * warps + first) * 512;
+        if constexpr (WIDE) {  // eight lanes hold a block
+          float m = magnitude16(v[c]);
+#pragma unroll
+          for (int d = 4; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+          const Fp8Scale s = fp8_scale(abs_bits(m));
+          const int col = base + lane * 16;
+          uint32_t o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[j] = e4m3x4(v[c][4 * j] * s.inv, v[c][4 * j + 1] * s.inv, v[c][4 * j + 2] * s.inv, v[c][4 * j + 3] * s.inv);
+          if (col < a.width) *reinterpret_cast<uint2*>(q + col) = make_uint2(o[0], o[1]);
+          if (col + 8 < a.width) *reinterpret_cast<uint2*>(q + col + 8) = make_uint2(o[2], o[3]);
+          if ((lane & 7) == 0 && col < a.width) a.scale[row * nb + col / kFp8Block] = s.scale;
+        } else {  // a warp's four columns of each lane are a block
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = max(m, abs_bits(v[c][4 * b + i]));
+            const Fp8Scale s = fp8_scale(__reduce_max_sync(0xffffffffu, m));
+            const uint32_t o = e4m3x4(v[c][4 * b] * s.inv, v[c][4 * b + 1] * s.inv, v[c][4 * b + 2] * s.inv,
+                                      v[c][4 * b + 3] * s.inv);
+            const int col = base + 128 * b + lane;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (col + 32 * i < a.width) q[col + 32 * i] = uint8_t(o >> (8 * i));
+            if (lane == 0 && col < a.width) a.scale[row * nb + col / kFp8Block] = s.scale;
+          }
         }
       }
     }
-  }
-  if constexpr (OUT == kNvOut) {
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (!a.per_warp) {
-      uint32_t* tops = reinterpret_cast<uint32_t*>(red[2]);
-      if (lane == 0) tops[warp] = top;
-      __syncthreads();
-      for (int i = 0; i < warps; ++i) top = max(top, tops[i]);
-    }
-    const float factor = nvfp4_factor(top);
-    uint8_t* rec = a.q + row * fp4_stride(kNv, a.width);
+    if constexpr (OUT == kNvOut) {
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (!a.per_warp) {
+        uint32_t* tops = reinterpret_cast<uint32_t*>(red[2][turn]);
+        if (lane == 0) tops[warp] = top;
+        __syncthreads();
+        for (int i = 0; i < warps; ++i) top = max(top, tops[i]);
+      }
+      const float factor = nvfp4_factor(top);
+      uint8_t* rec = a.q + row * fp4_stride(kNv, a.width);
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int col = (c * warps + first) * 512 + lane * 16;
-      if (col >= a.width) continue;
-      float unit;
-      const uint32_t s = nvfp4_scale(magnitude16(v[c]), factor, unit);
-      *reinterpret_cast<uint2*>(rec + col / 2) = nvfp4_codes(v[c], unit);
-      rec[a.width / 2 + col / 16] = uint8_t(s);
+      for (int c = 0; c < C; ++c) {
+        const int col = (c * warps + first) * 512 + lane * 16;
+        if (col >= a.width) continue;
+        float unit;
+        const uint32_t s = nvfp4_scale(magnitude16(v[c]), factor, unit);
+        *reinterpret_cast<uint2*>(rec + col / 2) = nvfp4_codes(v[c], unit);
+        rec[a.width / 2 + col / 16] = uint8_t(s);
+      }
+      if (first == 0 && lane == 0) finish_record(rec, kNv, a.width, factor);
     }
-    if (first == 0 && lane == 0) finish_record(rec, kNv, a.width, factor);
-  }
-  if constexpr (OUT == kMxOut) {
-    uint8_t* rec = a.q + row * fp4_stride(kMx, a.width);
+    if constexpr (OUT == kMxOut) {
+      uint8_t* rec = a.q + row * fp4_stride(kMx, a.width);
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int col = (c * warps + first) * 512 + lane * 16;
-      float m = magnitude16(v[c]), inv;
-      m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      if (col >= a.width) continue;
-      const uint32_t s = mxfp4_scale(m, inv);
-      *reinterpret_cast<uint2*>(rec + col / 2) = mxfp4_codes(v[c], inv);
-      if (!(lane & 1)) rec[a.width / 2 + col / 32] = uint8_t(s);
+      for (int c = 0; c < C; ++c) {
+        const int col = (c * warps + first) * 512 + lane * 16;
+        float m = magnitude16(v[c]), inv;
+        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        if (col >= a.width) continue;
+        const uint32_t s = mxfp4_scale(m, inv);
+        *reinterpret_cast<uint2*>(rec + col / 2) = mxfp4_codes(v[c], inv);
+        if (!(lane & 1)) rec[a.width / 2 + col / 32] = uint8_t(s);
+      }
+      if (first == 0 && lane == 0) finish_record(rec, kMx, a.width, 1.f);
     }
-    if (first == 0 && lane == 0) finish_record(rec, kMx, a.width, 1.f);
   }
 }
 
 // ----------------------------------------------------------------- gradient
 struct GradArgs {
-  const void* s;  // the stored sum (or x), f32 where s_f32
+  const void* s;  // the stored sum (or x)
   int64_t s_stride;
-  int s_f32;
   const void* dy;  // T
   int64_t dy_stride;
   const void* ds;  // the sum's own gradient, of the sum's type, or null
@@ -290,37 +296,62 @@ struct GradArgs {
   float* parts;    // [slots][width], or null
 };
 
-template <typename T, bool WIDE, int C>
-__global__ void __launch_bounds__(kMaxThreads, 1) norm_grad_kernel(const GradArgs a) {
+// T: x's and grad_y's type, TS: the sum's.
+template <typename T, typename TS, bool WIDE, int C>
+__global__ void __launch_bounds__(kMaxThreads, C == 1 ? 2 : 1) norm_grad_kernel(const GradArgs a) {
   __shared__ float red[4][kMaxThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int warps = a.per_warp ? 1 : blockDim.x / 32, first = a.per_warp ? 0 : warp;
   const int64_t slot = a.per_warp ? int64_t(blockIdx.x) * (blockDim.x / 32) + warp : blockIdx.x;
   const int64_t slots = a.per_warp ? int64_t(gridDim.x) * (blockDim.x / 32) : gridDim.x;
+  // 16-bit rows stay as loaded, so that two of them fit in the registers; f32 rows are fetched when their turn comes
+  constexpr bool kAhead = C == 1 && sizeof(TS) == 2;
   float dw[C][16], w[C][16];
+  Vec<TS, 8> rs[C][2], rd[C][2];
+  Vec<T, 8> ry[C][2];
+  auto fetch = [&](int64_t row) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int base = (c * warps + first) * 512;
+      load_raw<TS, WIDE>(static_cast<const TS*>(a.s) + row * a.s_stride, base, lane, a.width, a.vec, rs[c]);
+      load_raw<T, WIDE>(static_cast<const T*>(a.dy) + row * a.dy_stride, base, lane, a.width, a.vec, ry[c]);
+      if (a.ds) load_raw<TS, WIDE>(static_cast<const TS*>(a.ds) + row * a.ds_stride, base, lane, a.width, a.vec, rd[c]);
+    }
+  };
   pdl_wait();
   pdl_trigger();
+  if (kAhead && slot < a.rows) fetch(slot);
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    load_either<T, WIDE>(a.weight, a.w_f32, 0, (c * warps + first) * 512, lane, a.width, a.vec, w[c]);
+    load_weight<T, WIDE>(a.weight, a.w_f32, (c * warps + first) * 512, lane, a.width, a.vec, w[c]);
 #pragma unroll
     for (int i = 0; i < 16; ++i) dw[c][i] = 0.f;
   }
   const float inv_width = __fdiv_rn(1.f, float(a.width));
   for (int64_t row = slot; row < a.rows; row += slots) {  // the same turns for every thread of a row
-    float s[C][16], dy[C][16];
+    if (!kAhead) fetch(row);
+    Vec<TS, 8> cs[C][2], cd[C][2];
+    Vec<T, 8> cy[C][2];
     float ss = 0.f, dot = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int base = (c * warps + first) * 512;
-      load_either<T, WIDE>(a.s, a.s_f32, row * a.s_stride, base, lane, a.width, a.vec, s[c]);
-      load_row<T, WIDE>(static_cast<const T*>(a.dy) + row * a.dy_stride, base, lane, a.width, a.vec, dy[c]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        cs[c][h] = rs[c][h];
+        cd[c][h] = rd[c][h];
+        cy[c][h] = ry[c][h];
+      }
+      float part = 0.f, part_dot = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        ss = fmaf(s[c][i], s[c][i], ss);
-        dot = fmaf(dy[c][i] * w[c][i], s[c][i], dot);
+        const float v = cs[c][i / 8].get(i % 8);
+        part = fmaf(v, v, part);
+        part_dot = fmaf(cy[c][i / 8].get(i % 8) * w[c][i], v, part_dot);
       }
+      ss += part;
+      dot += part_dot;
     }
+    if (kAhead && row + slots < a.rows) fetch(row + slots);
     // both sums at once; the places are those of the row before last, which every thread has read
     ss = warp_sum(ss);
     dot = warp_sum(dot);
@@ -345,7 +376,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_grad_kernel(const GradArg
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s2 = fmaf(s[c][i] * kFar, s[c][i] * kFar, s2);
+        for (int i = 0; i < 16; ++i) {
+          const float v = cs[c][i / 8].get(i % 8) * kFar;
+          s2 = fmaf(v, v, s2);
+        }
       if (!a.per_warp) __syncthreads();  // the places' last readers
       s2 = row_sum(s2, a.per_warp, far[0]);
       if (!(ss < INFINITY)) {
@@ -356,25 +390,21 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_grad_kernel(const GradArg
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) dot = fmaf(dy[c][i] * w[c][i], s[c][i] * k * rstd, dot);
+        for (int i = 0; i < 16; ++i)
+          dot = fmaf(cy[c][i / 8].get(i % 8) * w[c][i], cs[c][i / 8].get(i % 8) * k * rstd, dot);
       mean = row_sum(dot, a.per_warp, far[1]) * inv_width;
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int base = (c * warps + first) * 512;
       float d[16];
-      if (a.ds)
-        load_either<T, WIDE>(a.ds, a.s_f32, row * a.ds_stride, base, lane, a.width, a.vec, d);
-      else
-#pragma unroll
-        for (int i = 0; i < 16; ++i) d[i] = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float u = s[c][i] * k * rstd;
-        dw[c][i] = fmaf(dy[c][i], u, dw[c][i]);
-        d[i] = fmaf(rstd * k, dy[c][i] * w[c][i] - u * mean, d[i]);
+        const float u = cs[c][i / 8].get(i % 8) * k * rstd, dy = cy[c][i / 8].get(i % 8);
+        dw[c][i] = fmaf(dy, u, dw[c][i]);
+        d[i] = fmaf(rstd * k, dy * w[c][i] - u * mean, a.ds ? cd[c][i / 8].get(i % 8) : 0.f);
       }
-      if (a.grad_sum) store_either<T, WIDE>(a.grad_sum, a.s_f32, row * a.width, base, lane, a.width, a.vec, d);
+      if (a.grad_sum) store_row<TS, WIDE>(static_cast<TS*>(a.grad_sum) + row * a.width, base, lane, a.width, a.vec, d);
       if (a.grad_x) store_row<T, WIDE>(static_cast<T*>(a.grad_x) + row * a.width, base, lane, a.width, a.vec, d);
     }
   }
@@ -426,42 +456,57 @@ struct Shape {
 };
 Shape shape_of(int width) {
   if (width <= 512) return {1, 256, 1};
-  const int c = width <= kMaxThreads * 16 ? 1 : 2;
+  const int c = width <= kMaxThreads * 16 ? 1 : width <= kMaxThreads * 32 ? 2 : 4;
   return {0, (width + 512 * c - 1) / (512 * c) * 32, c};
 }
 
-template <typename T, int OUT>
-cudaError_t run_norm(cudaStream_t s, const NormArgs& a, const Shape& sh, bool wide) {
-  const int64_t grid = a.per_warp ? (int64_t(a.rows) + 7) / 8 : a.rows;
-  auto go = [&](auto kernel) { return launch_chain(kernel, dim3(unsigned(grid)), dim3(sh.threads), 0, s, a); };
+template <typename T, typename TR, int OUT>
+cudaError_t run_norm(cudaStream_t s, const NormArgs& a, const Shape& sh) {
+  static Residents residents[6];  // by kernel
+  auto go = [&](auto kernel, int which) {
+    const int64_t most = a.per_warp ? (int64_t(a.rows) + 7) / 8 : a.rows;
+    const int64_t grid = std::min(most, residents[which].ctas(kernel, sh.threads));
+    return launch_chain(kernel, dim3(unsigned(grid)), dim3(sh.threads), 0, s, a);
+  };
   if constexpr (OUT == kRows || OUT == kFp8) {  // 4-bit rows have whole blocks of 32 columns
-    if (!wide) return sh.pieces == 1 ? go(norm_kernel<T, OUT, false, 1>) : go(norm_kernel<T, OUT, false, 2>);
+    if (a.width % 8)
+      return sh.pieces == 1   ? go(norm_kernel<T, TR, OUT, false, 1>, 0)
+             : sh.pieces == 2 ? go(norm_kernel<T, TR, OUT, false, 2>, 1)
+                              : go(norm_kernel<T, TR, OUT, false, 4>, 2);
   }
-  return sh.pieces == 1 ? go(norm_kernel<T, OUT, true, 1>) : go(norm_kernel<T, OUT, true, 2>);
+  return sh.pieces == 1   ? go(norm_kernel<T, TR, OUT, true, 1>, 3)
+         : sh.pieces == 2 ? go(norm_kernel<T, TR, OUT, true, 2>, 4)
+                          : go(norm_kernel<T, TR, OUT, true, 4>, 5);
 }
 
-template <typename T>
-cudaError_t run_out(cudaStream_t s, const NormArgs& a, const Shape& sh, bool wide, int out) {
-  return out == kRows    ? run_norm<T, kRows>(s, a, sh, wide)
-         : out == kFp8   ? run_norm<T, kFp8>(s, a, sh, wide)
-         : out == kNvOut ? run_norm<T, kNvOut>(s, a, sh, wide)
-                         : run_norm<T, kMxOut>(s, a, sh, wide);
+template <typename T, typename TR>
+cudaError_t run_out(cudaStream_t s, const NormArgs& a, const Shape& sh, int out) {
+  return out == kRows    ? run_norm<T, TR, kRows>(s, a, sh)
+         : out == kFp8   ? run_norm<T, TR, kFp8>(s, a, sh)
+         : out == kNvOut ? run_norm<T, TR, kNvOut>(s, a, sh)
+                         : run_norm<T, TR, kMxOut>(s, a, sh);
 }
 
-// Slots of a gradient's walk: CTAs of the GPU's warps, at most one per row.
+// CTAs of a gradient's walk, at most one per row: their number fixes the order of the weight's gradient and its
+// workspace, so it goes by sizes alone and not by what runs at once.
 int64_t grad_grid(int rows, const Shape& sh) {
-  const int64_t per_sm = std::max(1, 1024 / sh.threads);
+  const int64_t per_sm = std::max(1, kGradThreads / sh.threads);
   const int64_t rows_per_cta = sh.per_warp ? sh.threads / 32 : 1;
   return std::min<int64_t>((rows + rows_per_cta - 1) / rows_per_cta, per_sm * sm_count());
 }
 
-template <typename T>
-cudaError_t run_grad(cudaStream_t s, const GradArgs& a, const Shape& sh, bool wide) {
+template <typename T, typename TS>
+cudaError_t run_grad(cudaStream_t s, const GradArgs& a, const Shape& sh) {
   auto go = [&](auto kernel) {
     return launch_chain(kernel, dim3(unsigned(grad_grid(a.rows, sh))), dim3(sh.threads), 0, s, a);
   };
-  if (wide) return sh.pieces == 1 ? go(norm_grad_kernel<T, true, 1>) : go(norm_grad_kernel<T, true, 2>);
-  return sh.pieces == 1 ? go(norm_grad_kernel<T, false, 1>) : go(norm_grad_kernel<T, false, 2>);
+  if (a.width % 8 == 0)
+    return sh.pieces == 1   ? go(norm_grad_kernel<T, TS, true, 1>)
+           : sh.pieces == 2 ? go(norm_grad_kernel<T, TS, true, 2>)
+                            : go(norm_grad_kernel<T, TS, true, 4>);
+  return sh.pieces == 1   ? go(norm_grad_kernel<T, TS, false, 1>)
+         : sh.pieces == 2 ? go(norm_grad_kernel<T, TS, false, 2>)
+                          : go(norm_grad_kernel<T, TS, false, 4>);
 }
 
 template <typename TW>
@@ -492,11 +537,13 @@ extern "C" int b200moe_rms_norm(void* stream, const void* x, int dtype, int64_t 
   if (!whole(q, 0, 1)) return B200MOE_ERR_ALIGN;
   const int vec = whole(x, x_stride, b) && whole(residual, residual_stride, rb) && whole(weight, 0, wb) &&
                   whole(sum, width, rb) && whole(y, width, b);
-  const bool wide = width % 8 == 0;
-  const NormArgs a{x,   x_stride, residual, residual_stride, residual_f32, weight, weight_f32, eps, rows, width, sh.per_warp,
+  const NormArgs a{x,   x_stride, residual, residual_stride, weight, weight_f32, eps, rows, width, sh.per_warp,
                    vec, sum,      y,        static_cast<uint8_t*>(q), scale};
-  auto run = dtype == B200MOE_F16 ? run_out<__half> : dtype == B200MOE_BF16 ? run_out<__nv_bfloat16> : run_out<float>;
-  return status(run(static_cast<cudaStream_t>(stream), a, sh, wide, out));
+  const bool far = residual_f32 && residual;  // a residual of another type than 16-bit rows
+  auto run = dtype == B200MOE_F16    ? (far ? run_out<__half, float> : run_out<__half, __half>)
+             : dtype == B200MOE_BF16 ? (far ? run_out<__nv_bfloat16, float> : run_out<__nv_bfloat16, __nv_bfloat16>)
+                                     : run_out<float, float>;
+  return status(run(static_cast<cudaStream_t>(stream), a, sh, out));
 }
 
 extern "C" size_t b200moe_rms_norm_grad_workspace_bytes(int rows, int width) {
@@ -518,15 +565,16 @@ extern "C" int b200moe_rms_norm_grad(void* stream, const void* s, int s_f32, int
     return B200MOE_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return B200MOE_ERR_ALIGN;
   const int b = dtype == B200MOE_F32 ? 4 : 2, sb = s_f32 ? 4 : b, wb = weight_f32 ? 4 : b;
-  const bool wide = width % 8 == 0;
   const int vec = whole(s, s_stride, sb) && whole(grad_y, grad_y_stride, b) && whole(grad_s, grad_s_stride, sb) &&
                   whole(weight, 0, wb) && whole(grad_x, width, b) && whole(grad_sum, width, sb);
   float* parts = grad_weight ? static_cast<float*>(workspace) : nullptr;
-  const GradArgs a{s, s_stride, s_f32, grad_y, grad_y_stride, grad_s, grad_s_stride, weight, weight_f32, eps, rows, width,
+  const GradArgs a{s, s_stride, grad_y, grad_y_stride, grad_s, grad_s_stride, weight, weight_f32, eps, rows, width,
                    sh.per_warp, vec, grad_x, grad_sum, parts};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto run = dtype == B200MOE_F16 ? run_grad<__half> : dtype == B200MOE_BF16 ? run_grad<__nv_bfloat16> : run_grad<float>;
-  cudaError_t e = run(st, a, sh, wide);
+  auto run = dtype == B200MOE_F16    ? (s_f32 ? run_grad<__half, float> : run_grad<__half, __half>)
+             : dtype == B200MOE_BF16 ? (s_f32 ? run_grad<__nv_bfloat16, float> : run_grad<__nv_bfloat16, __nv_bfloat16>)
+                                     : run_grad<float, float>;
+  cudaError_t e = run(st, a, sh);
   if (e == cudaSuccess && grad_weight)
     e = weight_f32 || dtype == B200MOE_F32 ? join<float>(st, parts, slots, width, grad_weight)
         : dtype == B200MOE_F16             ? join<__half>(st, parts, slots, width, grad_weight)
