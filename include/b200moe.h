@@ -449,7 +449,7 @@ int b200moe_fp4_matmul(void* stream, const void* a, const void* w, const void* w
 /* The same for one matrix and rows x of f16, bf16 or f32 (ldx elements between
  * them), quantized in the call, into the workspace where b200moe_fp4_linear_workspace_bytes
  * is not 0 (on a 16-byte address; S * b200moe_fp4_record_bytes always suffices).  0
- * holds for 16-bit x on 16 bytes, rows a multiple of 16 bytes apart. */
+ * holds for 16-bit x on 16 bytes, rows a multiple of 16 bytes apart, and w_scale on 2. */
 size_t b200moe_fp4_linear_workspace_bytes(int S, int N, int K, int format);
 int b200moe_fp4_linear(void* stream, const void* x, int x_dtype, int64_t ldx, const void* w, const void* w_scale,
                        const float* w_factor, int S, int N, int K, int format, void* out, int out_dtype, void* workspace,

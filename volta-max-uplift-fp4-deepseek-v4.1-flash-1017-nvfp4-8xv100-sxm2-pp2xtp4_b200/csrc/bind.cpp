@@ -658,7 +658,8 @@ Tensor fp4_linear(const Tensor& x, const Tensor& codes, const Tensor& scale, con
   Tensor out = empty({m, n}, dtype, x), ws;
   if (m == 0) return out;
   int64_t bytes = m * record_bytes(format, k);
-  if (x.scalar_type() != ScalarType::Float && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && x.stride(0) % 8 == 0)
+  if (x.scalar_type() != ScalarType::Float && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && x.stride(0) % 8 == 0 &&
+      reinterpret_cast<uintptr_t>(scale.data_ptr()) % 2 == 0)
     bytes = int64_t(b200moe_fp4_linear_workspace_bytes(int(m), int(n), int(k), int(format)));
   if (bytes) ws = empty({bytes}, ScalarType::Byte, x);
   check("b200moe_fp4_linear",

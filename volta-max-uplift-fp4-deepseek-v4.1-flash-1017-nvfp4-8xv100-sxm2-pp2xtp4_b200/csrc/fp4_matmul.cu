@@ -356,9 +356,10 @@ int product_status(const Fp4Product& p, int out_dtype) {
 //   their mean. 384 matrices 4096 x 4096: 555 / 554 / 616 at 8, 1070 / 601 / 643 / 737 / 839 at 24, 1875 / 1112 / 671 /
 //   848 / 962 at 48, - / - / 1633 / 1225 / 885 at 128: there 20 is before the crossing (7 % at 24).
 //   S counts rows without an expert too, and no spread is known here.
-// Returns 16, 32, 64, 128 or 256.
+// Returns 8 (fp4_skinny.cu), 16, 32, 64, 128 or 256.
 int choose(const Fp4Product& p) {
   if (!p.offsets) {
+    if (fp4_skinny_fits(p)) return 8;
     for (int t = 16; t <= 128; t *= 2)
       if (t != 64 && (p.S + t - 1) / t * int64_t((p.N + 127) / 128) <= sm_count()) return t;
     return p.S <= 32 ? 32 : p.S <= 128 ? 128 : 256;
@@ -375,7 +376,8 @@ int launch_status(int rc) {
 
 int run_product(cudaStream_t s, const Fp4Product& p, int out_dtype) {
   const int kind = choose(p);
-  return launch_status(kind == 256   ? launch_fp4_pairs(s, p, out_dtype)
+  return launch_status(kind == 8     ? launch_fp4_skinny(s, p, nullptr, 0, 0, out_dtype)
+                       : kind == 256 ? launch_fp4_pairs(s, p, out_dtype)
                        : kind == 128 ? launch_fp4_tiles(s, p, out_dtype)
                                      : launch_fp4_stream(s, p, kind, out_dtype));
 }
@@ -394,7 +396,13 @@ extern "C" int b200moe_fp4_matmul(void* stream, const void* a, const void* w, co
 }
 
 extern "C" size_t b200moe_fp4_linear_workspace_bytes(int S, int N, int K, int format) {
-  if (S < 1 || N < 1) return 0;
+  Fp4Product p{};
+  p.format = format;
+  p.S = S;
+  p.N = N;
+  p.K = K;
+  p.E = 1;
+  if (S < 1 || N < 1 || K < 32 || (choose(p) == 8 && fp4_skinny_quantizes(S, K))) return 0;
   return size_t(S) * b200moe_fp4_record_bytes(format, K);
 }
 
@@ -407,9 +415,14 @@ extern "C" int b200moe_fp4_linear(void* stream, const void* x, int x_dtype, int6
   if (st) return st;
   if (!x || ldx < 0) return B200MOE_ERR_INVALID_ARG;
   if (x_dtype < 0 || x_dtype > B200MOE_F32) return B200MOE_ERR_DTYPE;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t ld_bytes = ldx * (x_dtype == B200MOE_F32 ? 4 : 2);
+  if (choose(p) == 8 && fp4_skinny_quantizes(S, K) && x_dtype != B200MOE_F32 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_bytes % 16 == 0)
+    return launch_status(launch_fp4_skinny(s, p, x, x_dtype, ldx, out_dtype));
   if (!workspace || workspace_bytes < size_t(S) * b200moe_fp4_record_bytes(format, K)) return B200MOE_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return B200MOE_ERR_ALIGN;
   const int qs = b200moe_fp4_quantize(stream, x, x_dtype, ldx, S, K, format, 0, 1.f, workspace);
   if (qs) return qs;
   p.a = static_cast<const uint8_t*>(workspace);
-  return run_product(static_cast<cudaStream_t>(stream), p, out_dtype);
+  return run_product(s, p, out_dtype);
 }

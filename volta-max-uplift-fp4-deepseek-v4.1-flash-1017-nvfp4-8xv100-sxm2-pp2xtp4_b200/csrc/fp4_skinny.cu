@@ -1,0 +1,242 @@
+// NVFP4 products of at most eight rows with one matrix: the weights go straight from
+// global memory into the registers of the warps that multiply them. One launch does
+// it all: one or two rows of f16 or bf16 are quantized by every CTA for itself.
+//
+// A warp owns 16 weight rows and every KS-th block of 256 columns; per block each lane
+// loads four 16-byte pieces (32 columns each: rows g and g + 8, pieces q and q + 4; g =
+// lane / 4, q = lane % 4) and their scales.  Operands are f16, which holds a value times
+// its block's scale exactly (six bits, 2^-10 to 2688), by one conversion and one product
+// per two values; both operands take the columns in the same order, so no value moves
+// between lanes.  The KS warps of a row tile add their f32 sums in shared memory in a
+// fixed order.  MXFP4's scales pass f16's range: its rows take the streaming kernel.
+//
+// Bound: latency: all of a small matrix is in flight at once. Taken as long as all
+// CTAs, of 16 or 32 weight rows, run at once.
+#include <algorithm>
+#include <atomic>
+
+#include "fp4_ops.h"
+#include "fp4_rows.cuh"
+#include "internal.h"
+
+namespace b200moe {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTokens = 8;
+constexpr int kBlockK = 256;
+constexpr int kDeep = 2;  // blocks of a warp in flight
+constexpr int kSmemMost = 200 * 1024;
+constexpr int kPieceBytes = 80;  // 32 bf16 values and 16 bytes, so that a fragment load's lanes do not meet
+
+// Bytes of a row in shared memory: 64 above a multiple of 128, so that neighbouring rows do not meet either.
+__host__ __device__ constexpr int row_pitch(int K) { return (K / 32 * kPieceBytes + 63) / 128 * 128 + 64; }
+
+struct SkinnyArgs {
+  const uint8_t* a;  // records, or the rows to quantize (stride ldx elements)
+  int64_t ldx;
+  const uint8_t* w;
+  const uint8_t* w_scale;
+  const float* w_factor;
+  void* out;
+  int S, N, K;
+};
+
+__device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {  // weights: read once
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+// 16 columns of a row (half a piece), as codes and their scale's value, to shared memory.  The codes' values come from
+// their bits: ptxas 12.9 joins cvt.rn.f16x2.e2m1x2 with the conversion that made the codes in the same thread, and takes a
+// wrong byte of it (rows came out as zeros).
+__device__ __forceinline__ void put_tokens(uint8_t* row, int p, uint2 codes, float scale) {
+  const __half2 s = __float2half2_rn(scale);
+  uint4* dst = reinterpret_cast<uint4*>(row + p / 2 * kPieceBytes + (p & 1) * 32);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t w = h ? codes.y : codes.x;
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // exponent and mantissa bits in f16's place are the value times 2^-14
+      const uint32_t b = w >> (8 * i);
+      const uint32_t bits = (b & 7u) << 9 | (b & 8u) << 12 | (b & 0x70u) << 21 | (b & 0x80u) << 24;
+      o[i] = hmul2(hmul2(bits, 0x74007400u), *reinterpret_cast<const uint32_t*>(&s));
+    }
+    dst[h] = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// The rows' values in shared memory and their factors; TX of one byte: records.
+template <typename TX>
+__device__ __forceinline__ void stage_tokens(const SkinnyArgs& A, uint8_t* xs, float* factor, uint32_t* top) {
+  const int pieces = A.K / 16, total = A.S * pieces, pitch = row_pitch(A.K);
+  if constexpr (sizeof(TX) == 1) {
+    const int stride = fp4_stride(kNv, A.K);
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+      const int r = i / pieces, p = i - r * pieces;
+      const uint8_t* rec = A.a + int64_t(r) * stride;
+      put_tokens(xs + r * pitch, p, __ldg(reinterpret_cast<const uint2*>(rec) + p), e4m3_f32(__ldg(rec + A.K / 2 + p)));
+    }
+    if (threadIdx.x < A.S)
+      factor[threadIdx.x] = *reinterpret_cast<const float*>(A.a + int64_t(threadIdx.x) * stride + fp4_factor_at(A.K));
+  } else {
+    const TX* x = reinterpret_cast<const TX*>(A.a);
+    float v[16], m = 0.f;
+    auto load = [&](int i) {
+      const int r = i / pieces, p = i - r * pieces;
+      Vec<TX, 16> raw;
+      raw.load(x + r * A.ldx + p * 16);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = raw.get(j);
+      m = magnitude16(v);
+    };
+    if (threadIdx.x < kTokens) top[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i0 = threadIdx.x & ~31; i0 < total; i0 += kThreads) {
+      const int i = i0 + (threadIdx.x & 31);
+      uint32_t t = 0;
+      if (i < total) {
+        load(i);
+        t = abs_bits(m);
+      }
+      if (pieces % 32 == 0) t = __reduce_max_sync(0xffffffffu, t);  // the warp's columns are of one row
+      if (i < total && (pieces % 32 || i == i0)) atomicMax(top + i / pieces, t);  // in any order, a maximum is the same
+    }
+    __syncthreads();
+    if (threadIdx.x < A.S) factor[threadIdx.x] = nvfp4_factor(top[threadIdx.x]);
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+      if (total > kThreads) load(i);  // else the columns are still here
+      const int r = i / pieces;
+      float unit;
+      const uint32_t s = nvfp4_scale(m, nvfp4_factor(top[r]), unit);
+      put_tokens(xs + r * pitch, i - r * pieces, nvfp4_codes(v, unit), e4m3_f32(s));
+    }
+  }
+}
+
+template <typename TX, typename TO, int KS>
+__global__ void __launch_bounds__(kThreads, 2) fp4_skinny_kernel(const SkinnyArgs A) {
+  constexpr int RT = kWarps / KS;  // 16-row tiles of w per CTA
+  __shared__ float red[kWarps][4][32];
+  __shared__ float factor[kTokens];
+  __shared__ uint32_t top[kTokens];
+  extern __shared__ __align__(16) uint8_t xs[];  // [S][row_pitch]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int ksub = warp % KS, rsub = warp / KS;
+  const int n0 = (blockIdx.x * RT + rsub) * 16, KB = (A.K + kBlockK - 1) / kBlockK;
+  const int per_warp = (KB + KS - 1) / KS, n_steps = (per_warp + kDeep - 1) / kDeep;
+  const int half_k = A.K / 2, scales = A.K / 16;
+  pdl_wait();
+
+  uint4 w[kDeep][4];
+  uint32_t ws[kDeep][4];  // the pieces' scale bytes
+  auto fetch = [&](int step, int j) {
+    const int kb = (step * kDeep + j) * KS + ksub;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int row = n0 + g + 8 * h, piece = kb * 8 + c * 4 + q;
+        const bool in = row < A.N && piece * 32 < A.K;
+        w[j][h * 2 + c] = in ? ld_stream(A.w + int64_t(row) * half_k + piece * 16) : make_uint4(0, 0, 0, 0);
+        ws[j][h * 2 + c] =
+            in ? uint32_t(__ldg(reinterpret_cast<const uint16_t*>(A.w_scale + int64_t(row) * scales + 2 * piece))) : 0u;
+      }
+  };
+
+#pragma unroll
+  for (int j = 0; j < kDeep; ++j) fetch(0, j);
+  stage_tokens<TX>(A, xs, factor, top);
+  __syncthreads();
+  const uint8_t* mine = xs + g * row_pitch(A.K);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int step = 0; step < n_steps; ++step) {
+#pragma unroll
+    for (int j = 0; j < kDeep; ++j) {
+      const int kb = (step * kDeep + j) * KS + ksub;
+      if (kb < KB) {  // the same for the whole warp
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int piece = kb * 8 + c * 4 + q;
+          const uint32_t lo[4] = {w[j][c].x, w[j][c].y, w[j][c].z, w[j][c].w};
+          const uint32_t hi[4] = {w[j][2 + c].x, w[j][2 + c].y, w[j][2 + c].z, w[j][2 + c].w};
+          const uint32_t ml = e4m3x2_to_f16x2(ws[j][c]), mh = e4m3x2_to_f16x2(ws[j][2 + c]);  // of both halves
+          const bool in = g < A.S && piece * 32 < A.K;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {  // eight columns of this lane: two MMAs of 16 columns
+            const uint4 x = in ? *reinterpret_cast<const uint4*>(mine + piece * kPieceBytes + i * 16) : make_uint4(0, 0, 0, 0);
+            uint32_t a[4], b[4];
+            e2m1x8_scaled(lo[i], i < 2 ? lo_half2(ml) : hi_half2(ml), a);
+            e2m1x8_scaled(hi[i], i < 2 ? lo_half2(mh) : hi_half2(mh), b);
+            mma_16816(acc, {a[0], b[0], a[1], b[1]}, x.x, x.y);
+            mma_16816(acc, {a[2], b[2], a[3], b[3]}, x.z, x.w);
+          }
+        }
+      }
+      if (step + 1 < n_steps) fetch(step + 1, j);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) red[warp][i][lane] = acc[i];
+  __syncthreads();
+  const float fw = *A.w_factor;
+  for (int o = ksub * 32 + lane; o < 16 * kTokens; o += KS * 32) {
+    const int t = o >> 4, r = o & 15, col = n0 + r;
+    const int slot = (r >> 3) * 2 + (t & 1), src = (r & 7) * 4 + (t >> 1);
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) sum += red[rsub * KS + k][slot][src];
+    if (t < A.S && col < A.N) static_cast<TO*>(A.out)[int64_t(t) * A.N + col] = from_f32<TO>(sum * factor[t] * fw);
+  }
+  pdl_trigger();
+}
+
+// Eight warps along K where each has two blocks, else two row tiles of four warps.
+bool deep(int K) { return K > 4 * kDeep * kBlockK; }
+int skinny_grid(int N, int K) {
+  const int rows = 16 * (deep(K) ? 1 : 2);
+  return (N + rows - 1) / rows;
+}
+size_t skinny_smem(int S, int K) { return size_t(S) * row_pitch(K); }
+
+template <typename TX, typename TO, int KS>
+int launch_one(cudaStream_t s, const SkinnyArgs& a) {
+  auto kernel = fp4_skinny_kernel<TX, TO, KS>;
+  static std::atomic<uint64_t> attr_set{0};  // devices whose attribute is set
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -1;
+  if (!(attr_set.load() >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost) != cudaSuccess) return -1;
+    attr_set.fetch_or(uint64_t(1) << dev);
+  }
+  return launch_chain(kernel, dim3(skinny_grid(a.N, a.K)), dim3(kThreads), skinny_smem(a.S, a.K), s, a) == cudaSuccess ? 0 : -1;
+}
+
+template <typename TX>
+int launch_out(cudaStream_t s, const SkinnyArgs& a, int out_dtype) {
+  const bool d = deep(a.K);
+  if (out_dtype == B200MOE_F16) return d ? launch_one<TX, __half, 8>(s, a) : launch_one<TX, __half, 4>(s, a);
+  if (out_dtype == B200MOE_BF16)
+    return d ? launch_one<TX, __nv_bfloat16, 8>(s, a) : launch_one<TX, __nv_bfloat16, 4>(s, a);
+  return d ? launch_one<TX, float, 8>(s, a) : launch_one<TX, float, 4>(s, a);
+}
+
+}  // namespace
+
+bool fp4_skinny_fits(const Fp4Product& p) {
+  if (p.format != kNv || p.E != 1 || p.offsets || p.S > kTokens || reinterpret_cast<uintptr_t>(p.w_scale) % 2) return false;
+  const size_t smem = skinny_smem(p.S, p.K);
+  return smem <= kSmemMost && skinny_grid(p.N, p.K) <= sm_count() * (smem <= 100 * 1024 ? 2 : 1);
+}
+
+int launch_fp4_skinny(cudaStream_t s, const Fp4Product& p, const void* x, int x_dtype, int64_t ldx, int out_dtype) {
+  const SkinnyArgs a{x ? static_cast<const uint8_t*>(x) : p.a, ldx, p.w, p.w_scale, p.w_factor, p.out, p.S, p.N, p.K};
+  if (!x) return launch_out<uint8_t>(s, a, out_dtype);
+  return x_dtype == B200MOE_F16 ? launch_out<__half>(s, a, out_dtype) : launch_out<__nv_bfloat16>(s, a, out_dtype);
+}
+
+}  // namespace b200moe

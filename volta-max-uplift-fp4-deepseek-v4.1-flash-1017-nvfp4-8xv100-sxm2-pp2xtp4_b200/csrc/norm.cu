@@ -18,7 +18,11 @@
 // Backward: a CTA walks rows (rows apart by the grid), holds its columns' part of
 // dw in registers, and loads the next row before it works on this one; the parts
 // are joined by a second launch in a fixed order, so equal inputs give equal bits.
-// Bound: HBM both ways.
+// Bound: HBM. 16384 x 4096 bf16 with a residual: rows 83 us (6.4 TB/s), E4M3 76, MXFP4 72
+// (6.1), NVFP4 93 (4.7: two sums over the CTA, and the codes' quotients), gradient 98
+// (5.5). What held it back was instructions: 41 per value forward and 56 backward by
+// single conversions and sums read one by one, 109 (NVFP4) and 187 us. The gradient
+// with its weights and the sum's gradient a row ahead in registers too: 115, spilled.
 #include <algorithm>
 
 #include "fp4_rows.cuh"
@@ -28,25 +32,57 @@ namespace b200moe {
 namespace {
 
 constexpr int kMaxThreads = 256;
-constexpr int kGradThreads = 512;  // of a gradient's CTAs per SM
 constexpr int kMaxWidth = kMaxThreads * 16 * 4;
 enum Out { kRows = 0, kFp8 = 1, kNvOut = 2, kMxOut = 3 };
 
-// Column i of a thread's 16: WIDE (a width of whole eights), consecutive ones; else single ones 32 apart, so that a
-// warp's access is one run of bytes.  The order of a row's sums goes by its width alone: whether WIDE columns move as
-// vectors (vec, where every address allows it) changes no bit.
-template <bool WIDE>
-__device__ __forceinline__ int column(int base, int lane, int i) {
-  return WIDE ? base + lane * 16 + i : base + lane + 32 * i;
+// A thread's columns: WIDE (a width of whole eights), consecutive ones; else single ones 32 apart, so that a warp's access
+// is one run of bytes.  The order of a row's sums goes by its width alone: whether WIDE columns move as vectors (vec, where
+// every address allows it) changes no bit.
+
+// Eight values by pairs: 16-bit types take one instruction per two of them into the type, one per value out of it.
+__device__ __forceinline__ void unpack8(const Vec<float, 8>& x, float* v) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = x.v[i];
+}
+__device__ __forceinline__ void unpack8(const Vec<__nv_bfloat16, 8>& x, float* v) {
+  const uint32_t(&u)[4] = reinterpret_cast<const uint32_t(&)[4]>(x.v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(u[i] << 16);
+    v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack8(const Vec<__half, 8>& x, float* v) {
+  const __half2(&h)[4] = reinterpret_cast<const __half2(&)[4]>(x.v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void pack8(Vec<float, 8>& x, const float* v) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x.v[i] = v[i];
+}
+__device__ __forceinline__ void pack8(Vec<__nv_bfloat16, 8>& x, const float* v) {
+  __nv_bfloat162(&h)[4] = reinterpret_cast<__nv_bfloat162(&)[4]>(x.v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+}
+__device__ __forceinline__ void pack8(Vec<__half, 8>& x, const float* v) {
+  __half2(&h)[4] = reinterpret_cast<__half2(&)[4]>(x.v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
 }
 
-// The thread's 16 values of a row of T from the warp's first column; zeros past the width.
-template <typename T, bool WIDE>
-__device__ __forceinline__ void load_raw(const T* row, int base, int lane, int width, int vec, Vec<T, 8> (&v)[2]) {
+// The thread's 8 PARTS values of a row of T from the warp's first column; zeros past the width.
+template <typename T, bool WIDE, int PARTS>
+__device__ __forceinline__ void load_raw(const T* row, int base, int lane, int width, int vec, Vec<T, 8> (&v)[PARTS]) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < PARTS; ++h) {
     if constexpr (WIDE) {
-      const int c = base + lane * 16 + 8 * h;
+      const int c = base + lane * 8 * PARTS + 8 * h;
       if (c < width && vec) {
         v[h].load(row + c);
       } else if (c < width) {
@@ -61,34 +97,39 @@ __device__ __forceinline__ void load_raw(const T* row, int base, int lane, int w
     }
   }
 }
-template <typename T, bool WIDE>
-__device__ __forceinline__ void load_row(const T* row, int base, int lane, int width, int vec, float (&v)[16]) {
-  Vec<T, 8> r[2];
+template <typename T, bool WIDE, int N>
+__device__ __forceinline__ void load_row(const T* row, int base, int lane, int width, int vec, float (&v)[N]) {
+  Vec<T, 8> r[N / 8];
   load_raw<T, WIDE>(row, base, lane, width, vec, r);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = r[i / 8].get(i % 8);
+  for (int h = 0; h < N / 8; ++h) unpack8(r[h], v + 8 * h);
 }
-template <typename T, bool WIDE>
-__device__ __forceinline__ void store_row(T* row, int base, int lane, int width, int vec, const float (&v)[16]) {
+template <typename T, bool WIDE, int PARTS>
+__device__ __forceinline__ void store_raw(T* row, int base, int lane, int width, int vec, const Vec<T, 8> (&v)[PARTS]) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const float(&part)[8] = *reinterpret_cast<const float(*)[8]>(v + 8 * h);
-    if constexpr (WIDE) {
-      const int c = base + lane * 16 + 8 * h;
-      if (c < width && vec) {
-        store_vec<T, 8>(row + c, part);
-      } else if (c < width) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) row[c + i] = from_f32<T>(part[i]);
-      }
+  for (int h = 0; h < PARTS; ++h) {
+    const int c = WIDE ? base + lane * 8 * PARTS + 8 * h : base + lane + 256 * h;
+    if (WIDE && vec) {
+      if (c < width) v[h].store(row + c);
     } else {
-      store_columns<false>(row, base + lane + 256 * h, 32, width, part);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = WIDE ? c + i : c + 32 * i;
+        if (at < width) row[at] = v[h].v[i];
+      }
     }
   }
 }
+template <typename T, bool WIDE, int N>
+__device__ __forceinline__ void store_row(T* row, int base, int lane, int width, int vec, const float (&v)[N]) {
+  Vec<T, 8> r[N / 8];
+#pragma unroll
+  for (int h = 0; h < N / 8; ++h) pack8(r[h], v + 8 * h);
+  store_raw<T, WIDE>(row, base, lane, width, vec, r);
+}
 // A row of the weight: T, or float where f32 is set.
-template <typename T, bool WIDE>
-__device__ __forceinline__ void load_weight(const void* p, int f32, int base, int lane, int width, int vec, float (&v)[16]) {
+template <typename T, bool WIDE, int N>
+__device__ __forceinline__ void load_weight(const void* p, int f32, int base, int lane, int width, int vec, float (&v)[N]) {
   if (sizeof(T) == 4 || f32)
     load_row<float, WIDE>(static_cast<const float*>(p), base, lane, width, vec, v);
   else
@@ -100,23 +141,19 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
 }
-// The sum over the row's threads, the same bits in each; red: a place of kMaxThreads / 32 floats that no sum before used
-// since the last barrier.
-__device__ __forceinline__ float row_sum(float v, int per_warp, float* red) {
+// The sums over the row's threads, the same bits in each; red: a place of its own for each warp, zeros in those that the CTA
+// does not have, that no sum before used since the last barrier.
+__device__ __forceinline__ float row_sum(float v, int per_warp, float (&red)[kMaxThreads / 32]) {
   v = warp_sum(v);
   if (per_warp) return v;
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = 0.f;
-  for (int i = 0; i < int(blockDim.x / 32); ++i) v += red[i];
-  return v;
+  static_assert(kMaxThreads == 256, "eight warps");
+  const float4 a = reinterpret_cast<const float4*>(red)[0], b = reinterpret_cast<const float4*>(red)[1];
+  return ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
 }
 
-// What a row is scaled by before its squares are taken, and 1 / sqrt of their mean and eps.
-struct Rms {
-  float k, rstd;
-};
-constexpr float kFar = 0x1p-100f;
+constexpr float kFar = 0x1p-100f;  // what a row is scaled by where its squares pass f32
 
 struct NormArgs {
   const void* x;
@@ -136,9 +173,11 @@ struct NormArgs {
 
 // T: x's type, TR: the residual's and the sum's.
 template <typename T, typename TR, int OUT, bool WIDE, int C>
-__global__ void __launch_bounds__(kMaxThreads, C == 1 ? 3 : 1) norm_kernel(const NormArgs a) {
-  __shared__ float red[3][2][kMaxThreads / 32];
+__global__ void __launch_bounds__(kMaxThreads, C > 1 ? 1 : sizeof(TR) == 2 && OUT >= kNvOut ? 4 : 3) norm_kernel(const NormArgs a) {
+  __shared__ __align__(16) float red[3][2][kMaxThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x < 3 * 2 * kMaxThreads / 32) (&red[0][0][0])[threadIdx.x] = 0.f;
+  if (!a.per_warp) __syncthreads();
   const int warps = a.per_warp ? 1 : blockDim.x / 32, first = a.per_warp ? 0 : warp;
   const int64_t slot = a.per_warp ? int64_t(blockIdx.x) * (blockDim.x / 32) + warp : blockIdx.x;
   const int64_t slots = a.per_warp ? int64_t(gridDim.x) * (blockDim.x / 32) : gridDim.x;
@@ -164,11 +203,18 @@ __global__ void __launch_bounds__(kMaxThreads, C == 1 ? 3 : 1) norm_kernel(const
     for (int c = 0; c < C; ++c) {
       const int base = (c * warps + first) * 512;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[c][i] = x[c][i / 8].get(i % 8);
+      for (int h = 0; h < 2; ++h) unpack8(x[c][h], v[c] + 8 * h);
       if (a.residual) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[c][i] = to_f32(from_f32<TR>(v[c][i] + r[c][i / 8].get(i % 8)));
-        store_row<TR, WIDE>(static_cast<TR*>(a.sum) + row * a.width, base, lane, a.width, a.vec, v[c]);
+        for (int h = 0; h < 2; ++h) {
+          float add[8];
+          unpack8(r[c][h], add);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) add[i] += v[c][8 * h + i];
+          pack8(r[c][h], add);  // the one rounding, as stored
+          unpack8(r[c][h], v[c] + 8 * h);
+        }
+        store_raw<TR, WIDE>(static_cast<TR*>(a.sum) + row * a.width, base, lane, a.width, a.vec, r[c]);
       }
       float part = 0.f;
 #pragma unroll
@@ -177,30 +223,32 @@ __global__ void __launch_bounds__(kMaxThreads, C == 1 ? 3 : 1) norm_kernel(const
     }
     if (row + slots < a.rows) fetch(row + slots);
     ss = row_sum(ss, a.per_warp, red[0][turn]);
-    Rms n{1.f, 0.f};
+    float eps = a.eps;
     if (!(ss < INFINITY)) {  // too large for f32, or not finite
-      n.k = kFar;
-      ss = 0.f;
+      eps = ss = 0.f;
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) ss = fmaf(v[c][i] * kFar, v[c][i] * kFar, ss);
+        for (int i = 0; i < 16; ++i) {
+          v[c][i] *= kFar;
+          ss = fmaf(v[c][i], v[c][i], ss);
+        }
       ss = row_sum(ss, a.per_warp, red[1][turn]);
     }
-    n.rstd = __frsqrt_rn(__fdiv_rn(ss, float(a.width)) + (n.k == 1.f ? a.eps : 0.f));
+    const float rstd = __frsqrt_rn(__fdiv_rn(ss, float(a.width)) + eps);
     uint32_t top = 0;
+    float mag[C];  // of each piece
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int base = (c * warps + first) * 512;
       float w[16];
       load_weight<T, WIDE>(a.weight, a.w_f32, base, lane, a.width, a.vec, w);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[c][i] = v[c][i] * n.k * n.rstd * w[i];
+      for (int i = 0; i < 16; ++i) v[c][i] = v[c][i] * rstd * w[i];
       if (a.y) store_row<T, WIDE>(static_cast<T*>(a.y) + row * a.width, base, lane, a.width, a.vec, v[c]);
       if constexpr (OUT == kNvOut) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (column<WIDE>(base, lane, i) < a.width) top = max(top, abs_bits(v[c][i]));
+        mag[c] = magnitude16(v[c]);
+        if (base + lane * 16 < a.width) top = max(top, abs_bits(mag[c]));
       }
     }
     if constexpr (OUT == kFp8) {
@@ -246,7 +294,8 @@ __global__ void __launch_bounds__(kMaxThreads, C == 1 ? 3 : 1) norm_kernel(const
         uint32_t* tops = reinterpret_cast<uint32_t*>(red[2][turn]);
         if (lane == 0) tops[warp] = top;
         __syncthreads();
-        for (int i = 0; i < warps; ++i) top = max(top, tops[i]);
+        const uint4 t0 = reinterpret_cast<const uint4*>(tops)[0], t1 = reinterpret_cast<const uint4*>(tops)[1];
+        top = max(max(max(t0.x, t0.y), max(t0.z, t0.w)), max(max(t1.x, t1.y), max(t1.z, t1.w)));
       }
       const float factor = nvfp4_factor(top);
       uint8_t* rec = a.q + row * fp4_stride(kNv, a.width);
@@ -255,7 +304,7 @@ __global__ void __launch_bounds__(kMaxThreads, C == 1 ? 3 : 1) norm_kernel(const
         const int col = (c * warps + first) * 512 + lane * 16;
         if (col >= a.width) continue;
         float unit;
-        const uint32_t s = nvfp4_scale(magnitude16(v[c]), factor, unit);
+        const uint32_t s = nvfp4_scale(mag[c], factor, unit);
         *reinterpret_cast<uint2*>(rec + col / 2) = nvfp4_codes(v[c], unit);
         rec[a.width / 2 + col / 16] = uint8_t(s);
       }
@@ -299,15 +348,21 @@ struct GradArgs {
 // T: x's and grad_y's type, TS: the sum's.
 template <typename T, typename TS, bool WIDE, int C>
 __global__ void __launch_bounds__(kMaxThreads, C == 1 ? 2 : 1) norm_grad_kernel(const GradArgs a) {
-  __shared__ float red[4][kMaxThreads / 32];
+  __shared__ __align__(16) float2 red[2][kMaxThreads / 32];
+  __shared__ __align__(16) float far[2][kMaxThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int warps = a.per_warp ? 1 : blockDim.x / 32, first = a.per_warp ? 0 : warp;
   const int64_t slot = a.per_warp ? int64_t(blockIdx.x) * (blockDim.x / 32) + warp : blockIdx.x;
   const int64_t slots = a.per_warp ? int64_t(gridDim.x) * (blockDim.x / 32) : gridDim.x;
+  if (threadIdx.x < 2 * kMaxThreads / 32) {
+    (&red[0][0])[threadIdx.x] = make_float2(0.f, 0.f);
+    (&far[0][0])[threadIdx.x] = 0.f;
+  }
+  if (!a.per_warp) __syncthreads();
   // 16-bit rows stay as loaded, so that two of them fit in the registers; f32 rows are fetched when their turn comes
   constexpr bool kAhead = C == 1 && sizeof(TS) == 2;
-  float dw[C][16], w[C][16];
-  Vec<TS, 8> rs[C][2], rd[C][2];
+  float dw[C][16];
+  Vec<TS, 8> rs[C][2];
   Vec<T, 8> ry[C][2];
   auto fetch = [&](int64_t row) {
 #pragma unroll
@@ -315,38 +370,46 @@ __global__ void __launch_bounds__(kMaxThreads, C == 1 ? 2 : 1) norm_grad_kernel(
       const int base = (c * warps + first) * 512;
       load_raw<TS, WIDE>(static_cast<const TS*>(a.s) + row * a.s_stride, base, lane, a.width, a.vec, rs[c]);
       load_raw<T, WIDE>(static_cast<const T*>(a.dy) + row * a.dy_stride, base, lane, a.width, a.vec, ry[c]);
-      if (a.ds) load_raw<TS, WIDE>(static_cast<const TS*>(a.ds) + row * a.ds_stride, base, lane, a.width, a.vec, rd[c]);
     }
   };
   pdl_wait();
   pdl_trigger();
   if (kAhead && slot < a.rows) fetch(slot);
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    load_weight<T, WIDE>(a.weight, a.w_f32, (c * warps + first) * 512, lane, a.width, a.vec, w[c]);
+  for (int c = 0; c < C; ++c)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dw[c][i] = 0.f;
-  }
   const float inv_width = __fdiv_rn(1.f, float(a.width));
-  for (int64_t row = slot; row < a.rows; row += slots) {  // the same turns for every thread of a row
+  int turn = 0;
+  for (int64_t row = slot; row < a.rows; row += slots, turn ^= 1) {  // the same turns for every thread of a row
     if (!kAhead) fetch(row);
-    Vec<TS, 8> cs[C][2], cd[C][2];
+    float u[C][16];  // s
+    Vec<TS, 8> cd[C][2];
     Vec<T, 8> cy[C][2];
+    if (a.ds) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)  // wanted behind the sums
+        load_raw<TS, WIDE>(static_cast<const TS*>(a.ds) + row * a.ds_stride, (c * warps + first) * 512, lane, a.width, a.vec,
+                           cd[c]);
+    }
     float ss = 0.f, dot = 0.f;
+    auto weights = [&](int c, float(&w)[16]) {  // from L1 where they are used: registers hold rows on their way
+      load_weight<T, WIDE>(a.weight, a.w_f32, (c * warps + first) * 512, lane, a.width, a.vec, w);
+    };
 #pragma unroll
     for (int c = 0; c < C; ++c) {
+      float w[16], dy[16], part = 0.f, part_dot = 0.f;
+      weights(c, w);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        cs[c][h] = rs[c][h];
-        cd[c][h] = rd[c][h];
+        unpack8(rs[c][h], u[c] + 8 * h);
+        unpack8(ry[c][h], dy + 8 * h);
         cy[c][h] = ry[c][h];
       }
-      float part = 0.f, part_dot = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float v = cs[c][i / 8].get(i % 8);
-        part = fmaf(v, v, part);
-        part_dot = fmaf(cy[c][i / 8].get(i % 8) * w[c][i], v, part_dot);
+        part = fmaf(u[c][i], u[c][i], part);
+        part_dot = fmaf(dy[i] * w[i], u[c][i], part_dot);
       }
       ss += part;
       dot += part_dot;
@@ -356,30 +419,22 @@ __global__ void __launch_bounds__(kMaxThreads, C == 1 ? 2 : 1) norm_grad_kernel(
     ss = warp_sum(ss);
     dot = warp_sum(dot);
     if (!a.per_warp) {
-      const int turn = int((row - slot) / slots) & 1;
-      if (lane == 0) {
-        red[turn][warp] = ss;
-        red[2 + turn][warp] = dot;
-      }
+      if (lane == 0) red[turn][warp] = make_float2(ss, dot);
       __syncthreads();
-      ss = dot = 0.f;
-      for (int i = 0; i < warps; ++i) {
-        ss += red[turn][i];
-        dot += red[2 + turn][i];
-      }
+      static_assert(kMaxThreads == 256, "eight warps");
+      const float4* r = reinterpret_cast<const float4*>(red[turn]);
+      const float4 r0 = r[0], r1 = r[1], r2 = r[2], r3 = r[3];
+      ss = ((r0.x + r0.z) + (r1.x + r1.z)) + ((r2.x + r2.z) + (r3.x + r3.z));
+      dot = ((r0.y + r0.w) + (r1.y + r1.w)) + ((r2.y + r2.w) + (r3.y + r3.w));
     }
     float k = 1.f, rstd = __frsqrt_rn(__fmul_rn(ss, inv_width) + a.eps);
     float mean = dot * rstd * inv_width;  // of g u
     if (!(ss < INFINITY) || !(fabsf(dot) < INFINITY)) {
-      __shared__ float far[2][kMaxThreads / 32];
       float s2 = 0.f;
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float v = cs[c][i / 8].get(i % 8) * kFar;
-          s2 = fmaf(v, v, s2);
-        }
+        for (int i = 0; i < 16; ++i) s2 = fmaf(u[c][i] * kFar, u[c][i] * kFar, s2);
       if (!a.per_warp) __syncthreads();  // the places' last readers
       s2 = row_sum(s2, a.per_warp, far[0]);
       if (!(ss < INFINITY)) {
@@ -388,21 +443,40 @@ __global__ void __launch_bounds__(kMaxThreads, C == 1 ? 2 : 1) norm_grad_kernel(
       }
       dot = 0.f;
 #pragma unroll
+      for (int c = 0; c < C; ++c) {
+        float w[16], dy[16];
+        weights(c, w);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) unpack8(cy[c][h], dy + 8 * h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dot = fmaf(dy[i] * w[i], u[c][i] * k * rstd, dot);
+      }
+      mean = row_sum(dot, a.per_warp, far[1]) * inv_width;
+#pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          dot = fmaf(cy[c][i / 8].get(i % 8) * w[c][i], cs[c][i / 8].get(i % 8) * k * rstd, dot);
-      mean = row_sum(dot, a.per_warp, far[1]) * inv_width;
+        for (int i = 0; i < 16; ++i) u[c][i] *= k;
     }
+    const float scale = rstd * k;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int base = (c * warps + first) * 512;
-      float d[16];
+      float d[16], dy[16], w[16];
+      weights(c, w);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) unpack8(cy[c][h], dy + 8 * h);
+      if (a.ds) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) unpack8(cd[c][h], d + 8 * h);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) d[i] = 0.f;
+      }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float u = cs[c][i / 8].get(i % 8) * k * rstd, dy = cy[c][i / 8].get(i % 8);
-        dw[c][i] = fmaf(dy, u, dw[c][i]);
-        d[i] = fmaf(rstd * k, dy * w[c][i] - u * mean, a.ds ? cd[c][i / 8].get(i % 8) : 0.f);
+        const float n = u[c][i] * rstd;
+        dw[c][i] = fmaf(dy[i], n, dw[c][i]);
+        d[i] = fmaf(scale, fmaf(-n, mean, dy[i] * w[i]), d[i]);
       }
       if (a.grad_sum) store_row<TS, WIDE>(static_cast<TS*>(a.grad_sum) + row * a.width, base, lane, a.width, a.vec, d);
       if (a.grad_x) store_row<T, WIDE>(static_cast<T*>(a.grad_x) + row * a.width, base, lane, a.width, a.vec, d);
@@ -490,7 +564,7 @@ cudaError_t run_out(cudaStream_t s, const NormArgs& a, const Shape& sh, int out)
 // CTAs of a gradient's walk, at most one per row: their number fixes the order of the weight's gradient and its
 // workspace, so it goes by sizes alone and not by what runs at once.
 int64_t grad_grid(int rows, const Shape& sh) {
-  const int64_t per_sm = std::max(1, kGradThreads / sh.threads);
+  const int64_t per_sm = std::max(1, 512 / sh.threads);
   const int64_t rows_per_cta = sh.per_warp ? sh.threads / 32 : 1;
   return std::min<int64_t>((rows + rows_per_cta - 1) / rows_per_cta, per_sm * sm_count());
 }

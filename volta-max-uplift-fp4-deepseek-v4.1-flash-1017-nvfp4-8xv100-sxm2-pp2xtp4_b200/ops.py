@@ -1,4 +1,4 @@
-"""What the stateless operators (``permute``, ``fp8``) share: their binding and the
+"""What the stateless operators (``permute``, ``fp8``, ``fp4``, ``norm``) share: their binding and the
 device's operator error word.
 
 Gradients are of first order and reverse mode: a second differentiation and a tensor
