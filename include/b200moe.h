@@ -438,7 +438,7 @@ int b200moe_fp4_quantize_weight(void* stream, const void* w, int dtype, int mats
                                 void* scale, float* factor);
 /* What codes, scales and factors (NULL: 1) stand for: out [rows][k] = value *
  * scale * factor, rounded once.  ld_*: bytes between rows (ld_factor 0: one factor
- * for all); codes on 8 bytes, ld_codes a multiple of 8. */
+ * for all); codes and factors on 4 bytes, out on 16. */
 int b200moe_fp4_values(void* stream, const void* codes, int64_t ld_codes, const void* scale, int64_t ld_scale,
                        const void* factor, int64_t ld_factor, int64_t rows, int k, int format, void* out, int dtype);
 /* out [S][N] = records a [S] . w^T with scales and factors, f32 sums: w [E][N][K / 2]

@@ -2,8 +2,8 @@
 // fused in front of the rows' quantizer, and the values that records stand for.
 //
 // A thread holds 16 columns.  NVFP4 needs the row's maximum before its first
-// code: a CTA (up to 512 columns a warp) holds a row in registers, so that it is
-// read once; longer rows than a CTA holds are read twice.  MXFP4's blocks stand
+// code: a CTA or, of many rows, a warp holds a row in registers, so that it is read
+// once; longer rows than a CTA holds are read twice.  MXFP4's blocks stand
 // alone and take two threads each, whatever their row.
 // Bound: HBM for rows as they are, instruction issue for the SwiGLU.
 #include <algorithm>
@@ -41,33 +41,70 @@ struct Piece {
   }
 };
 
-// A walk over rows, a row per CTA, or per warp (blockDim.x / 32 of them) where per_warp is set. Where the row's threads
-// hold all of it (once), the next row is on its way while this one is worked on.
+// A warp per row, its columns in registers as N pieces of 16 a lane: no barrier, for as many rows as keep the GPU's warps
+// busy.
+template <typename T, bool SWIGLU, bool WIDE, int N>
+__global__ void __launch_bounds__(256, N <= 3 ? 3 : 2) nvfp4_warp_rows_kernel(const T* __restrict__ x, int64_t x_stride, int rows,
+                                                                            int width, float limit,
+                                                                            uint8_t* __restrict__ out) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  pdl_wait();
+  pdl_trigger();
+  if (row >= rows) return;
+  const int pieces = width / 16;
+  float v[N][16], mag[N];
+  uint32_t m = 0;
+  Piece<T, SWIGLU, WIDE> raw[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    if (lane + 32 * n < pieces) raw[n].load(x + row * x_stride, (lane + 32 * n) * 16, width);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    if (lane + 32 * n >= pieces) continue;
+    raw[n].values(limit, v[n]);
+    mag[n] = magnitude16(v[n]);
+    m = max(m, abs_bits(mag[n]));
+  }
+  const float factor = nvfp4_factor(__reduce_max_sync(0xffffffffu, m));
+  uint8_t* rec = out + row * fp4_stride(kNv, width);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int p = lane + 32 * n;
+    if (p >= pieces) continue;
+    float unit;
+    const uint32_t s = nvfp4_scale(mag[n], factor, unit);
+    *reinterpret_cast<uint2*>(rec + p * 8) = nvfp4_codes(v[n], unit);
+    rec[width / 2 + p] = uint8_t(s);
+  }
+  if (lane == 0) finish_record(rec, kNv, width, factor);
+}
+
+// A CTA walks rows. Where its threads hold all of a row (once), the next row is on its way while this one is worked on.
 template <typename T, bool SWIGLU, bool WIDE>
-__global__ void __launch_bounds__(kMaxRowThreads) nvfp4_rows_kernel(const T* __restrict__ x, int64_t x_stride, int rows,
-                                                                    int width, float limit, int per_warp,
+__global__ void __launch_bounds__(kMaxRowThreads, sizeof(T) == 2 ? 2 : 1) nvfp4_rows_kernel(const T* __restrict__ x, int64_t x_stride, int rows,
+                                                                    int width, float limit,
                                                                     uint8_t* __restrict__ out) {
   __shared__ uint32_t warp_max[2][kMaxRowThreads / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int tid = per_warp ? lane : threadIdx.x, threads = per_warp ? 32 : blockDim.x;
-  const int64_t slot = per_warp ? int64_t(blockIdx.x) * (blockDim.x / 32) + warp : blockIdx.x;
-  const int64_t slots = per_warp ? int64_t(gridDim.x) * (blockDim.x / 32) : gridDim.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x, threads = blockDim.x;
   const int pieces = width / 16;
   const bool once = pieces <= threads, in = tid < pieces;
   pdl_wait();
   pdl_trigger();
+  constexpr bool kAhead = !SWIGLU;  // what the SwiGLU wants is warps
   Piece<T, SWIGLU, WIDE> next;
-  if (once && in && slot < rows) next.load(x + slot * x_stride, tid * 16, width);
+  if (kAhead && once && in && blockIdx.x < rows) next.load(x + blockIdx.x * x_stride, tid * 16, width);
   int turn = 0;
-  for (int64_t row = slot; row < rows; row += slots, turn ^= 1) {
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
     const T* src = x + row * x_stride;
     float v[16], top = 0.f;
     uint32_t m = 0;
     if (once) {
       if (in) {
+        if (!kAhead) next.load(src, tid * 16, width);
         next.values(limit, v);
         top = magnitude16(v);
-        if (row + slots < rows) next.load(src + slots * x_stride, tid * 16, width);
+        if (kAhead && row + gridDim.x < rows) next.load(src + gridDim.x * x_stride, tid * 16, width);
       }
       m = abs_bits(top);
     } else {
@@ -78,11 +115,9 @@ __global__ void __launch_bounds__(kMaxRowThreads) nvfp4_rows_kernel(const T* __r
       }
     }
     m = __reduce_max_sync(0xffffffffu, m);
-    if (!per_warp) {  // the places are those of the row before last, which every thread has read
-      if (lane == 0) warp_max[turn][warp] = m;
-      __syncthreads();
-      for (int i = 0; i < int(blockDim.x / 32); ++i) m = max(m, warp_max[turn][i]);
-    }
+    if (lane == 0) warp_max[turn][warp] = m;  // the places are those of the row before last, which every thread has read
+    __syncthreads();
+    for (int i = 0; i < threads / 32; ++i) m = max(m, warp_max[turn][i]);
     const float factor = nvfp4_factor(m);
     uint8_t* rec = out + row * fp4_stride(kNv, width);
     for (int p = tid; p < pieces; p += threads) {
@@ -179,37 +214,54 @@ __global__ void __launch_bounds__(256) fp4_weight_kernel(const T* __restrict__ w
 }
 
 // ---------------------------------------------------------------- read back
-// A thread per 32 columns: value * scale (exact in f32, and in f16 for NVFP4) * factor, rounded once.
+// Pieces of 8 columns, neighbouring threads' side by side, four of a thread's in flight: value * scale (exact) * factor,
+// rounded once.  d_row, d_piece: the grid's step over rows of width / 8 pieces.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) fp4_values_kernel(const uint8_t* __restrict__ codes, int64_t ld_codes,
                                                          const uint8_t* __restrict__ scale, int64_t ld_scale,
                                                          const uint8_t* __restrict__ factor, int64_t ld_factor,
-                                                         int64_t rows, int width, T* __restrict__ out) {
-  const int pieces = width / 32;
-  const int64_t total = rows * pieces, step = int64_t(gridDim.x) * 256;
+                                                         int64_t rows, int width, int64_t d_row, int d_piece,
+                                                         T* __restrict__ out) {
+  constexpr int U = 4;
+  const int pieces = width / 8;
+  const int64_t first = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  int64_t row = first / pieces;
+  int p = int(first - row * pieces);
   pdl_wait();
   pdl_trigger();
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += step) {
-    const int64_t row = i <= INT32_MAX ? int64_t(uint32_t(i) / uint32_t(pieces)) : i / pieces;
-    const int p = int(i - row * pieces);
-    const uint4 c = __ldg(reinterpret_cast<const uint4*>(codes + row * ld_codes) + p);
-    const uint8_t* sp = scale + row * ld_scale + (FMT == kMx ? p : 2 * p);
-    const float f = factor ? __ldg(reinterpret_cast<const float*>(factor + row * ld_factor)) : 1.f;
-    const uint32_t s0 = __ldg(sp), s1 = FMT == kMx ? s0 : __ldg(sp + 1);
-    const float m0 = FMT == kMx ? e8m0_f32(s0) : e4m3_f32(s0), m1 = FMT == kMx ? m0 : e4m3_f32(s1);
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  while (row < rows) {
+    uint32_t w[U], sb[U];
+    float f[U];
+    int64_t at[U];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float m = j < 2 ? m0 : m1;
-      const uint32_t h[4] = {e2m1x2_byte<0>(w[j]), e2m1x2_byte<1>(w[j]), e2m1x2_byte<2>(w[j]), e2m1x2_byte<3>(w[j])};
+    for (int u = 0; u < U; ++u) {
+      at[u] = -1;
+      if (row < rows) {
+        at[u] = row * pieces + p;
+        w[u] = __ldg(reinterpret_cast<const uint32_t*>(codes + row * ld_codes) + p);
+        sb[u] = __ldg(scale + row * ld_scale + p / (FMT == kMx ? 4 : 2));
+        f[u] = factor ? __ldg(reinterpret_cast<const float*>(factor + row * ld_factor)) : 1.f;
+      }
+      row += d_row;
+      p += d_piece;
+      if (p >= pieces) {
+        p -= pieces;
+        ++row;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (at[u] < 0) break;
+      const float m = FMT == kMx ? e8m0_f32(sb[u]) : e4m3_f32(sb[u]);
+      const uint32_t h[4] = {e2m1x2_byte<0>(w[u]), e2m1x2_byte<1>(w[u]), e2m1x2_byte<2>(w[u]), e2m1x2_byte<3>(w[u])};
       float v[8];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
-        v[2 * k] = q.x * m * f;
-        v[2 * k + 1] = q.y * m * f;
+        v[2 * k] = q.x * m * f[u];
+        v[2 * k + 1] = q.y * m * f[u];
       }
-      store_vec<T, 8>(out + i * 32 + j * 8, v);
+      store_vec<T, 8>(out + at[u] * 8, v);
     }
   }
 }
@@ -234,12 +286,26 @@ cudaError_t run_rows(cudaStream_t s, int fmt, const void* x, int64_t x_stride, i
     return launch_chain(kernel, dim3(grid_of(int64_t(rows) * (width / 16))), dim3(256), 0, s, src, x_stride, rows, width,
                         limit, out);
   }
-  const int pieces = width / 16, per_warp = pieces <= 32;
-  const int threads = per_warp ? 256 : std::min(kMaxRowThreads, (pieces + 31) / 32 * 32);
+  // a warp per row where all of a row's pieces fit its lanes' registers and every SM gets eight rows, or a row fits one
+  // piece per lane: SwiGLU of 49152 x 1408 takes 132 us with a CTA per row
+  const int pieces = width / 16, per_lane = (pieces + 31) / 32;
+  if (per_lane == 1 || (per_lane <= 4 && rows >= 8 * sm_count())) {
+    auto go = [&](auto kernel) {
+      return launch_chain(kernel, dim3(unsigned((int64_t(rows) + 7) / 8)), dim3(256), 0, s, src, x_stride, rows, width, limit, out);
+    };
+    if (per_lane == 1)
+      return wide ? go(nvfp4_warp_rows_kernel<T, SWIGLU, true, 1>) : go(nvfp4_warp_rows_kernel<T, SWIGLU, false, 1>);
+    if (per_lane == 2)
+      return wide ? go(nvfp4_warp_rows_kernel<T, SWIGLU, true, 2>) : go(nvfp4_warp_rows_kernel<T, SWIGLU, false, 2>);
+    if (per_lane == 3)
+      return wide ? go(nvfp4_warp_rows_kernel<T, SWIGLU, true, 3>) : go(nvfp4_warp_rows_kernel<T, SWIGLU, false, 3>);
+    return wide ? go(nvfp4_warp_rows_kernel<T, SWIGLU, true, 4>) : go(nvfp4_warp_rows_kernel<T, SWIGLU, false, 4>);
+  }
+  const int threads = std::min(kMaxRowThreads, (pieces + 31) / 32 * 32);
   auto kernel = wide ? nvfp4_rows_kernel<T, SWIGLU, true> : nvfp4_rows_kernel<T, SWIGLU, false>;
   static Residents residents[2];  // by kernel
-  const int64_t grid = std::min<int64_t>(per_warp ? (int64_t(rows) + 7) / 8 : rows, residents[wide].ctas(kernel, threads));
-  return launch_chain(kernel, dim3(unsigned(grid)), dim3(threads), 0, s, src, x_stride, rows, width, limit, per_warp, out);
+  const int64_t grid = std::min<int64_t>(rows, residents[wide].ctas(kernel, threads));
+  return launch_chain(kernel, dim3(unsigned(grid)), dim3(threads), 0, s, src, x_stride, rows, width, limit, out);
 }
 
 template <typename T>
@@ -266,8 +332,11 @@ template <typename T>
 cudaError_t run_values(cudaStream_t s, int fmt, const uint8_t* codes, int64_t ld_codes, const uint8_t* scale,
                        int64_t ld_scale, const uint8_t* factor, int64_t ld_factor, int64_t rows, int width, void* out) {
   auto kernel = fmt == kMx ? fp4_values_kernel<T, kMx> : fp4_values_kernel<T, kNv>;
-  return launch_chain(kernel, dim3(grid_of(rows * (width / 32))), dim3(256), 0, s, codes, ld_codes, scale, ld_scale,
-                      factor, ld_factor, rows, width, static_cast<T*>(out));
+  const int pieces = width / 8;
+  const unsigned grid = grid_of((rows * pieces + 3) / 4);
+  const int64_t step = int64_t(grid) * 256;
+  return launch_chain(kernel, dim3(grid), dim3(256), 0, s, codes, ld_codes, scale, ld_scale, factor, ld_factor, rows, width,
+                      step / pieces, int(step % pieces), static_cast<T*>(out));
 }
 
 bool bad_format(int fmt) { return fmt != kNv && fmt != kMx; }
@@ -313,7 +382,7 @@ extern "C" int b200moe_fp4_values(void* stream, const void* codes, int64_t ld_co
       ld_factor < 0)
     return B200MOE_ERR_INVALID_ARG;
   if (dtype < 0 || dtype > B200MOE_F32) return B200MOE_ERR_DTYPE;
-  if (!on(codes, 16) || ld_codes % 16 || !on(factor, 4) || ld_factor % 4 || !on(out, 16)) return B200MOE_ERR_ALIGN;
+  if (!on(codes, 4) || ld_codes % 4 || !on(factor, 4) || ld_factor % 4 || !on(out, 16)) return B200MOE_ERR_ALIGN;
   auto run = dtype == B200MOE_F16 ? run_values<__half> : dtype == B200MOE_BF16 ? run_values<__nv_bfloat16>
                                                                                : run_values<float>;
   return status(run(static_cast<cudaStream_t>(stream), format, static_cast<const uint8_t*>(codes), ld_codes,

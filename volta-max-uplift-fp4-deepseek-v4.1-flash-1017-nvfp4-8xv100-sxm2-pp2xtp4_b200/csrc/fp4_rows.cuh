@@ -104,11 +104,11 @@ __device__ __forceinline__ uint2 nvfp4_codes(const float (&v)[16], float unit) {
   return o;
 }
 
-// 16 of the 32 values of an MXFP4 block (inv 0: a block without values of its own).
+// 16 of the 32 values of an MXFP4 block (inv 0: a block whose scale is a NaN, whatever its codes).
 __device__ __forceinline__ uint2 mxfp4_codes(const float (&v)[16], float inv) {
   float t[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) t[i] = inv > 0.f ? v[i] * inv : 0.f;
+  for (int i = 0; i < 16; ++i) t[i] = v[i] * inv;
   return make_uint2(e2m1x8(t), e2m1x8(t + 8));
 }
 
@@ -121,8 +121,12 @@ __device__ __forceinline__ float magnitude16(const float (&v)[16]) {
 
 // The bytes of a record behind its scales: zeros, and the factor.
 __device__ __forceinline__ void finish_record(uint8_t* rec, int fmt, int K, float factor) {
-  const int end = fp4_stride(fmt, K);
-  for (int i = K / 2 + K / fp4_block(fmt); i < end; ++i) rec[i] = 0;
+  const int begin = K / 2 + K / fp4_block(fmt), end = fp4_stride(fmt, K);
+  if (fmt == kNv && begin % 16 == 0) {  // K a multiple of 256
+    *reinterpret_cast<uint4*>(rec + begin) = make_uint4(__float_as_uint(factor), 0u, 0u, 0u);
+    return;
+  }
+  for (int i = begin; i < end; ++i) rec[i] = 0;
   if (fmt == kNv) *reinterpret_cast<float*>(rec + fp4_factor_at(K)) = factor;
 }
 

@@ -173,7 +173,7 @@ struct NormArgs {
 
 // T: x's type, TR: the residual's and the sum's.
 template <typename T, typename TR, int OUT, bool WIDE, int C>
-__global__ void __launch_bounds__(kMaxThreads, C > 1 ? 1 : sizeof(TR) == 2 && OUT >= kNvOut ? 4 : 3) norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kMaxThreads, C > 1 ? 1 : sizeof(TR) == 2 && OUT > kNvOut ? 4 : 3) norm_kernel(const NormArgs a) {
   __shared__ __align__(16) float red[3][2][kMaxThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x < 3 * 2 * kMaxThreads / 32) (&red[0][0][0])[threadIdx.x] = 0.f;
