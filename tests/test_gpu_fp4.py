@@ -346,6 +346,37 @@ def test_graph_replay_and_another_stream(ops, m):
     assert torch.equal(y, ops.fp4.linear(x, w)) and not torch.equal(y, want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_past_32_bit_offsets(ops, fmt):
+    """Rows whose records, and whose own values, pass 4 GB: the last ones as by a call of their own."""
+    m, k = 2_000_001, 4096
+    x = torch.empty(m, k, device="cuda", dtype=torch.bfloat16)
+    x[:64], x[-64:] = randn(1, 64, k), randn(2, 64, k)
+    x[64:-64] = 0.0
+    w = ops.fp4.quantize_weight(randn(3, 32, k) * 0.02, fmt)
+    rows = ops.fp4.quantize(x, fmt)
+    del x
+    assert rows.record.numel() > 2**32
+    y = ops.fp4.matmul(rows, w)
+    for s in (slice(0, 64), slice(m - 64, m)):
+        part = rows._replace(record=rows.record[s].clone())
+        assert torch.equal(part.record, ops.fp4.quantize(randn(1 if s.start == 0 else 2, 64, k, dtype=torch.bfloat16), fmt).record)
+        check_product(y[s], row_values(part), weight_values(w))
+        assert torch.equal(ops.fp4.dequantize(rows)[s], ops.fp4.dequantize(part))
+    assert not y[64:-64].any()
+
+
+@pytest.mark.gpu
+def test_mxfp4_scales_of_any_size(ops):
+    """Rows near the ends of f32's range times ordinary weights, by each kernel; results within its normal range."""
+    w = ops.fp4.quantize_weight(randn(1, 300, 256), "mxfp4")
+    for m in (1, 40, 300):
+        for size in (2.0**-110, 2.0**100):
+            rows = ops.fp4.quantize(randn(m, m, 256) * size, "mxfp4")
+            check_product(ops.fp4.matmul(rows, w, torch.float32), row_values(rows), weight_values(w))
+
+
 # -------------------------------------------------------------------- refusals
 @pytest.mark.gpu
 def test_refusals(ops):

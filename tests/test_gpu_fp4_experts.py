@@ -93,6 +93,13 @@ def test_rows_and_their_quantized_form_give_the_same(ops, fmt):
 
 
 @pytest.mark.gpu
+def test_no_tokens(ops):
+    layer = ops.experts.Fp4Experts.from_weights(randn(1, 4, 128, 64), randn(2, 4, 64, 64))
+    ids, weights = torch.empty(0, 2, dtype=torch.int32, device="cuda"), torch.empty(0, 2, device="cuda")
+    assert layer(torch.empty(0, 64, device="cuda", dtype=torch.bfloat16), ids, weights).shape == (0, 64)
+
+
+@pytest.mark.gpu
 def test_captured_and_replayed(ops):
     layer = ops.experts.Fp4Experts.from_weights(randn(1, 8, 256, 256) / 16, randn(2, 8, 256, 128) / 11)
     x, r, gain = randn(3, 5, 256, dtype=torch.bfloat16), randn(4, 5, 256, dtype=torch.bfloat16), torch.ones(256, device="cuda")

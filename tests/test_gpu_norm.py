@@ -233,6 +233,39 @@ def test_empty_and_refused(ops):
 
 
 @pytest.mark.gpu
+def test_past_32_bit_offsets(ops):
+    """More than 2^31 values: the last rows as by a call of their own, the weight's gradient as of the rows that count."""
+    m, h = 540_001, 4096
+    x, r = torch.zeros(m, h, device="cuda", dtype=torch.bfloat16), torch.zeros(m, h, device="cuda", dtype=torch.bfloat16)
+    tail = slice(m - 40, m)
+    x[tail], r[tail] = randn(1, 40, h), randn(2, 40, h)
+    w = 1 + 0.1 * randn(3, h)
+    y, total = ops.norm.rms_norm(x, w, r)
+    want = ops.norm.rms_norm(x[tail], w, r[tail])
+    assert torch.equal(y[tail], want.y) and torch.equal(total[tail], want.sum) and not y[:-40].any()
+    q = ops.norm.rms_norm_quantize(x, w, r, format="nvfp4").rows.record
+    assert torch.equal(q[tail], ops.norm.rms_norm_quantize(x[tail], w, r[tail], format="nvfp4").rows.record)
+    del q, y
+    gx, _, gw = ops.norm.rms_norm_grad(total, x, w, r)
+    wx, _, ww = ops.norm.rms_norm_grad(total[tail], x[tail], w, r[tail])
+    assert torch.equal(gx[tail], wx)
+    _, rstd = formula(total[tail], w)
+    mag = (x[tail].double() * total[tail].double() * rstd).abs().sum(0)
+    within(gw, ww.double(), mag * 2.0**-18)
+
+
+@pytest.mark.gpu
+def test_leaves_get_gradients_of_their_own(ops):
+    x, r, w = (t.requires_grad_() for t in inputs(6, 64, torch.bfloat16, "same", False))
+    y, total = ops.norm.rms_norm(x, w, r)
+    (y.float().sum() + total.float().sum()).backward()
+    assert torch.equal(x.grad, r.grad) and x.grad.data_ptr() != r.grad.data_ptr()
+    both = x.detach().clone().requires_grad_()  # the same tensor twice
+    ops.norm.rms_norm(both, w, both).sum.float().sum().backward()
+    assert torch.equal(both.grad, torch.full_like(both, 2.0))
+
+
+@pytest.mark.gpu
 def test_graph_replay(ops):
     x, r, w = inputs(130, 2048, torch.bfloat16, "same", False)
     g = torch.cuda.CUDAGraph()

@@ -165,14 +165,32 @@ __global__ void __launch_bounds__(256) mxfp4_rows_kernel(const T* __restrict__ x
 }
 
 // ------------------------------------------------------------------ weights
-// Largest magnitude of each matrix, as bits, into its factor's place (zero before).
+// Sixteen values from p: by vectors where every address allows it.
 template <typename T>
-__global__ void __launch_bounds__(256) fp4_weight_max_kernel(const T* __restrict__ w, int64_t n, uint32_t* __restrict__ top) {
-  const T* src = w + int64_t(blockIdx.y) * n;
+__device__ __forceinline__ void load16(const T* p, int vec, float (&v)[16]) {
+  Vec<T, 16> x;
+  if (vec) {
+    x.load(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x.v[i] = p[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = x.get(i);
+}
+
+// Largest magnitude of each matrix, as bits, into its factor's place (zero before).  n: its pieces of 16.
+template <typename T>
+__global__ void __launch_bounds__(256) fp4_weight_max_kernel(const T* __restrict__ w, int64_t n, int vec,
+                                                             uint32_t* __restrict__ top) {
+  const T* src = w + int64_t(blockIdx.y) * n * 16;
   uint32_t m = 0;
   pdl_wait();
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256)
-    m = max(m, abs_bits(to_f32(src[i])));
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
+    float v[16];
+    load16(src + i * 16, vec, v);
+    m = max(m, abs_bits(magnitude16(v)));
+  }
   m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0 && m) atomicMax(top + blockIdx.y, m);  // a maximum: any order gives the same
   pdl_trigger();
@@ -185,7 +203,7 @@ __global__ void fp4_weight_factor_kernel(uint32_t* top, int mats) {
 
 // A thread per 16 columns of any matrix; codes and scales in arrays of their own.
 template <typename T, int FMT>
-__global__ void __launch_bounds__(256) fp4_weight_kernel(const T* __restrict__ w, int64_t per_mat, int64_t total,
+__global__ void __launch_bounds__(256) fp4_weight_kernel(const T* __restrict__ w, int64_t per_mat, int64_t total, int vec,
                                                          const float* __restrict__ factor, uint8_t* __restrict__ codes,
                                                          uint8_t* __restrict__ scale) {
   pdl_wait();
@@ -193,10 +211,11 @@ __global__ void __launch_bounds__(256) fp4_weight_kernel(const T* __restrict__ w
   const int64_t step = int64_t(gridDim.x) * 256;
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; __any_sync(0xffffffffu, i < total); i += step) {
     const bool in = i < total;
-    float v[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = in ? to_f32(w[i * 16 + j]) : 0.f;
-    float m = magnitude16(v);
+    float v[16], m = 0.f;
+    if (in) {
+      load16(w + i * 16, vec, v);
+      m = magnitude16(v);
+    }
     if constexpr (FMT == kMx) {
       float inv;
       m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
@@ -313,17 +332,18 @@ cudaError_t run_weight(cudaStream_t s, int fmt, const void* w, int mats, int64_t
                        float* factor) {
   const T* src = static_cast<const T*>(w);
   const int64_t total = mats * (n / 16);
+  const int vec = on(w, 16);
   if (fmt == kMx)
-    return launch_chain(fp4_weight_kernel<T, kMx>, dim3(grid_of(total)), dim3(256), 0, s, src, n / 16, total,
+    return launch_chain(fp4_weight_kernel<T, kMx>, dim3(grid_of(total)), dim3(256), 0, s, src, n / 16, total, vec,
                         static_cast<const float*>(nullptr), codes, scale);
   cudaError_t e = cudaMemsetAsync(factor, 0, mats * sizeof(float), s);
   uint32_t* top = reinterpret_cast<uint32_t*>(factor);
-  const unsigned per = unsigned(std::min<int64_t>((n + 4095) / 4096, std::max(1, sm_count() * 8 / mats)));
+  const unsigned per = unsigned(std::min<int64_t>((n + 4095) / 4096, std::max(1, sm_count() * 16 / mats)));
   if (e == cudaSuccess)
-    e = launch_chain(fp4_weight_max_kernel<T>, dim3(per, mats), dim3(256), 0, s, src, n, top);
+    e = launch_chain(fp4_weight_max_kernel<T>, dim3(per, mats), dim3(256), 0, s, src, n / 16, vec, top);
   if (e == cudaSuccess) e = launch_chain(fp4_weight_factor_kernel, dim3(1), dim3(256), 0, s, top, mats);
   if (e == cudaSuccess)
-    e = launch_chain(fp4_weight_kernel<T, kNv>, dim3(grid_of(total)), dim3(256), 0, s, src, n / 16, total,
+    e = launch_chain(fp4_weight_kernel<T, kNv>, dim3(grid_of(total)), dim3(256), 0, s, src, n / 16, total, vec,
                      static_cast<const float*>(factor), codes, scale);
   return e;
 }

@@ -55,5 +55,6 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
 def rms_norm_grad(s: torch.Tensor, grad_y: torch.Tensor, weight: torch.Tensor, grad_sum: torch.Tensor | None = None,
                   eps: float = 1e-6, need_x: bool = True, need_residual: bool = True, need_weight: bool = True):
     """Gradients of ``rms_norm`` in x (``grad_y``'s type), residual (``s``'s type) and weight, None where not
-    needed; ``s``: the stored sum, or x where there was no residual."""
+    needed (one tensor for x and residual where they have one type); ``s``: the stored sum, or x where
+    there was no residual."""
     return _lib.ops().rms_norm_grad(s, grad_y, grad_sum, weight, eps, need_x, need_residual, need_weight)
