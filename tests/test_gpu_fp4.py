@@ -257,6 +257,24 @@ def test_linear_types_and_strides(ops, dtype, m):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", [1, 3, 20, 300, 2500])
+@pytest.mark.parametrize("k", [32, 96, 352, 512, 1408])
+def test_weight_scales_at_any_address(ops, fmt, m, k):
+    """Scales behind 1, 2, 4 or 8 bytes of something else, which must not be taken for theirs."""
+    w = ops.fp4.quantize_weight(randn(k, 700, k) * 0.05, fmt)
+    rows = ops.fp4.quantize(randn(m, m, k), fmt)
+    want = ops.fp4.matmul(rows, w, torch.float32)
+    check_product(want, row_values(rows), weight_values(w))
+    for at in (1, 2, 4, 8):
+        room = torch.full((w.scale.numel() + at + 16,), 255, dtype=torch.uint8, device="cuda")
+        scale = room[at: at + w.scale.numel()].view(w.scale.shape)
+        scale.copy_(w.scale)
+        assert torch.equal(ops.fp4.matmul(rows, w._replace(scale=scale), torch.float32), want) or m <= 8
+        check_product(ops.fp4.matmul(rows, w._replace(scale=scale), torch.float32), row_values(rows), weight_values(w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("counts,tail,n,k", [
     ([1], 0, 128, 64), ([0, 3, 0, 17, 1, 0], 5, 200, 96), ([40, 0, 33, 64, 65], 0, 333, 352), ([1] * 300, 0, 256, 256),
     ([200, 0, 129, 1, 300], 7, 512, 640), ([5000, 1, 0, 700], 0, 2816, 288), ([0, 0, 0], 9, 130, 64),
@@ -327,7 +345,7 @@ def test_offsets_out_of_range_are_reported(ops, pkg):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m", [1, 40, 500])
+@pytest.mark.parametrize("m", [1, 40, 500, 5000])
 def test_graph_replay_and_another_stream(ops, m):
     w = ops.fp4.quantize_weight(randn(1, 512, 1024) * 0.02)
     x = randn(m, m, 1024, dtype=torch.bfloat16)

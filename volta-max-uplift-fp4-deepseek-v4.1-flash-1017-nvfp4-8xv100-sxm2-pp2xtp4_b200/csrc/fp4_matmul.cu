@@ -98,6 +98,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_kernel(const TileArgs a, cons
                  "r"(uint32_t(C::kTmem)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  if (threadIdx.x == 0) prefetch_maps(maps, w_chunks, a.copy_out);
   fence_before();
   __syncthreads();
   fence_after();
@@ -217,12 +218,15 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_kernel(const TileArgs a, cons
             out[int64_t(row0 + i) * a.N + col] = from_f32<TO>(__uint_as_float(p[i / 16][i % 16]) * f * fw);
         }
       } else {
+        constexpr int kTileOut = 32 * BN * int(sizeof(TO));  // of a warp
+        static_assert(4 * kTileOut <= ST * C::kStage, "the last tile's room");
         const float fa = row_factor(a, row0 + quarter * 32 + lane);
         ok = poll_warp(&acc_full[b], (tile >> 1) & 1, a.err);
         if (!ok) break;
         fence_after();
-        store_tile<BN, TO>(a, &maps.out, acc, stage_out + quarter * kOutBytes, row0 + quarter * 32, end, col0, fa, fw, 0,
-                           BN / 32, [&] { mbar_arrive(&acc_empty[b]); });
+        const bool last = tiles.next(item) >= tiles.stop();
+        store_tile<BN, TO>(a, &maps.out, acc, last ? stages + quarter * kTileOut : stage_out + quarter * kOutBytes,
+                           row0 + quarter * 32, end, col0, fa, fw, 0, BN / 32, last, [&] { mbar_arrive(&acc_empty[b]); });
       }
     }
     if (!ok) *abort_ptr = 1;

@@ -164,6 +164,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                  "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
+  if (threadIdx.x == 0) prefetch_maps(maps, w_chunks, a.copy_out);
   fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs' barriers stand before either arrives at the other's
@@ -264,8 +265,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       fence_after();
       const uint32_t bar = even_cta(&acc_empty[b]);
       // the shared columns first: the last two pieces of accumulator 0, the first two of accumulator 1
-      store_tile<kTile, TO>(a, &maps.out, lanes + b * kAcc1, stage_out + quarter * kOutBytes, row0, end, col0, fa, fw,
-                            b ? 0 : kAcc1 / 32, kSharedCols / 32, [&] { arrive_at(bar); });
+      constexpr int kTileOut = 32 * kTile * int(sizeof(TO));  // of a warp
+      static_assert(4 * kTileOut <= kStages * kStage, "the last tile's room");
+      const bool last = tiles.next(item) >= tiles.stop();
+      store_tile<kTile, TO>(a, &maps.out, lanes + b * kAcc1, last ? stages + quarter * kTileOut : stage_out + quarter * kOutBytes,
+                            row0, end, col0, fa, fw, b ? 0 : kAcc1 / 32, kSharedCols / 32, last, [&] { arrive_at(bar); });
     }
     if (!ok) *abort_ptr = 1;
     if (lane == 0) tma_stores_done();

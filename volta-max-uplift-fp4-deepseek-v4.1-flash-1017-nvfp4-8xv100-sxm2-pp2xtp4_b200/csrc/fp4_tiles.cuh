@@ -294,10 +294,11 @@ __device__ __forceinline__ void scale_warp_by(int w, const TileArgs& a, const Ti
 // A warp's 32 rows of a finished tile, BN columns of its TMEM lanes from `acc`, times both factors, through 2 KB of shared
 // memory in pieces of 64 bytes per row, 16-byte chunks swizzled by pairs of rows.  Pieces of 32 columns are read from
 // `first` on, around the end; after `release` of them `free()` tells the MMA warp.  row0: the warp's first; end: of the
-// expert's rows.
+// expert's rows.  roomy: the CTA's last tile, whose pieces find room of their own at `mine` and none waits for the one
+// before to leave (the ring of stages, which is done with).
 template <int BN, typename TO, typename Free>
 __device__ __forceinline__ void store_tile(const TileArgs& a, const CUtensorMap* map_out, uint32_t acc, uint8_t* mine, int row0,
-                                           int end, int col0, float fa, float fw, int first, int release, const Free& free) {
+                                           int end, int col0, float fa, float fw, int first, int release, bool roomy, const Free& free) {
   constexpr int PW = 64 / int(sizeof(TO)), CW = 16 / int(sizeof(TO));  // columns per piece, per 16-byte chunk
   const int lane = threadIdx.x & 31;
   TO* out = static_cast<TO*>(a.out);
@@ -317,8 +318,12 @@ __device__ __forceinline__ void store_tile(const TileArgs& a, const CUtensorMap*
     }
 #pragma unroll
     for (int pc = 0; pc < 32 / PW; ++pc) {
-      if (lane == 0) tma_stores_read();  // the piece before has left
-      __syncwarp();
+      if (roomy) {
+        if (i || pc) mine += 32 * 64;
+      } else {
+        if (lane == 0) tma_stores_read();  // the piece before has left
+        __syncwarp();
+      }
 #pragma unroll
       for (int ch = 0; ch < 4; ++ch) {
         float v[CW];
@@ -361,6 +366,17 @@ __device__ __forceinline__ float row_factor(const TileArgs& a, int row) {
 struct TileMaps {
   CUtensorMap a, w, sa, sw, out;
 };
+// The descriptors in use, which the launch carries, on their way before the work that it waits for is done.
+__device__ __forceinline__ void prefetch_maps(const TileMaps& m, bool w_chunks, bool copy_out) {
+  auto one = [](const CUtensorMap& p) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&p)) : "memory");
+  };
+  one(m.a);
+  one(m.w);
+  one(m.sa);
+  if (w_chunks) one(m.sw);
+  if (copy_out) one(m.out);
+}
 int make_tile_args(const Fp4Product& p, int out_dtype, int a_box, int w_box, int sa_box, int sw_box, int cr, bool copy_out,
                   TileArgs& a, TileMaps& m);
 
