@@ -171,9 +171,21 @@ struct NormArgs {
   float* scale;      // E4M3: [rows][ceil(width / 128)]
 };
 
+// CTAs per SM that the registers have to leave room for. f32 rows hold twice the registers of 16-bit ones ahead: 8192 x
+// 4096 take 105 us with two CTAs and 118 with three, E4M3 81 and 97, 8192 x 2001 E4M3 36 and 67; NVFP4 100 and 97.
+// E4M3 of 16-bit rows with an f32 residual, one column at a time, 16384 x 3999: 166 and 251 (rows 150 and 139; with a
+// 16-bit residual E4M3 of 16384 x 2001 90 and 87).
+template <typename T, typename TR, int OUT, bool WIDE, int C>
+__host__ __device__ constexpr int norm_ctas() {
+  if (C > 1) return 1;
+  if (sizeof(T) == 4 && OUT != kNvOut) return 2;
+  if (sizeof(TR) == 4 && OUT == kFp8 && !WIDE) return 2;
+  return sizeof(TR) == 2 && OUT == kMxOut ? 4 : 3;
+}
+
 // T: x's type, TR: the residual's and the sum's.
 template <typename T, typename TR, int OUT, bool WIDE, int C>
-__global__ void __launch_bounds__(kMaxThreads, C > 1 ? 1 : sizeof(TR) == 2 && OUT > kNvOut ? 4 : 3) norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kMaxThreads, norm_ctas<T, TR, OUT, WIDE, C>()) norm_kernel(const NormArgs a) {
   __shared__ __align__(16) float red[3][2][kMaxThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x < 3 * 2 * kMaxThreads / 32) (&red[0][0][0])[threadIdx.x] = 0.f;
