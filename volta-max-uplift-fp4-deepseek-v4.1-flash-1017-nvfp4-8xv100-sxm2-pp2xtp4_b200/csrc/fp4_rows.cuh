@@ -8,8 +8,8 @@
 //     (e8m0: e + 127), and x becomes e2m1(x / 2^e).
 // All roundings are to nearest, ties to even, and the largest E2M1 value is 6.  A
 // power of two as the row's factor adds no rounding, so a value halfway between
-// two codes is seen as one (a factor of amax / 2688 moved such ties, one scale in
-// a hundred for 16-bit rows, by its own rounding).  A NaN or an infinity makes the
+// two codes is seen as one (a factor of amax / 2688 moved such ties, 0.05 % of
+// the scales of normally distributed bf16 rows, by its own rounding).  A NaN or an infinity makes the
 // factor (NVFP4: the whole row) or the block's scale (MXFP4) a NaN.
 //
 // A record is one run of bytes per row: K / 2 of codes (the even column in the

@@ -154,7 +154,7 @@ struct ScaleWay {
 };
 
 constexpr int kScaleWarps = 4;  // and buffers: warp w puts every fourth stage into buffer w
-// One warp for all stages of 128 rows each takes 560 clocks a stage.
+// With one warp for all stages one row x 4096 x 4096 took 8.4 us.
 
 // Warp w's walk over the tiles' stages.  CR: bytes of a row in a chunk, 32 or 64; BLOCKS: 128 rows of the MMA's M, then of its N; SWAP: the weights are M.  W 16:
 // all scales from the chunks; else the weights' by loads of W bytes (row w_row(item) of a tile, four stages ahead).

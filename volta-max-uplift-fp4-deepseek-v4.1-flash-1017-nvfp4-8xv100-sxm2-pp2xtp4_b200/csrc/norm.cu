@@ -18,8 +18,8 @@
 // Backward: a CTA walks rows (rows apart by the grid), holds its columns' part of
 // dw in registers, and loads the next row before it works on this one; the parts
 // are joined by a second launch in a fixed order, so equal inputs give equal bits.
-// Bound: HBM. 16384 x 4096 bf16 with a residual: rows 83 us (6.4 TB/s), E4M3 76, MXFP4 72
-// (6.1), NVFP4 93 (4.7: two sums over the CTA, and the codes' quotients), gradient 98
+// Bound: HBM. 16384 x 4096 bf16 with a residual: rows 83 us (6.4 TB/s), E4M3 76, MXFP4 69
+// (6.4), NVFP4 91 (4.9: two sums over the CTA, and the codes' quotients), gradient 98
 // (5.5). What held it back was instructions: 41 per value forward and 56 backward by
 // single conversions and sums read one by one, 109 (NVFP4) and 187 us. The gradient
 // with its weights and the sum's gradient a row ahead in registers too: 115, spilled.
