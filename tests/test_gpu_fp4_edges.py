@@ -1,0 +1,33 @@
+"""The 4-bit operators (``fp4``, ``experts.Fp4Experts``) where they are easiest to get wrong: scales and factors at the ends
+of f32, every kernel's own range of rows and columns, gradients that have no way back, offsets that fall, two streams.
+
+Products: a truncation of 2^-23 per addition times the sum of magnitudes, the factors' products and one rounding, as
+in ``test_gpu_fp4``; where values are small integers every partial sum is one below 2^24 and the product is exact."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from test_gpu_fp4 import FORMATS, check_product, ops, randn, row_values, weight_values  # noqa: F401
+
+
+# ----------------------------------------------------------- the ends of f32
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 8, 40, 300, 2500])
+@pytest.mark.parametrize("rows_size,factor", [(2.0**122, None), (2.0**122, 3.1e-9), (2.0**-95, 1.3e-11), (2.0**-60, 7e30),
+                                              (2.0**90, 1.7e-33)])
+def test_nvfp4_factors_of_any_size(ops, m, rows_size, factor):  # noqa: F811
+    """Rows near the ends of f32 times a matrix factor (None: 0.02's, a power of two) that brings results back: no kernel may
+    pass f32 on the way (sums reach 2^24 before their factors)."""
+    w = ops.fp4.quantize_weight(randn(1, 300, 256) * 0.02)
+    if factor is not None:
+        w = w._replace(factor=torch.full_like(w.factor, factor))
+    x = randn(m, m, 256) * rows_size
+    rows = ops.fp4.quantize(x)
+    a, wv = row_values(rows), weight_values(w)
+    assert 2.0**-126 < float((a @ wv.t()).abs().max()) < 3e38
+    check_product(ops.fp4.matmul(rows, w, torch.float32), a, wv)
+    check_product(ops.fp4.linear(x, w), a, wv)
+    y = ops.fp4.grouped_matmul(rows, torch.tensor([0, m], dtype=torch.int32, device="cuda"),
+                               w._replace(codes=w.codes[None], scale=w.scale[None]), torch.float32)
+    check_product(y, a, wv)

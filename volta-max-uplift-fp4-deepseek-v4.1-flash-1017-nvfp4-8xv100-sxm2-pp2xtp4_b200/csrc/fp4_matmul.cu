@@ -198,7 +198,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_kernel(const TileArgs a, cons
       const int b = tile & 1;
       const uint32_t acc = lanes + b * BN;
       if constexpr (SWAP) {
-        const float fa = lane < BN ? row_factor(a, row0 + lane) : 1.f, fa2 = BN > 32 ? row_factor(a, row0 + 32 + lane) : 1.f;
+        const Fp4Factors f0 = fp4_factors(lane < BN ? row_factor(a, row0 + lane) : 1.f, fw);
+        const Fp4Factors f1 = BN > 32 ? fp4_factors(row_factor(a, row0 + 32 + lane), fw) : Fp4Factors{1.f, 1.f};
+        const bool two = __any_sync(0xffffffffu, f0.second != 1.f || f1.second != 1.f);  // hardly ever
+        const float last0 = two ? f0.second : f0.first, last1 = two ? f1.second : f1.first;
         ok = poll_warp(&acc_full[b], (tile >> 1) & 1, a.err);
         if (!ok) break;
         fence_after();
@@ -211,22 +214,28 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_kernel(const TileArgs a, cons
         __syncwarp();
         if (lane == 0) mbar_arrive(&acc_empty[b]);
         const int col = col0 + quarter * 32 + lane;
+        if (two) {
+#pragma unroll
+          for (int i = 0; i < BN; ++i)
+            p[i / 16][i % 16] = __float_as_uint(__uint_as_float(p[i / 16][i % 16]) *
+                                                __shfl_sync(0xffffffffu, i < 32 ? f0.first : f1.first, i & 31));
+        }
 #pragma unroll
         for (int i = 0; i < BN; ++i) {
-          const float f = __shfl_sync(0xffffffffu, i < 32 ? fa : fa2, i & 31);
+          const float f = __shfl_sync(0xffffffffu, i < 32 ? last0 : last1, i & 31);
           if (row0 + i < end && col < a.N)
-            out[int64_t(row0 + i) * a.N + col] = from_f32<TO>(__uint_as_float(p[i / 16][i % 16]) * f * fw);
+            out[int64_t(row0 + i) * a.N + col] = from_f32<TO>(__uint_as_float(p[i / 16][i % 16]) * f);
         }
       } else {
         constexpr int kTileOut = 32 * BN * int(sizeof(TO));  // of a warp
         static_assert(4 * kTileOut <= ST * C::kStage, "the last tile's room");
-        const float fa = row_factor(a, row0 + quarter * 32 + lane);
+        const Fp4Factors f = fp4_factors(row_factor(a, row0 + quarter * 32 + lane), fw);
         ok = poll_warp(&acc_full[b], (tile >> 1) & 1, a.err);
         if (!ok) break;
         fence_after();
         const bool last = tiles.next(item) >= tiles.stop();
         store_tile<BN, TO>(a, &maps.out, acc, last ? stages + quarter * kTileOut : stage_out + quarter * kOutBytes,
-                           row0 + quarter * 32, end, col0, fa, fw, 0, BN / 32, last, [&] { mbar_arrive(&acc_empty[b]); });
+                           row0 + quarter * 32, end, col0, f, 0, BN / 32, last, [&] { mbar_arrive(&acc_empty[b]); });
       }
     }
     if (!ok) *abort_ptr = 1;

@@ -257,8 +257,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int item = tiles.first(); ok && item < tiles.stop(); item = tiles.next(item), ++tile) {
       const int e = tile_expert(start, a.E, item), local = item - start[e], end = off(e + 1);
       const int row0 = off(e) + local / n_ct * kTile + rank * kHalf + quarter * 32, col0 = local % n_ct * kTile;
-      const float fw = a.w_factor ? __ldg(a.w_factor + e) : 1.f;
-      const float fa = row_factor(a, row0 + lane);
+      const Fp4Factors f = fp4_factors(row_factor(a, row0 + lane), a.w_factor ? __ldg(a.w_factor + e) : 1.f);
       const int b = tile & 1;
       ok = poll_cluster(&acc_full[b], (tile >> 1) & 1, a.err);
       if (!ok) break;
@@ -269,7 +268,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       static_assert(4 * kTileOut <= kStages * kStage, "the last tile's room");
       const bool last = tiles.next(item) >= tiles.stop();
       store_tile<kTile, TO>(a, &maps.out, lanes + b * kAcc1, last ? stages + quarter * kTileOut : stage_out + quarter * kOutBytes,
-                            row0, end, col0, fa, fw, b ? 0 : kAcc1 / 32, kSharedCols / 32, last, [&] { arrive_at(bar); });
+                            row0, end, col0, f, b ? 0 : kAcc1 / 32, kSharedCols / 32, last, [&] { arrive_at(bar); });
     }
     if (!ok) *abort_ptr = 1;
     if (lane == 0) tma_stores_done();

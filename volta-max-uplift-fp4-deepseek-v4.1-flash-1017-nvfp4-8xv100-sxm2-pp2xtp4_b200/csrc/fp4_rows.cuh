@@ -130,6 +130,20 @@ __device__ __forceinline__ void finish_record(uint8_t* rec, int fmt, int K, floa
   if (fmt == kNv) *reinterpret_cast<float*>(rec + fp4_factor_at(K)) = factor;
 }
 
+// A product's factors, its row's and its matrix's: sum * first * second. Their product and 1 where that is a normal number (a
+// power of two as the row's makes it exact: one rounding). Else both, the one first that leaves the sum (at most 2^40) inside
+// f32 if the result is: rows near f32's largest times a small matrix factor came out infinite as (sum * row's) * matrix's.
+struct Fp4Factors {
+  float first, second;
+};
+__device__ __forceinline__ Fp4Factors fp4_factors(float row, float matrix) {
+  const float both = row * matrix, m = fabsf(both);
+  if ((m >= 0x1p-126f && m < INFINITY) || !(fabsf(row) > 0.f && fabsf(matrix) > 0.f)) return {both, 1.f};  // 0, NaN too
+  const bool less = fabsf(row) < fabsf(matrix);
+  const float small = less ? row : matrix, large = less ? matrix : row;
+  return m < 1.f ? Fp4Factors{large, small} : Fp4Factors{small, large};
+}
+
 __device__ __forceinline__ float e4m3_f32(uint32_t byte) {  // 0x7f / 0xff are NaN
   if ((byte & 0x7fu) == 0x7fu) return fp4_nan();
   const uint32_t ex = (byte >> 3) & 15u, mn = byte & 7u;

@@ -166,8 +166,10 @@ __device__ __forceinline__ void join(const SkinnyArgs& A, float (&red)[kWarps][4
     float sum = 0.f;
 #pragma unroll
     for (int k = 0; k < KS; ++k) sum += red[rsub * KS + k][slot][src];
-    if (t < A.S && col < A.N)
-      static_cast<TO*>(A.out)[int64_t(t) * A.N + col] = from_f32<TO>(factor ? sum * factor[t] * fw : sum);
+    if (t < A.S && col < A.N) {
+      const Fp4Factors f = factor ? fp4_factors(factor[t], fw) : Fp4Factors{1.f, 1.f};
+      static_cast<TO*>(A.out)[int64_t(t) * A.N + col] = from_f32<TO>(sum * f.first * f.second);
+    }
   }
 }
 

@@ -298,7 +298,7 @@ __device__ __forceinline__ void scale_warp_by(int w, const TileArgs& a, const Ti
 // before to leave (the ring of stages, which is done with).
 template <int BN, typename TO, typename Free>
 __device__ __forceinline__ void store_tile(const TileArgs& a, const CUtensorMap* map_out, uint32_t acc, uint8_t* mine, int row0,
-                                           int end, int col0, float fa, float fw, int first, int release, bool roomy, const Free& free) {
+                                           int end, int col0, Fp4Factors f, int first, int release, bool roomy, const Free& free) {
   constexpr int PW = 64 / int(sizeof(TO)), CW = 16 / int(sizeof(TO));  // columns per piece, per 16-byte chunk
   const int lane = threadIdx.x & 31;
   TO* out = static_cast<TO*>(a.out);
@@ -328,7 +328,7 @@ __device__ __forceinline__ void store_tile(const TileArgs& a, const CUtensorMap*
       for (int ch = 0; ch < 4; ++ch) {
         float v[CW];
 #pragma unroll
-        for (int k = 0; k < CW; ++k) v[k] = __uint_as_float(p[pc * PW + ch * CW + k]) * fa * fw;
+        for (int k = 0; k < CW; ++k) v[k] = __uint_as_float(p[pc * PW + ch * CW + k]) * f.first * f.second;
         store_vec<TO, CW>(reinterpret_cast<TO*>(mine + lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4)), v);
       }
       const int col = col0 + c * 32 + pc * PW;
