@@ -31,3 +31,28 @@ def test_nvfp4_factors_of_any_size(ops, m, rows_size, factor):  # noqa: F811
     y = ops.fp4.grouped_matmul(rows, torch.tensor([0, m], dtype=torch.int32, device="cuda"),
                                w._replace(codes=w.codes[None], scale=w.scale[None]), torch.float32)
     check_product(y, a, wv)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 40, 300])
+@pytest.mark.parametrize("weights_size,rows_size", [(2.0**122, 2.0**-60), (2.0**122, 2.0**-110), (2.0**-110, 2.0**100),
+                                                    (2.0**124, 2.0**-20), (2.0**-115, 2.0**122)])
+def test_mxfp4_scales_of_both_sides(ops, m, weights_size, rows_size):  # noqa: F811
+    """Scales of weights and rows near opposite ends of f32: the product of a block's sum with one of them alone passes it."""
+    w = ops.fp4.quantize_weight(randn(1, 300, 256) * weights_size, "mxfp4")
+    rows = ops.fp4.quantize(randn(m, m, 256) * rows_size, "mxfp4")
+    check_product(ops.fp4.matmul(rows, w, torch.float32), row_values(rows), weight_values(w))
+
+
+@pytest.mark.gpu
+def test_mxfp4_scales_that_are_no_number(ops):  # noqa: F811
+    """A NaN scale on either side, by few rows' kernel and by the tiles': its rows and columns, and nothing else."""
+    for m in (2, 40):
+        w = ops.fp4.quantize_weight(randn(1, 50, 256), "mxfp4")
+        w.scale[7, 3] = 255
+        rows = ops.fp4.quantize(randn(m, m, 256), "mxfp4")
+        rows.scale[1, 5] = 255
+        gone = ops.fp4.matmul(rows, w).isnan()
+        want = torch.zeros(m, 50, dtype=torch.bool, device="cuda")
+        want[1], want[:, 7] = True, True
+        assert torch.equal(gone, want)

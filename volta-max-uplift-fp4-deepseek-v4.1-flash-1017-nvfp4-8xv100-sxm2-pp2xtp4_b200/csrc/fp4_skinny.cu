@@ -20,6 +20,7 @@
 // Taken as long as all CTAs, of 16 or 32 weight rows, run at once.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "fp4_ops.h"
 #include "fp4_rows.cuh"
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 2) mxfp4_skinny_kernel(const SkinnyA
 #pragma unroll
     for (int j = 0; j < kDeep; ++j) {
       const int kb = (step * kDeep + j) * KS + ksub;
-      if (kb < KB) {  // the same for the whole warp
+      auto blocks = [&](auto careful) {
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
           const int block = kb * 8 + b;
@@ -301,11 +302,28 @@ __global__ void __launch_bounds__(kThreads, 2) mxfp4_skinny_kernel(const SkinnyA
           const float sl = e8m0_f32((b < 4 ? ws[j][0].x : ws[j][0].y) >> (8 * (b % 4)) & 255u);
           const float sh = e8m0_f32((b < 4 ? ws[j][1].x : ws[j][1].y) >> (8 * (b % 4)) & 255u);
           const float2 sa = *reinterpret_cast<const float2*>(ss + block * kTokens + 2 * q);
-          acc[0] = fmaf(d[0] * sl, sa.x, acc[0]);
-          acc[1] = fmaf(d[1] * sl, sa.y, acc[1]);
-          acc[2] = fmaf(d[2] * sh, sa.x, acc[2]);
-          acc[3] = fmaf(d[3] * sh, sa.y, acc[3]);
+          auto add = [&](float& to, float sum, float sw, float sx) {
+            if constexpr (careful)
+              to = fmaf(sum * min_nan(sw, sx), max_nan(sw, sx), to);
+            else
+              to = fmaf(sum * sw, sx, to);
+          };
+          add(acc[0], d[0], sl, sa.x);
+          add(acc[1], d[1], sl, sa.y);
+          add(acc[2], d[2], sh, sa.x);
+          add(acc[3], d[3], sh, sa.y);
         }
+      };
+      // A block's sum (a multiple of 1/4 up to 1152) times the weights' scale alone is exact below 1 and passes f32 from
+      // 2^118 up, where the row's scale would bring it back: weights with a byte from 192 (2^65) up take the smaller scale
+      // first (for all weights that costs 5 %: 4096 x 4096, one row, 7.9 us instead of 7.5).
+      if (kb < KB) {  // the same for the whole warp
+        const uint32_t s0 = ws[j][0].x, s1 = ws[j][0].y, s2 = ws[j][1].x, s3 = ws[j][1].y;
+        const uint32_t high = (s0 & s0 << 1) | (s1 & s1 << 1) | (s2 & s2 << 1) | (s3 & s3 << 1);
+        if (__any_sync(0xffffffffu, high & 0x80808080u))
+          blocks(std::true_type{});
+        else
+          blocks(std::false_type{});
       }
       if (step + 1 < n_steps) fetch(step + 1, j);
     }
