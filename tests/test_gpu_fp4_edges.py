@@ -56,3 +56,28 @@ def test_mxfp4_scales_that_are_no_number(ops):  # noqa: F811
         want = torch.zeros(m, 50, dtype=torch.bool, device="cuda")
         want[1], want[:, 7] = True, True
         assert torch.equal(gone, want)
+
+
+# ------------------------------------------------------------- gradients lost
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_what_has_no_gradient_refuses_it(ops, fmt):  # noqa: F811
+    """Tokens or router weights that require a gradient, whatever form the tokens come in; under no_grad all serve."""
+    from b200moe.experts import Fp4Experts
+
+    layer = Fp4Experts.from_weights(randn(1, 4, 128, 64, dtype=torch.bfloat16).requires_grad_(), randn(2, 4, 64, 64), fmt)
+    x = randn(3, 6, 64, dtype=torch.bfloat16)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    ids = torch.randint(0, 4, (6, 2), generator=g, device="cuda", dtype=torch.int32)
+    weights, rows = torch.rand(6, 2, generator=g, device="cuda"), ops.fp4.quantize(x, fmt)
+    want = layer(x, ids, weights)
+    learned, leaf = weights.clone().requires_grad_(), x.clone().requires_grad_()
+    for bad in (lambda: layer(rows, ids, learned), lambda: layer(x, ids, learned), lambda: layer(leaf, ids, weights),
+                lambda: ops.fp4.quantize(leaf, fmt), lambda: ops.fp4.swiglu_quantize(leaf, 10.0, fmt)):
+        with pytest.raises(ValueError, match="gradient"):
+            bad()
+    with torch.no_grad():
+        assert torch.equal(layer(rows, ids, learned), want) and torch.equal(layer(leaf, ids, learned), want)
+        assert torch.equal(ops.fp4.quantize(leaf, fmt).record, rows.record)
+        ops.fp4.swiglu_quantize(leaf, 10.0, fmt)

@@ -504,6 +504,10 @@ int64_t record_bytes(int64_t format, int64_t k) {
 }
 int64_t fp4_scales(int64_t format, int64_t k) { return k / (format == kMxfp4 ? 32 : 16); }
 
+void no_fp4_gradient(const Tensor& x) {
+  TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !x.requires_grad(), "4-bit rows and products have no gradient");
+}
+
 Tensor run_fp4_quantize(const Tensor& x, int64_t k, int64_t format, bool swiglu, float limit) {
   const int64_t bytes = record_bytes(format, k), rows = x.size(0);
   const c10::cuda::CUDAGuard guard(x.device());
@@ -517,11 +521,13 @@ Tensor run_fp4_quantize(const Tensor& x, int64_t k, int64_t format, bool swiglu,
 
 Tensor fp4_quantize(const Tensor& x, int64_t format) {
   want("x", x, kFloats, 2, nullptr, true);
+  no_fp4_gradient(x);
   return run_fp4_quantize(x, x.size(1), format, false, 1.f);
 }
 
 Tensor fp4_swiglu_quantize(const Tensor& h, const std::optional<double>& limit, int64_t format) {
   check_gate_up(h);
+  no_fp4_gradient(h);
   return run_fp4_quantize(h, h.size(1) / 2, format, true, check_limit(limit));
 }
 
@@ -653,7 +659,7 @@ Tensor fp4_linear(const Tensor& x, const Tensor& codes, const Tensor& scale, con
   TORCH_CHECK_VALUE(2 * codes.size(1) == k, "the weights have ", 2 * codes.size(1), " columns, the rows ", k);
   const ScalarType dtype = out_dtype.value_or(x.scalar_type());
   check_out(dtype);
-  TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !x.requires_grad(), "4-bit products have no gradient");
+  no_fp4_gradient(x);
   const c10::cuda::CUDAGuard guard(x.device());
   Tensor out = empty({m, n}, dtype, x), ws;
   if (m == 0) return out;

@@ -126,12 +126,13 @@ class Fp4Experts:
     def forward(self, x: torch.Tensor | fp4.Rows, topk_ids: torch.Tensor, topk_weights: torch.Tensor,
                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """x [T, H] (bf16, f16 or f32) or its ``fp4.Rows``, int32 ids and fp32 weights [T, k] -> [T, H], in x's
-        dtype where that has 16 bits, else in ``out_dtype``.  An id outside [0, E) contributes nothing."""
+        dtype where that has 16 bits, else in ``out_dtype``.  An id outside [0, E) contributes nothing.  Tokens or
+        weights that require a gradient are refused."""
         if topk_weights.shape != topk_ids.shape:
             raise ValueError(f"bad routing shape {tuple(topk_ids.shape)} with weights {tuple(topk_weights.shape)}")
+        if torch.is_grad_enabled() and (topk_weights.requires_grad or (not isinstance(x, fp4.Rows) and x.requires_grad)):
+            raise ValueError("4-bit experts have no gradient")
         if not isinstance(x, fp4.Rows):
-            if torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad):
-                raise ValueError("4-bit experts have no gradient")
             if x.dtype != torch.float32:
                 out_dtype = x.dtype
             x = fp4.quantize(x, self.format)

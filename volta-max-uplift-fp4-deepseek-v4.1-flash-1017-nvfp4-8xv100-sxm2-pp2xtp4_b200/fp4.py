@@ -10,8 +10,8 @@ factor (NVFP4) or a block's scale (MXFP4) a NaN, and so its product's row.  Prod
 both operands in the same format, sum in f32 and round once.  Weights are ``quantize_weight``'s or a
 pack's: ``Weights(*packing.quantize_nvfp4(w))``, ``Weights(*packing.quantize_mxfp4(w))``.
 
-For serving: values come back without a graph, and ``linear`` refuses rows that require a
-gradient.  Columns come in multiples of 32.  Arguments that do not fit raise ``ValueError`` (a
+For serving: rows that require a gradient are refused (``quantize``, ``swiglu_quantize``, ``linear``) but
+under ``torch.no_grad``, and values come back without a graph.  Columns come in multiples of 32.  Arguments that do not fit raise ``ValueError`` (a
 packed operand's address off 16 bytes ``B200MoeError``); offsets out of range are cut and reported by
 ``check_errors``.
 """
