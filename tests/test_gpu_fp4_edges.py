@@ -81,3 +81,30 @@ def test_what_has_no_gradient_refuses_it(ops, fmt):  # noqa: F811
         assert torch.equal(layer(rows, ids, learned), want) and torch.equal(layer(leaf, ids, learned), want)
         assert torch.equal(ops.fp4.quantize(leaf, fmt).record, rows.record)
         ops.fp4.swiglu_quantize(leaf, 10.0, fmt)
+
+
+# ------------------------------------------------------------------ values back
+def once(v, dtype):
+    """64-bit values rounded once to bf16 or f16 (torch's own conversion passes through f32)."""
+    bits, least = (8, -133) if dtype == torch.bfloat16 else (11, -24)
+    e = (torch.frexp(v)[1] - bits).clamp_min(least)
+    return torch.ldexp(torch.ldexp(v, -e).round(), e).to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("low,high", [(1e-4, 1.0), (1e-10, 1e-6), (1e-40, 1e-36)])
+def test_values_of_any_factor_are_rounded_once(ops, dtype, low, high):  # noqa: F811
+    """Factors of 24 bits, as a pack's: products of 30 bits, of which some round in f32 to a border of 16-bit values: one in
+    2^14 for f16, in 2^17 for bf16."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(11)
+    e, n, k = 4096, 8, 256
+    factor = torch.exp(torch.rand(e, generator=g, device="cuda", dtype=torch.float64) *
+                       torch.log(torch.tensor(high / low, dtype=torch.float64)).item() +
+                       torch.log(torch.tensor(low, dtype=torch.float64)).item()).float()
+    codes = torch.randint(0, 256, (e, n, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scale = torch.randint(0, 127, (e, n, k // 16), generator=g, device="cuda", dtype=torch.uint8)
+    w = ops.fp4.Weights(codes, scale, factor)
+    want = once(weight_values(w), dtype)
+    assert torch.equal(ops.fp4.dequantize(w, dtype), want)
