@@ -108,3 +108,39 @@ def test_values_of_any_factor_are_rounded_once(ops, dtype, low, high):  # noqa: 
     w = ops.fp4.Weights(codes, scale, factor)
     want = once(weight_values(w), dtype)
     assert torch.equal(ops.fp4.dequantize(w, dtype), want)
+
+
+# ------------------------------------------------------------- offsets that fall
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", FORMATS + ["fp8"])
+@pytest.mark.parametrize("c", [1, 2, 5, 20])  # rows per expert by which another kernel is chosen
+@pytest.mark.parametrize("offsets,held", [([0, 30, 10, 50], [(0, 0, 30)]), ([0, 30, 40, 10], [(0, 0, 30), (1, 30, 40)]),
+                                          ([10, 5, 20, 30], [(2, 20, 30)]), ([0, 60, 0, 60], [(0, 0, 60)]),
+                                          ([5, 20, 70, 40], [(0, 5, 20)]), ([-10, 20, 15, 40], [(2, 15, 40)]),
+                                          ([0, 20, 10, 30], [(0, 0, 20)])])
+def test_offsets_that_fall(ops, pkg, which, c, offsets, held):  # noqa: F811
+    """Experts whose rows lie in order keep their results: a later expert that goes back over them, or the rows behind the last
+    offset, must not write there.  Rows before the first offset are zeros."""
+    n, k, s = 200, 96, 60 * c
+    x, w = randn(c, s, k), randn(2, 3, n, k)
+    if which == "fp8":
+        q, wq = ops.fp8.quantize(x), ops.fp8.quantize_weight(w)
+        run = lambda off: ops.fp8.grouped_matmul(*q, off, *wq)  # noqa: E731
+        one = lambda e, a, b: ops.fp8.grouped_matmul(*q, good(e, a, b), *wq)  # noqa: E731
+    else:
+        q, wq = ops.fp4.quantize(x, which), ops.fp4.quantize_weight(w, which)
+        run = lambda off: ops.fp4.grouped_matmul(q, off, wq)  # noqa: E731
+        one = lambda e, a, b: ops.fp4.grouped_matmul(q, good(e, a, b), wq)  # noqa: E731
+
+    def good(e, a, b):
+        return torch.tensor([a] * (e + 1) + [b] * (3 - e), dtype=torch.int32, device="cuda")
+
+    want = [(c * a, c * b, one(e, c * a, c * b)[c * a: c * b]) for e, a, b in held]
+    ops.fp4.check_errors()
+    y = run(torch.tensor([c * o for o in offsets], dtype=torch.int32, device="cuda"))
+    for a, b, rows in want:
+        assert torch.equal(y[a:b], rows) and rows.any()
+    assert not y[: max(0, c * offsets[0])].any()
+    with pytest.raises(pkg._lib.B200MoeError):
+        ops.fp4.check_errors()
+    ops.fp4.check_errors()

@@ -45,7 +45,7 @@ struct Cfg {
   static constexpr size_t kSmem = 1024 + size_t(kStages) * kStage + kChunks * kChunk + kSfBufs * kSfBytes + 4 * kOutBytes +
                                   8 * (2 * kStages + 2 * kChunks + 2 * kSfBufs + 4);
   static_assert(4 * kOutBytes >= 4 * (kFp4MaxExperts + 1), "the offsets, while the tile table is made");
-  static_assert(kSmem + 4 * (kFp4MaxExperts + 1) + 64 <= 227 * 1024, "shared memory, with the tile table");
+  static_assert(kSmem + 4 * (kFp4MaxExperts + 2) + 64 <= 227 * 1024, "shared memory, with the tile table");
 };
 
 template <int BN, bool SWAP, int FMT, typename TO>
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_kernel(const TileArgs a, cons
   using C = Cfg<BN>;
   constexpr int ST = C::kStages, CH = C::kChunks;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int start[kFp4MaxExperts + 1];
+  __shared__ int start[kFp4MaxExperts + 2];
   __shared__ uint32_t tmem_base_sh;
   __shared__ int abort_flag;
   const uint32_t base_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_kernel(const TileArgs a, cons
     }
     if (!ok) *abort_ptr = 1;
     if (!SWAP && lane == 0) tma_stores_done();
-    if (a.offsets) zero_rows(out, a.N, off(0), off(a.E), a.S, threadIdx.x - 128, 128);
+    if (a.offsets) zero_rows(out, a.N, off(0), start[a.E + 1], a.S, threadIdx.x - 128, 128);
   } else {
     const ScaleWay way{chunks, C::kChunk, CH, chunk_full, chunk_empty, sf, sf_empty, BN};
     auto w_row = [&](int item) {

@@ -49,7 +49,7 @@ struct Cfg {
   static constexpr int kChunk = (kHalf + kTile) * kChunkRow;
   static constexpr size_t kSmem = 1024 + kStages * kStage + kChunks * kChunk + kSfBufs * kSfBytes + 4 * kOutBytes +
                                   8 * (2 * kStages + 2 * kChunks + 2 * kSfBufs + 4);
-  static_assert(kSmem + 4 * (kFp4MaxExperts + 1) + 64 <= 227 * 1024, "shared memory, with the tile table");
+  static_assert(kSmem + 4 * (kFp4MaxExperts + 2) + 64 <= 227 * 1024, "shared memory, with the tile table");
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -118,7 +118,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   using C = Cfg<FMT>;
   constexpr int kStages = C::kStages, kChunkRow = C::kChunkRow, kChunk = C::kChunk;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int start[kFp4MaxExperts + 1];
+  __shared__ int start[kFp4MaxExperts + 2];
   __shared__ uint32_t tmem_base_sh;
   __shared__ int abort_flag;
   const uint32_t base_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -273,7 +273,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (!ok) *abort_ptr = 1;
     if (lane == 0) tma_stores_done();
     if (a.offsets)
-      zero_rows(static_cast<TO*>(a.out), a.N, off(0), off(a.E), a.S, threadIdx.x - 128, 128);
+      zero_rows(static_cast<TO*>(a.out), a.N, off(0), start[a.E + 1], a.S, threadIdx.x - 128, 128);
   } else {
     const ScaleWay way{chunks, kChunk, kChunks, chunk_full, chunk_empty, sf, sf_empty, kTile};
     auto w_row = [&](int item) {

@@ -42,8 +42,11 @@ __device__ __forceinline__ uint32_t e4m3x4(float v0, float v1, float v2, float v
 
 // Tiles of a product whose rows are sorted by expert: expert e has
 // ceil(count / rows_per_tile) * per_row_tile tiles, from start[e] on.  Called by
-// every thread of the CTA; off and start are shared int [E + 1].  Offsets that
-// fall or pass n_rows are cut to what lies inside, and reported.
+// every thread of the CTA; off and start are shared int [E + 1] and [E + 2], the
+// last of it where the experts' rows end.  Offsets that fall or pass n_rows are
+// reported, and their experts get no tiles, nor do those that begin before the
+// end of an earlier one's rows: a row has one expert, so that no two tiles write
+// the same rows and the tiles are never more than the rows ask for.
 __device__ __forceinline__ void build_tile_table(const int32_t* __restrict__ offsets, int E, int n_rows,
                                                  int rows_per_tile, int per_row_tile, int* off, int* start,
                                                  uint32_t* err) {
@@ -60,11 +63,13 @@ __device__ __forceinline__ void build_tile_table(const int32_t* __restrict__ off
   __syncthreads();
   if (threadIdx.x < 32) {
     int carry = 0;
+    bool fell = false;
     for (int e0 = 0; e0 < E; e0 += 32) {
       const int e = e0 + threadIdx.x;
       int tiles = 0;
       if (e < E) {
         const int lo = off[e], hi = off[e + 1];
+        fell |= hi < lo;
         if (lo < 0 || hi < lo || hi > n_rows)
           set_error(err, kErrBounds);
         else
@@ -79,7 +84,24 @@ __device__ __forceinline__ void build_tile_table(const int32_t* __restrict__ off
       if (e < E) start[e] = carry + incl - tiles;
       carry += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (threadIdx.x == 0) start[E] = carry;
+    fell = __any_sync(0xffffffffu, fell);
+    __syncwarp();
+    if (threadIdx.x == 0) {
+      int end = off[E];
+      if (fell) {
+        end = max(off[0], 0);
+        carry = 0;
+        for (int e = 0; e < E; ++e) {
+          const int lo = off[e], hi = off[e + 1];
+          start[e] = carry;
+          if (lo < end || hi < lo || hi > n_rows) continue;
+          carry += (hi - lo + rows_per_tile - 1) / rows_per_tile * per_row_tile;
+          end = hi;
+        }
+      }
+      start[E] = carry;
+      start[E + 1] = end;
+    }
   }
   __syncthreads();
 }

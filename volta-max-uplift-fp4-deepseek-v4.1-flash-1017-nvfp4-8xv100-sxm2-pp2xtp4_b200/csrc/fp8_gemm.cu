@@ -66,7 +66,7 @@ struct Cfg {
   static constexpr int kCols = BN / 2;                        // columns per sum thread
   static constexpr size_t kSmem = 1024 + size_t(kStages) * (kABytes + kWBytes) + kSumWarps * kOutBytes + 256;
   static constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
-  static_assert(kSmem + 8 * (kMaxExperts + 1) + 64 <= 227 * 1024, "shared memory, with the tile table");
+  static_assert(kSmem + 8 * (kMaxExperts + 2) + 64 <= 227 * 1024, "shared memory, with the tile table");
 };
 
 struct GemmArgs {
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<BN>;
   constexpr int ST = C::kStages, NBUF = C::kBufs, COLS = C::kCols;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int off[kMaxExperts + 1], start[kMaxExperts + 1];
+  __shared__ int off[kMaxExperts + 1], start[kMaxExperts + 2];
   __shared__ uint32_t tmem_base_sh;
   __shared__ int abort_flag;
   const uint32_t base_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (lane == 0) tma_stores_done();
-    if (a.offsets) zero_rows(static_cast<TO*>(a.out), a.N, off[0], off[a.E], a.S, threadIdx.x - kSumWarp0 * 32, kSumWarps * 32);
+    if (a.offsets) zero_rows(static_cast<TO*>(a.out), a.N, off[0], start[a.E + 1], a.S, threadIdx.x - kSumWarp0 * 32, kSumWarps * 32);
   }
   fence_before();
   __syncthreads();

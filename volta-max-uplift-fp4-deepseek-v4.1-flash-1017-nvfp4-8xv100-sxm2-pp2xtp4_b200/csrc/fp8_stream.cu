@@ -50,7 +50,7 @@ struct Cfg {
   static_assert(kStages % 2 == 0 && kBufs % 2 == 0, "stages and buffers by MMA warp");
   static constexpr size_t kSmem = 1024 + size_t(kStages) * kStage + kScaleBytes + 512;
   static constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(NTOK >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
-  static_assert(kSmem + 8 * (kMaxExperts + 1) + 64 <= 227 * 1024, "shared memory, with the tile table");
+  static_assert(kSmem + 8 * (kMaxExperts + 2) + 64 <= 227 * 1024, "shared memory, with the tile table");
   static_assert(kBufs * NTOK <= 512, "TMEM");
 };
 
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<NTOK>;
   constexpr int ST = C::kStages;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int off[kMaxExperts + 1], start[kMaxExperts + 1];
+  __shared__ int off[kMaxExperts + 1], start[kMaxExperts + 2];
   __shared__ uint32_t tmem_base_sh;
   __shared__ int abort_flag;
   const uint32_t base_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (row0 + i < end) out[int64_t(row0 + i) * a.N + col] = from_f32<TO>(acc[i]);
       }
     }
-    if (a.offsets) zero_rows(out, a.N, off[0], off[a.E], a.S, tid, 128);
+    if (a.offsets) zero_rows(out, a.N, off[0], start[a.E + 1], a.S, tid, 128);
   }
   fence_before();
   __syncthreads();

@@ -123,7 +123,8 @@ def matmul(a: Rows, w: Weights, out_dtype: torch.dtype = torch.bfloat16) -> torc
 def grouped_matmul(a: Rows, offsets: torch.Tensor, w: Weights, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """Rows sorted by expert (``permute``) times each expert's weights [E, N, K]: rows
     ``offsets[e] : offsets[e + 1]`` use ``w[e]``; rows before ``offsets[0]`` and from ``offsets[E]``
-    on become zeros.  Offsets that fall or pass the rows are reported; those experts' rows hold no result."""
+    on become zeros.  Offsets that fall or pass the rows are reported; those experts have no result, nor
+    have later ones that go back over an earlier one's rows."""
     return _lib.ops().fp4_grouped_matmul(a.record, a.columns, _format(a.format), offsets, *w, out_dtype)
 
 
