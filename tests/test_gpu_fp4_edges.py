@@ -144,3 +144,50 @@ def test_offsets_that_fall(ops, pkg, which, c, offsets, held):  # noqa: F811
     with pytest.raises(pkg._lib.B200MoeError):
         ops.fp4.check_errors()
     ops.fp4.check_errors()
+
+
+# ------------------------------------------------- each kernel's rows and columns
+def integers(seed, *shape):
+    """E2M1's integers, a 6 in each block of 16: quantizing leaves them as they are."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    x = torch.tensor([0.0, 1, 2, 3, 4, 6, -1, -2, -3, -4, -6], device="cuda")[
+        torch.randint(0, 11, shape, generator=g, device="cuda")]
+    x[..., ::16] = 6.0
+    return x
+
+
+def check_exact(ops, fmt, m, n, k):  # noqa: F811
+    """Sums stay below 36 * 2^14 < 2^24: whatever their order, a product is the integer."""
+    assert 36 * k < 2**24
+    x, w = integers(m + k, m, k), integers(n + k, n, k)
+    rows, q = ops.fp4.quantize(x, fmt), ops.fp4.quantize_weight(w, fmt)
+    assert torch.equal(ops.fp4.dequantize(rows, torch.float32), x) and torch.equal(ops.fp4.dequantize(q, torch.float32), w)
+    want = (x.double() @ w.double().t()).float()
+    assert torch.equal(ops.fp4.matmul(rows, q, torch.float32), want)
+    assert torch.equal(ops.fp4.linear(x.bfloat16(), q, torch.float32), want)
+    assert torch.equal(ops.fp4.linear(x, q), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", [1, 2, 3, 8])
+@pytest.mark.parametrize("n,k", [(333, 32), (65, 1056), (333, 2048), (333, 2080), (64, 4064), (333, 4096), (333, 4128), (120, 7168),
+                                 (17, 8224), (333, 14336), (2368, 6144)])
+def test_few_rows_are_exact(ops, fmt, m, n, k):  # noqa: F811
+    """Four warps and eight along K, blocks that end inside, more blocks than a warp has in flight (K above 4096), rows that
+    fill shared memory (8 x 7168, 3 x 14336), one row tile more than the GPU has SMs."""
+    check_exact(ops, fmt, m, n, k)
+    ops.fp4.check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,k", [(2, 2048), (4, 1024), (8, 512), (3, 1312), (5, 800), (7, 96), (8, 32), (1, 4064)])
+def test_few_rows_quantized_by_the_product(ops, fmt, m, k):  # noqa: F811
+    """Up to 4096 values, by the pieces of 16 that whole warps, or not, share with a row; two rows of very different size."""
+    check_exact(ops, fmt, m, 100, k)
+    x, w = randn(m, m, k, dtype=torch.bfloat16), ops.fp4.quantize_weight(randn(k, 100, k), fmt)
+    x[-1] *= 1000
+    check_product(ops.fp4.linear(x, w), row_values(ops.fp4.quantize(x, fmt)), weight_values(w))
+    assert torch.equal(ops.fp4.linear(x, w), ops.fp4.matmul(ops.fp4.quantize(x, fmt), w))

@@ -32,8 +32,9 @@ int launch_fp4_stream(cudaStream_t s, const Fp4Product& p, int rows_per_tile, in
 int launch_fp4_skinny(cudaStream_t s, const Fp4Product& p, const void* x, int x_dtype, int64_t ldx, int out_dtype);
 // whether its rows fit in shared memory and its CTAs run in one wave
 bool fp4_skinny_fits(const Fp4Product& p);
-// whether it quantizes rows itself: as many as its threads hold at once. One row of 4096 columns takes 6.3 us so, 7.1 by a
-// launch of its own; two take 7.9 and 7.5
-inline bool fp4_skinny_quantizes(int S, int K) { return int64_t(S) * K <= 4096; }
+// whether it quantizes rows itself: as many values as its threads hold at once, 16 each. One row of 4096 columns takes 6.3 us
+// so, 7.1 by a launch of its own; two, with turns, 7.9 and 7.5
+constexpr int kFp4SkinnyThreads = 256;
+inline bool fp4_skinny_quantizes(int S, int K) { return int64_t(S) * K <= 16 * kFp4SkinnyThreads; }
 
 }  // namespace b200moe

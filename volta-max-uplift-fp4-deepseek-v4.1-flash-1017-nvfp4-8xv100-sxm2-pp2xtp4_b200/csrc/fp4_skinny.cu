@@ -1,6 +1,6 @@
 // 4-bit products of at most eight rows with one matrix: the weights go straight from
 // global memory into the registers of the warps that multiply them. One launch does
-// it all: one or two rows of f16 or bf16 are quantized by every CTA for itself.
+// it all: up to 4096 values of f16 or bf16 rows (one row of 4096 columns, eight of 512) are quantized by every CTA for itself.
 //
 // A warp owns 16 weight rows and every KS-th block of 256 columns.  NVFP4: each lane
 // loads four 16-byte pieces per block (32 columns each: rows g and g + 8, pieces q and q + 4; g =
@@ -31,6 +31,7 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
+static_assert(kThreads == kFp4SkinnyThreads, "16 values of the rows that it quantizes per thread");
 constexpr int kTokens = 8;
 constexpr int kBlockK = 256;
 constexpr int kDeep = 2;  // blocks of a warp in flight
@@ -102,52 +103,37 @@ __device__ __forceinline__ void stage_tokens(const SkinnyArgs& A, uint8_t* xs, f
     if (FMT == kNv && threadIdx.x < A.S)
       factor[threadIdx.x] = *reinterpret_cast<const float*>(A.a + int64_t(threadIdx.x) * stride + fp4_factor_at(A.K));
   } else {
-    const TX* x = reinterpret_cast<const TX*>(A.a);
+    // a piece per thread; pieces is even, so both halves of an MXFP4 block are in one warp
+    const int i = threadIdx.x, r = i / pieces, p = i - r * pieces;
+    const bool in = i < total;
     float v[16], m = 0.f;
-    auto load = [&](int i) {
-      const int r = i / pieces, p = i - r * pieces;
+    if (in) {
       Vec<TX, 16> raw;
-      raw.load(x + r * A.ldx + p * 16);
+      raw.load(reinterpret_cast<const TX*>(A.a) + r * A.ldx + p * 16);
 #pragma unroll
       for (int j = 0; j < 16; ++j) v[j] = raw.get(j);
       m = magnitude16(v);
-    };
+    }
     if constexpr (FMT == kMx) {
-      // pieces is even, and whole warps take the same turns: both halves of a block are there
-      for (int i0 = threadIdx.x & ~31; i0 < total; i0 += kThreads) {
-        const int i = i0 + (threadIdx.x & 31);
-        m = 0.f;
-        if (i < total) load(i);
-        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        if (i < total) {
-          const int r = i / pieces, p = i - r * pieces;
-          float inv;
-          const uint32_t s = mxfp4_scale(m, inv);
-          put_tokens(place(r, p), mxfp4_codes(v, inv), 1.f);
-          if (!(p & 1)) scales[p / 2 * kTokens + r] = e8m0_f32(s);
-        }
+      m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      if (in) {
+        float inv;
+        const uint32_t s = mxfp4_scale(m, inv);
+        put_tokens(place(r, p), mxfp4_codes(v, inv), 1.f);
+        if (!(p & 1)) scales[p / 2 * kTokens + r] = e8m0_f32(s);
       }
     } else {
       if (threadIdx.x < kTokens) top[threadIdx.x] = 0;
       __syncthreads();
-      for (int i0 = threadIdx.x & ~31; i0 < total; i0 += kThreads) {
-        const int i = i0 + (threadIdx.x & 31);
-        uint32_t t = 0;
-        if (i < total) {
-          load(i);
-          t = abs_bits(m);
-        }
-        if (pieces % 32 == 0) t = __reduce_max_sync(0xffffffffu, t);  // the warp's columns are of one row
-        if (i < total && (pieces % 32 || i == i0)) atomicMax(top + i / pieces, t);  // in any order, a maximum is the same
-      }
+      uint32_t t = in ? abs_bits(m) : 0u;
+      if (pieces % 32 == 0) t = __reduce_max_sync(0xffffffffu, t);  // the warp's columns are of one row
+      if (in && (pieces % 32 || threadIdx.x % 32 == 0)) atomicMax(top + r, t);  // in any order, a maximum is the same
       __syncthreads();
       if (threadIdx.x < A.S) factor[threadIdx.x] = nvfp4_factor(top[threadIdx.x]);
-      for (int i = threadIdx.x; i < total; i += kThreads) {
-        if (total > kThreads) load(i);  // else the columns are still here
-        const int r = i / pieces;
+      if (in) {
         float unit;
         const uint32_t s = nvfp4_scale(m, nvfp4_factor(top[r]), unit);
-        put_tokens(place(r, i - r * pieces), nvfp4_codes(v, unit), e4m3_f32(s));
+        put_tokens(place(r, p), nvfp4_codes(v, unit), e4m3_f32(s));
       }
     }
   }
