@@ -9,6 +9,7 @@ from __future__ import annotations
 import pytest
 import torch
 from test_gpu_fp4 import FORMATS, check_product, ops, randn, row_values, weight_values  # noqa: F401
+from test_gpu_fp4_experts import test_a_block_by_its_steps as block_by_steps
 
 
 # ----------------------------------------------------------- the ends of f32
@@ -191,3 +192,78 @@ def test_few_rows_quantized_by_the_product(ops, fmt, m, k):  # noqa: F811
     x[-1] *= 1000
     check_product(ops.fp4.linear(x, w), row_values(ops.fp4.quantize(x, fmt)), weight_values(w))
     assert torch.equal(ops.fp4.linear(x, w), ops.fp4.matmul(ops.fp4.quantize(x, fmt), w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,n,k", [(16, 520, 4128), (40, 2000, 4128), (100, 520, 14336), (200, 4096, 7168), (1000, 520, 6144),
+                                   (3000, 1000, 4128), (9, 8192, 2080)])
+def test_more_rows_are_exact(ops, fmt, m, n, k):  # noqa: F811
+    check_exact(ops, fmt, m, n, k)
+    ops.fp4.check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("counts,tail,n,k", [
+    ([60, 0, 128, 129, 1], 0, 333, 352), ([100, 90, 130, 127, 65], 20, 512, 1408), ([53], 0, 100, 64), ([0, 0, 0, 440], 3, 1000, 4128),
+    ([70] * 40, 0, 256, 608)])
+def test_grouped_rows_of_128_are_exact(ops, fmt, dtype, counts, tail, n, k):  # noqa: F811
+    """52 to 112 rows per matrix: the kernel with 128 of them as the MMA's M."""
+    e, s = len(counts), sum(counts) + tail
+    assert 52 * e < s <= 112 * e
+    x, w = integers(s, s, k), integers(n, e, n, k)
+    off = torch.tensor([0] + counts, device="cuda").cumsum(0).to(torch.int32)
+    y = ops.fp4.grouped_matmul(ops.fp4.quantize(x, fmt), off, ops.fp4.quantize_weight(w, fmt), dtype)
+    for i in range(e):
+        lo, hi = int(off[i]), int(off[i + 1])
+        assert torch.equal(y[lo:hi], (x[lo:hi].double() @ w[i].double().t()).float().to(dtype))
+    assert not y[s - tail:].any()
+    ops.fp4.check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("t,k,e", [(50, 3, 5), (100, 4, 5), (400, 4, 5), (6, 5, 3)])
+def test_a_block_by_every_kernel(pkg, fmt, t, k, e):
+    """30, 80, 320 and 10 rows per expert (in the last, tokens name experts twice)."""
+    from b200moe import experts, fp4, norm, permute
+
+    every = type("Ops", (), {"experts": experts, "fp4": fp4, "norm": norm, "permute": permute})
+    if k <= e:
+        return block_by_steps(every, fmt, torch.bfloat16, t, k, e, 512, 352, 0.0)
+    layer = experts.Fp4Experts.from_weights(randn(1, e, 128, 64) / 8, randn(2, e, 64, 64) / 8, fmt)
+    x, weights = randn(3, t, 64, dtype=torch.bfloat16), torch.rand(t, k, device="cuda")
+    ids = (torch.arange(t * k, device="cuda").view(t, k) % e).to(torch.int32)
+    parts = torch.stack([layer(x, ids[:, i: i + 1].contiguous(), torch.ones(t, 1, device="cuda"), torch.float32)
+                         for i in range(k)], 1).double() * weights.double()[..., None]
+    bound = 2.0**-8 * parts.sum(1).abs() + (k + 1) * 2.0**-23 * parts.abs().sum(1)
+    assert bool(((layer(x, ids, weights).double() - parts.sum(1)).abs() <= bound).all())
+
+
+# ------------------------------------------------------------------ two streams
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["linear_1", "linear_40", "linear_5000", "grouped"])
+def test_calls_on_two_streams_at_once(ops, what):  # noqa: F811
+    """Alternating calls with inputs of their own, nothing waiting in between: each result is the one of a call alone."""
+    w = ops.fp4.quantize_weight(randn(1, 4, 1024, 2048) * 0.02)
+    one = w._replace(codes=w.codes[0], scale=w.scale[0], factor=w.factor[:1])
+    if what == "grouped":
+        xs = [ops.fp4.quantize(randn(i, 300, 2048)) for i in range(6)]
+        offs = [torch.tensor([0, 10 * i, 100, 250 + i, 300], dtype=torch.int32, device="cuda") for i in range(6)]
+        run = lambda i: ops.fp4.grouped_matmul(xs[i], offs[i], w)  # noqa: E731
+    else:
+        xs = [randn(i, int(what[7:]), 2048, dtype=torch.bfloat16) for i in range(6)]
+        run = lambda i: ops.fp4.linear(xs[i], one)  # noqa: E731
+    want = [run(i) for i in range(6)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for j in range(60):
+        with torch.cuda.stream(streams[j % 2]):
+            got.append((j % 6, run(j % 6)))
+    torch.cuda.synchronize()
+    for i, y in got:
+        assert torch.equal(y, want[i])
+    ops.fp4.check_errors()
