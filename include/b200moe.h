@@ -436,8 +436,8 @@ int b200moe_fp4_quantize(void* stream, const void* x, int dtype, int64_t x_strid
  * (MXFP4: NULL). */
 int b200moe_fp4_quantize_weight(void* stream, const void* w, int dtype, int mats, int n, int k, int format, void* codes,
                                 void* scale, float* factor);
-/* What codes, scales and factors (NULL: 1) stand for: out [rows][k] = value *
- * scale * factor, rounded once.  ld_*: bytes between rows (ld_factor 0: one factor
+/* What codes, scales (E4M3 without a sign) and factors (NULL: 1) stand for: out
+ * [rows][k] = value * scale * factor, rounded once.  ld_*: bytes between rows (ld_factor 0: one factor
  * for all); codes and factors on 4 bytes, out on 16. */
 int b200moe_fp4_values(void* stream, const void* codes, int64_t ld_codes, const void* scale, int64_t ld_scale,
                        const void* factor, int64_t ld_factor, int64_t rows, int k, int format, void* out, int dtype);

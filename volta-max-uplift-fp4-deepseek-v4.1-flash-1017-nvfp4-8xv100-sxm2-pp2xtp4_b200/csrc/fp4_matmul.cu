@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_kernel(const TileArgs a, cons
         tma_2d(SWAP ? n : m, &maps.sa, x, off(e) + local / n_ct * row_tile, bar);
         if (w_chunks) tma_2d(SWAP ? m : n, &maps.sw, x, e * a.N + local % n_ct * col_tile, bar);
       };
-      chunk_warp<FMT, kChunkRow>(a, tiles, way, uint32_t((row_tile + (w_chunks ? col_tile : 0)) * kChunkRow), load, abort_ptr);
+      const uint32_t tx = uint32_t((row_tile + (w_chunks ? col_tile : 0)) * kChunkRow);
+      chunk_warp<FMT, kChunkRow>(a, tiles, way, tx, load, abort_ptr);
     } else {
       scale_warp_by<FMT, kChunkRow, 2, SWAP>(warp < 4 ? warp - 2 : warp - 6, a, tiles, way, w_row,
                                   [&](int b) { mbar_arrive(&sf_full[b]); }, abort_ptr);
@@ -360,16 +361,17 @@ int product_status(const Fp4Product& p, int out_dtype) {
 // The kernel by rows per matrix: that of a few rows where it fits (fp4_skinny.cu), else as measured on B200 (us, NVFP4;
 // kernels of 16, 32 and 64 rows as the MMA's N, of 128 as
 // its M, and of 256 as that of two CTAs; weights from HBM):
-//   one matrix 4096 x 4096: 8.7 / 9.2 / 9.9 / 9.9 / 12.5 at 1 row, 9.6 / 9.9 / 11.1 / 10.1 / 12.5 at 64, 14.3 / 10.0 /
-//   11.2 / 10.4 / 12.8 at 96, - / 15.2 / 11.5 / 10.4 / 13.0 at 192, - / - / 17.1 / 11.1 / 13.4 at 512, - / - / - / 16.5 /
-//   13.5 at 768: a tile of fewer rows or columns gives more CTAs, so the smallest whose tiles run in one wave, and pairs
-//   where no kernel's do. 2816 x 2048: - / - / - / 8.0 / 9.4 at 768 (132 tiles of 128), 10.5 / 9.7 at 1024 (176). The
-//   64-row kernel never leads there.
+//   one matrix 4096 x 4096: 8.7 / 9.2 / 10.0 / 10.5 / 12.7 at 1 row, 9.0 / 9.7 / 10.9 / 10.0 / 12.3 at 64, 13.8 / 9.8 /
+//   10.9 / 10.1 / 12.4 at 96, 18.7 / 14.9 / 11.0 / 10.1 / 12.7 at 192, - / 24.7 / 16.7 / 10.3 / 12.8 at 512, - / - / 21.9 /
+//   16.0 / 12.9 at 768: a tile of fewer rows or columns gives more CTAs, so the smallest whose tiles run in one wave, and
+//   pairs where no kernel's do. 2816 x 2048: - / - / 11.5 / 7.1 / 8.7 at 768 (132 tiles of 128), 14.4 / 9.7 / 8.8 at 1024
+//   (176). The 64-row kernel never leads there.
 //   64 matrices 2816 x 2048: 46.6 / 40.7 / 40.6 / 46.7 / 54.0 at 16 rows each, 66.6 / 55.6 / 41.9 / 45.9 / 55.4 at 32,
 //   102 / 58.7 / 45.7 / 48.1 / 55.7 at 48, - / 70.7 / 62.8 / 46.2 / 56.2 at 64, - / 108 / 72.8 / 47.1 / 57.1 at 96, 131 /
-//   78.2 / 60.6 (the last three) at 192: an expert above a tile's rows reads its weights twice, and rows are drawn about
-//   their mean. 384 matrices 4096 x 4096: 555 / 554 / 616 at 8, 1070 / 601 / 643 / 737 / 839 at 24, 1875 / 1112 / 671 /
-//   848 / 962 at 48, - / - / 1633 / 1225 / 885 at 128: there 20 is before the crossing (7 % at 24).
+//   78.2 / 60.6 (the last three) at 192 (the last kernel by 6 us more in every other run): an expert above a tile's rows
+//   reads its weights twice, and rows are drawn about their mean. 384 matrices 4096 x 4096: 555 / 554 / 616 at 8, 1070 /
+//   601 / 643 / 737 / 839 at 24, 1875 / 1112 / 671 / 848 / 962 at 48, - / - / 1633 / 1225 / 885 at 128: there 20 is before
+//   the crossing (7 % at 24).
 //   S counts rows without an expert too, and no spread is known here.
 // Returns 8 (fp4_skinny.cu), 16, 32, 64, 128 or 256.
 int choose(const Fp4Product& p) {
@@ -431,8 +433,8 @@ extern "C" int b200moe_fp4_linear(void* stream, const void* x, int x_dtype, int6
   if (!x || ldx < 0) return B200MOE_ERR_INVALID_ARG;
   if (x_dtype < 0 || x_dtype > B200MOE_F32) return B200MOE_ERR_DTYPE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t ld_bytes = ldx * (x_dtype == B200MOE_F32 ? 4 : 2);
-  if (choose(p) == 8 && fp4_skinny_quantizes(S, K) && x_dtype != B200MOE_F32 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_bytes % 16 == 0)
+  const bool wide = x_dtype != B200MOE_F32 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0;
+  if (wide && choose(p) == 8 && fp4_skinny_quantizes(S, K))
     return launch_status(launch_fp4_skinny(s, p, x, x_dtype, ldx, out_dtype));
   if (!workspace || workspace_bytes < size_t(S) * b200moe_fp4_record_bytes(format, K)) return B200MOE_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return B200MOE_ERR_ALIGN;

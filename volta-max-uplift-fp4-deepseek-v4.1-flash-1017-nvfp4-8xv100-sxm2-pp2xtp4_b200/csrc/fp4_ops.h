@@ -27,8 +27,8 @@ int launch_fp4_tiles(cudaStream_t s, const Fp4Product& p, int out_dtype);
 int launch_fp4_pairs(cudaStream_t s, const Fp4Product& p, int out_dtype);
 // the same with the weights as the MMA's M, for few rows per matrix: tiles of 16, 32 or 64 rows x 128 columns
 int launch_fp4_stream(cudaStream_t s, const Fp4Product& p, int rows_per_tile, int out_dtype);
-// kernel for one matrix and few rows, NVFP4 eight at most, MXFP4 three (fp4_skinny.cu): records, or rows x of f16 or bf16 (stride ldx)
-// that it quantizes itself
+// kernel for one matrix and few rows, NVFP4 eight at most, MXFP4 three (fp4_skinny.cu): records, or rows x of f16 or bf16
+// (stride ldx) that it quantizes itself
 int launch_fp4_skinny(cudaStream_t s, const Fp4Product& p, const void* x, int x_dtype, int64_t ldx, int out_dtype);
 // whether its rows fit in shared memory and its CTAs run in one wave
 bool fp4_skinny_fits(const Fp4Product& p);

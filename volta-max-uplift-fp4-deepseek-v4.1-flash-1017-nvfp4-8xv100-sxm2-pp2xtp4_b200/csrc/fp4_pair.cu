@@ -99,15 +99,16 @@ __device__ __forceinline__ bool poll_cluster(uint64_t* bar, uint32_t parity, uin
 // Into this CTA's shared memory, counted on a barrier of the pair.
 __device__ __forceinline__ void tma_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          smem_u32(dst)),
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
 // At the same place in both CTAs, when the MMAs and copies issued so far are done.
 __device__ __forceinline__ void commit_pair(uint64_t* bar) {
   asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(smem_u32(bar)),
       "h"(uint16_t(3))
       : "memory");
 }
@@ -267,8 +268,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       constexpr int kTileOut = 32 * kTile * int(sizeof(TO));  // of a warp
       static_assert(4 * kTileOut <= kStages * kStage, "the last tile's room");
       const bool last = tiles.next(item) >= tiles.stop();
-      store_tile<kTile, TO>(a, &maps.out, lanes + b * kAcc1, last ? stages + quarter * kTileOut : stage_out + quarter * kOutBytes,
-                            row0, end, col0, f, b ? 0 : kAcc1 / 32, kSharedCols / 32, last, [&] { arrive_at(bar); });
+      uint8_t* mine = last ? stages + quarter * kTileOut : stage_out + quarter * kOutBytes;
+      store_tile<kTile, TO>(a, &maps.out, lanes + b * kAcc1, mine, row0, end, col0, f, b ? 0 : kAcc1 / 32,
+                            kSharedCols / 32, last, [&] { arrive_at(bar); });
     }
     if (!ok) *abort_ptr = 1;
     if (lane == 0) tma_stores_done();
@@ -331,7 +333,8 @@ int launch_one(cudaStream_t s, const TileArgs& a, const TileMaps& m, int64_t til
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -1;
   auto kernel = fp4_pair_kernel<FMT, TO>;
   if (!(attr_set.load() >> dev & 1)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg<FMT>::kSmem)) != cudaSuccess) return -1;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg<FMT>::kSmem)) != cudaSuccess)
+      return -1;
     attr_set.fetch_or(uint64_t(1) << dev);
   }
   if (!pairs.load()) pairs.store(resident_pairs(kernel, Cfg<FMT>::kSmem));
@@ -344,7 +347,8 @@ int launch_one(cudaStream_t s, const TileArgs& a, const TileMaps& m, int64_t til
 int launch_fp4_pairs(cudaStream_t s, const Fp4Product& p, int out_dtype) {
   TileArgs a{};
   TileMaps m{};
-  if (make_tile_args(p, out_dtype, kHalf, kHalf, kHalf, kTile, p.format == kMx ? Cfg<kMx>::kChunkRow : Cfg<kNv>::kChunkRow, true, a, m)) return -1;
+  const int chunk_row = p.format == kMx ? Cfg<kMx>::kChunkRow : Cfg<kNv>::kChunkRow;
+  if (make_tile_args(p, out_dtype, kHalf, kHalf, kHalf, kTile, chunk_row, true, a, m)) return -1;
   // upper bound of the row tiles: one per 256 rows and one more for every expert with rows
   const int64_t row_tiles = p.offsets ? int64_t(p.S) / kTile + std::min(p.E, p.S) : (p.S + kTile - 1) / kTile;
   const int64_t tiles = row_tiles * ((p.N + kTile - 1) / kTile);

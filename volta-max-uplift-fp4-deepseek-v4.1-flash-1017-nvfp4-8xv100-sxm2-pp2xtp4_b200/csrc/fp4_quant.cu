@@ -46,9 +46,9 @@ struct Piece {
 // A warp per row, its columns in registers as N pieces of 16 a lane: no barrier, for as many rows as keep the GPU's warps
 // busy.
 template <typename T, bool SWIGLU, bool WIDE, int N>
-__global__ void __launch_bounds__(256, N <= 3 ? 3 : 2) nvfp4_warp_rows_kernel(const T* __restrict__ x, int64_t x_stride, int rows,
-                                                                            int width, float limit,
-                                                                            uint8_t* __restrict__ out) {
+__global__ void __launch_bounds__(256, N <= 3 ? 3 : 2)
+    nvfp4_warp_rows_kernel(const T* __restrict__ x, int64_t x_stride, int rows, int width, float limit,
+                           uint8_t* __restrict__ out) {
   const int lane = threadIdx.x & 31;
   const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
   pdl_wait();
@@ -84,9 +84,9 @@ __global__ void __launch_bounds__(256, N <= 3 ? 3 : 2) nvfp4_warp_rows_kernel(co
 
 // A CTA walks rows. Where its threads hold all of a row (once), the next row is on its way while this one is worked on.
 template <typename T, bool SWIGLU, bool WIDE>
-__global__ void __launch_bounds__(kMaxRowThreads, sizeof(T) == 2 ? 2 : 1) nvfp4_rows_kernel(const T* __restrict__ x, int64_t x_stride, int rows,
-                                                                    int width, float limit,
-                                                                    uint8_t* __restrict__ out) {
+__global__ void __launch_bounds__(kMaxRowThreads, sizeof(T) == 2 ? 2 : 1)
+    nvfp4_rows_kernel(const T* __restrict__ x, int64_t x_stride, int rows, int width, float limit,
+                      uint8_t* __restrict__ out) {
   __shared__ uint32_t warp_max[2][kMaxRowThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x, threads = blockDim.x;
   const int pieces = width / 16;
@@ -328,7 +328,8 @@ cudaError_t run_rows(cudaStream_t s, int fmt, const void* x, int64_t x_stride, i
   const int pieces = width / 16, per_lane = (pieces + 31) / 32;
   if (per_lane == 1 || (per_lane <= 4 && rows >= 8 * sm_count())) {
     auto go = [&](auto kernel) {
-      return launch_chain(kernel, dim3(unsigned((int64_t(rows) + 7) / 8)), dim3(256), 0, s, src, x_stride, rows, width, limit, out);
+      const dim3 grid(unsigned((int64_t(rows) + 7) / 8));
+      return launch_chain(kernel, grid, dim3(256), 0, s, src, x_stride, rows, width, limit, out);
     };
     if (per_lane == 1)
       return wide ? go(nvfp4_warp_rows_kernel<T, SWIGLU, true, 1>) : go(nvfp4_warp_rows_kernel<T, SWIGLU, false, 1>);

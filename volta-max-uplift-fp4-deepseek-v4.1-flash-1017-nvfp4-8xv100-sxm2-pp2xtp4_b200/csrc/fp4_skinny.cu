@@ -1,6 +1,7 @@
 // 4-bit products of at most eight rows with one matrix: the weights go straight from
 // global memory into the registers of the warps that multiply them. One launch does
-// it all: up to 4096 values of f16 or bf16 rows (one row of 4096 columns, eight of 512) are quantized by every CTA for itself.
+// it all: up to 4096 values of f16 or bf16 rows (one row of 4096 columns, eight of
+// 512) are quantized by every CTA for itself.
 //
 // A warp owns 16 weight rows and every KS-th block of 256 columns.  NVFP4: each lane
 // loads four 16-byte pieces per block (32 columns each: rows g and g + 8, pieces q and q + 4; g =
@@ -14,10 +15,14 @@
 // shared memory in a fixed order.
 //
 // Bound: latency, and above a few rows the rows' way into every CTA's shared memory: all
-// of a small matrix is in flight at once. 4096 x 4096: NVFP4 5.5 us at one row, 6.7 at
-// four, 8.5 at eight, where the streaming kernel takes 8.7 to 8.9; MXFP4 7.5, 9.2 and
-// 11.5 (8.5 to 8.9), so three rows at most. 2816 x 2048: 3.6 and 4.6 at one row (5.7).
-// Taken as long as all CTAs, of 16 or 32 weight rows, run at once.
+// of a small matrix is in flight at once. 4096 x 4096: NVFP4 5.4 us at one row, 6.7 at
+// four, 8.5 at eight, where the streaming kernel takes 8.7 to 8.8; MXFP4 7.6, 8.2 at two,
+// 8.7 at three, 9.3 at four (8.6), so three rows at most. 2816 x 2048: 3.8 and 4.6 at one
+// row (5.5).  Taken as long as all CTAs, of 16 or 32 weight rows, run at once: to N 4736
+// at K above 2048 (5.5 us, one row NVFP4). Past it tiles of 128 weight rows give 38 CTAs
+// and more: 8.8 us at N 4864, 9.4 at 8192, 9.8 at 11008, where the bytes take 1.7, 2.9
+// and 3.9. Longer K runs block after block, two in flight: one row x 4096 x 7168 8.2 us
+// (2.6), x 14336 14.3 (5.1), eight rows 12.2 and, streamed, 20.3.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -58,9 +63,9 @@ __device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {  // weights: read
                : "l"(p));
   return v;
 }
-// 16 columns of a row, as codes, times scale to shared memory as f16.  The codes' values come from their bits: ptxas 12.9
-// joins cvt.rn.f16x2.e2m1x2 with the conversion that made the codes in the same thread, and takes a wrong byte of it (rows
-// came out as zeros).
+// 16 columns of a row, as codes, times scale to shared memory as f16.  The codes' values come from their bits: with
+// cvt.rn.f16x2.e2m1x2 of bytes that the same thread had just converted (CUDA 12.9), rows came out as zeros, while rows whose
+// codes were loaded came out right; why was not found.
 __device__ __forceinline__ void put_tokens(uint8_t* dst, uint2 codes, float scale) {
   const __half2 s = __float2half2_rn(scale);
 #pragma unroll
@@ -210,7 +215,8 @@ __global__ void __launch_bounds__(kThreads, 2) nvfp4_skinny_kernel(const SkinnyA
           const bool in = g < A.S && piece * 32 < A.K;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {  // eight columns of this lane: two MMAs of 16 columns
-            const uint4 x = in ? *reinterpret_cast<const uint4*>(mine + piece * piece_bytes(kNv) + i * 16) : make_uint4(0, 0, 0, 0);
+            const uint8_t* from = mine + piece * piece_bytes(kNv) + i * 16;
+            const uint4 x = in ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
             uint32_t a[4], b[4];
             e2m1x8_scaled(lo[i], i < 2 ? lo_half2(ml) : hi_half2(ml), a);
             e2m1x8_scaled(hi[i], i < 2 ? lo_half2(mh) : hi_half2(mh), b);
@@ -360,7 +366,8 @@ int launch_format(cudaStream_t s, const SkinnyArgs& a, int format, int out_dtype
 }  // namespace
 
 bool fp4_skinny_fits(const Fp4Product& p) {
-  if (p.E != 1 || p.offsets || p.S > (p.format == kMx ? 3 : kTokens) || reinterpret_cast<uintptr_t>(p.w_scale) % 2) return false;
+  const int most = p.format == kMx ? 3 : kTokens;
+  if (p.E != 1 || p.offsets || p.S > most || reinterpret_cast<uintptr_t>(p.w_scale) % 2) return false;
   const size_t smem = skinny_smem(p.format, p.S, p.K);
   return smem <= kSmemMost && skinny_grid(p.N, p.K) <= sm_count() * (smem <= 100 * 1024 ? 2 : 1);
 }

@@ -156,8 +156,9 @@ struct ScaleWay {
 constexpr int kScaleWarps = 4;  // and buffers: warp w puts every fourth stage into buffer w
 // With one warp for all stages one row x 4096 x 4096 took 8.4 us.
 
-// Warp w's walk over the tiles' stages.  CR: bytes of a row in a chunk, 32 or 64; BLOCKS: 128 rows of the MMA's M, then of its N; SWAP: the weights are M.  W 16:
-// all scales from the chunks; else the weights' by loads of W bytes (row w_row(item) of a tile, four stages ahead).
+// Warp w's walk over the tiles' stages.  CR: bytes of a row in a chunk, 32 or 64; BLOCKS: 128 rows of the MMA's M, then
+// of its N; SWAP: the weights are M.  W 16: all scales from the chunks; else the weights' by loads of W bytes (row
+// w_row(item) of a tile, four stages ahead).
 // arrive(w) tells the MMA warp that buffer w holds a stage.
 template <int FMT, int W, int CR, int BLOCKS, bool SWAP, typename RowOf, typename Arrive>
 __device__ __forceinline__ void scale_warp(int w, const TileArgs& a, const Tiles& tiles, const ScaleWay& way,
@@ -297,8 +298,9 @@ __device__ __forceinline__ void scale_warp_by(int w, const TileArgs& a, const Ti
 // expert's rows.  roomy: the CTA's last tile, whose pieces find room of their own at `mine` and none waits for the one
 // before to leave (the ring of stages, which is done with).
 template <int BN, typename TO, typename Free>
-__device__ __forceinline__ void store_tile(const TileArgs& a, const CUtensorMap* map_out, uint32_t acc, uint8_t* mine, int row0,
-                                           int end, int col0, Fp4Factors f, int first, int release, bool roomy, const Free& free) {
+__device__ __forceinline__ void store_tile(const TileArgs& a, const CUtensorMap* map_out, uint32_t acc, uint8_t* mine,
+                                           int row0, int end, int col0, Fp4Factors f, int first, int release, bool roomy,
+                                           const Free& free) {
   constexpr int PW = 64 / int(sizeof(TO)), CW = 16 / int(sizeof(TO));  // columns per piece, per 16-byte chunk
   const int lane = threadIdx.x & 31;
   TO* out = static_cast<TO*>(a.out);

@@ -23,6 +23,11 @@
 // (5.5). What held it back was instructions: 41 per value forward and 56 backward by
 // single conversions and sums read one by one, 109 (NVFP4) and 187 us. The gradient
 // with its weights and the sum's gradient a row ahead in registers too: 115, spilled.
+// Wider rows hold two or four pieces per thread, and one CTA per SM leaves few warps
+// for the memory's latency (5120 columns: 176 registers, 8 % of the warps): the same 67
+// million values take, in rows / E4M3 / NVFP4 / MXFP4 / gradient, 137 / 160 / 191 / 99 / 198 us
+// at 5120 columns, 111 / 125 / 153 / 125 / 160 at 7168, 104 / 115 / 145 / 114 / 149 at 8192, 109 /
+// 130 / 146 / 126 / 198 to 208 at 12288 and 96 / 111 / 126 / 107 / 166 to 174 at 16384.
 #include <algorithm>
 
 #include "fp4_rows.cuh"
@@ -174,7 +179,9 @@ struct NormArgs {
 // CTAs per SM that the registers have to leave room for. f32 rows hold twice the registers of 16-bit ones ahead: 8192 x
 // 4096 take 105 us with two CTAs and 118 with three, E4M3 81 and 97, 8192 x 2001 E4M3 36 and 67; NVFP4 100 and 97.
 // E4M3 of 16-bit rows with an f32 residual, one column at a time, 16384 x 3999: 166 and 251 (rows 150 and 139; with a
-// 16-bit residual E4M3 of 16384 x 2001 90 and 87).
+// 16-bit residual E4M3 of 16384 x 2001 90 and 87). Two pieces per thread take one: with two, 16-bit rows of 5120
+// to 8192 columns take less (rows 83, NVFP4 91 to 99, MXFP4 77 to 83 us; the gradient 152 at 5120 and the same above), f32
+// rows more (7168: 217 and 243, gradient 258 and 278).
 template <typename T, typename TR, int OUT, bool WIDE, int C>
 __host__ __device__ constexpr int norm_ctas() {
   if (C > 1) return 1;

@@ -65,7 +65,8 @@ class Rows(NamedTuple):
 
 class Weights(NamedTuple):
     """``codes`` uint8 [(E,) N, K / 2]; ``scale`` uint8 [(E,) N, K / 16] (E4M3) and ``factor`` f32 [E]
-    ([1] for one matrix) for NVFP4, ``scale`` [(E,) N, K / 32] (E8M0) and no factor for MXFP4."""
+    ([1] for one matrix) for NVFP4, ``scale`` [(E,) N, K / 32] (E8M0) and no factor for MXFP4.  Scales have
+    no sign: the products take a set sign bit of E4M3 as they like."""
 
     codes: torch.Tensor
     scale: torch.Tensor

@@ -5,7 +5,9 @@ for the product that follows, and its gradient.
     y = s / sqrt(mean(s^2) + eps) * weight
 
 The residual and the weight have x's type or f32 (a residual stream kept in f32), sums are in
-f32, and equal inputs give equal bits, gradients included.  ``rms_norm`` takes part in autograd
+f32, and equal inputs give equal bits, gradients included.  Quantized rows may differ from another
+f32 form's by a step of a code: a quotient of y and its block's maximum does not depend on the root,
+so exact ties of 16-bit rows (one value in some thousands) fall by how each form rounded it.  ``rms_norm`` takes part in autograd
 in x, weight and residual; the gradient of ``sum`` joins in the same pass.  Rows have 1 to
 16384 columns at any distance.  Arguments that do not fit raise ``ValueError``.
 """
